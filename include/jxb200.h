@@ -484,6 +484,80 @@ int jx_comm_layout(long long max_floats, int world, long long* out10);
 int jx_allreduce_f32(void* const* bases, int rank, int world, long long max_floats, int which, long long n,
                      float* out, int* status, int pdl, void* stream);
 
+/* ---- paged 4-bit KV cache (no counterpart in the reference, whose cache is dense: cache.py:69-282) ----
+ *
+ * Pages of 64 tokens.  The block of one (layer, page, KV head) is one contiguous run of 64 * hd + 8 * hd bytes:
+ * key codes [64][hd / 2], value codes [64][hd / 2], key scales [64][hd / 32] bfloat16, value scales [64][hd / 32]
+ * bfloat16.  Channel 2j of a token is the low nibble of byte j, channel 2j + 1 the high one; a value is
+ * (nibble - 8) * scale of its 32 channels.  scale = amax / 7 to 4 significant bits (nearest even), nibble = 8 +
+ * clamp(round(x / scale), -7, 7); a group of magnitude 2^122 or more, or not finite, decodes to NaN.
+ *
+ * Device errors (a row past its table, a pool without free pages, a parent or page out of range) set *status to
+ * JX_ERR_RANGE; nothing is read or written out of range.  hd is 64, 128 or 256; at most 8192 rows. */
+#define JX_KV4_PAGE 64
+typedef struct jx_kv4_cache {
+  unsigned char* pages;  /* [num_layers][num_pages][num_kv_heads][72 * head_dim], 16-byte aligned */
+  int* table;            /* [num_rows][row_pages] page ids, -1: none */
+  int* lengths;          /* [num_rows] tokens held, the current call's among them */
+  int* counts;           /* [num_rows] tokens of the current call: the last counts[r] of the row */
+  int* refs;             /* [num_pages] rows that hold the page */
+  int* status;           /* device status word */
+  int num_layers, num_pages, num_rows, row_pages, num_kv_heads, head_dim;
+} jx_kv4_cache;
+
+/* Writes keys and values [num_rows, S, num_kv_heads, hd] (element strides of the first three axes; the last is
+ * dense): token i < counts[r] of row r goes to position lengths[r] - counts[r] + i of the layer.  Tokens behind
+ * counts[r] are not read. */
+int jx_kv4_append(const jx_kv4_cache* cache, int layer, int S, const void* k, long long k_row, long long k_tok,
+                  long long k_head, const void* v, long long v_row, long long v_tok, long long v_head, int dtype,
+                  void* stream);
+/* The dequantised keys and values [num_rows, n, num_kv_heads, hd] of positions (start ? start[r] : 0) + start_add + i;
+ * zeros outside the row. */
+int jx_kv4_read(const jx_kv4_cache* cache, int layer, const int* start, int start_add, int n, void* k, void* v, int dtype,
+                void* stream);
+/* Attention of queries [num_rows, S, Hq, hd] (element strides; last axis dense) over a layer's pages.  Query i <
+ * counts[r] stands at position p = lengths[r] - counts[r] + i and sees positions <= p, with window > 0 those above p -
+ * window; float32 softmax of scale * q.k.  Query head h reads KV head h / (Hq / num_kv_heads).  out: dense
+ * [num_rows, S, Hq, hd]; rows of queries behind counts[r] are zero.  ws: jx_kv4_attend_workspace bytes, 16-byte
+ * aligned, used by this call alone until it has finished. */
+int jx_kv4_attend_workspace(const jx_kv4_cache* cache, int S, int Hq, int dtype, long long* bytes);
+int jx_kv4_attend(const jx_kv4_cache* cache, int layer, int S, int Hq, const void* q, long long q_row, long long q_tok,
+                  long long q_head, void* out, float scale, int window, void* ws, long long ws_bytes, int dtype,
+                  void* stream);
+/* Room for counts[r] (or count, when counts is NULL) more tokens of every row: lengths grow, counts become the current
+ * call's, new pages are the lowest free ones, and a shared page that a row will write on is copied first in every
+ * layer.  All or nothing: without room the status word is set, counts become zero and all else stays.  ws:
+ * jx_kv4_workspace_ints ints, used by this call alone until it has finished (jx_kv4_compact too). */
+int jx_kv4_workspace_ints(const jx_kv4_cache* cache, long long* ints);
+int jx_kv4_extend(const jx_kv4_cache* cache, const int* counts, int count, int* ws, long long ws_ints, void* stream);
+/* Every row r takes what row parents[r] held before the call (pages are shared, nothing is copied); parents[r] < 0
+ * empties it, parents[r] >= num_rows sets the status word and leaves it. */
+int jx_kv4_fork(const jx_kv4_cache* cache, const int* parents, void* stream);
+/* Every row loses its last n[r] (or n_all, when n is NULL) tokens; a row with fewer stays and the status word is set. */
+int jx_kv4_rollback(const jx_kv4_cache* cache, const int* n, int n_all, void* stream);
+/* Rows with a non-zero byte are emptied. */
+int jx_kv4_free(const jx_kv4_cache* cache, const unsigned char* rows, void* stream);
+/* Moves the used pages to the front of the pool in every layer and renumbers the tables; *used: the used pages. */
+int jx_kv4_compact(const jx_kv4_cache* cache, int* used, int* ws, long long ws_ints, void* stream);
+
+/* ---- scoring (beside the filters and draws of inference_engine/sampling.py:34-188) ----
+ * Of every logits row x [V]: log_probs = x[id] - log sum exp x (0 for a negative id, NaN for id >= V), entropy of
+ * softmax(x), and the top_n largest entries' ids (equal values: lowest id first) with their log probabilities.  Entries
+ * of -inf have probability 0; a row with NaN or +inf, or without a finite entry, has NaN results and the ids that its
+ * order gives.  top_n <= 64 and <= V. */
+typedef struct jx_log_probs_args {
+  int rows, V;
+  const void* logits;
+  long long ld;          /* elements between rows */
+  int dtype, top_n;
+  const int* ids;        /* [rows] */
+  float* log_probs;      /* [rows] */
+  float* entropy;        /* [rows] */
+  float* top_log_probs;  /* [rows, top_n] */
+  int* top_ids;          /* [rows, top_n] */
+} jx_log_probs_args;
+int jx_token_log_probs(const jx_log_probs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

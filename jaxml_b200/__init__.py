@@ -11,6 +11,7 @@ from .config import ModelConfig
 from .engine import Engine, InferenceConfig
 from .models import (GemmaModel, GemmaModelWithHead, GPTNeoXModel, GPTNeoXModelWithHead, LlamaModel,
                      LlamaModelWithHead)
+from .paged_cache import PagedKVCache
 from .sampling import SamplingMethod
 from .text_generation import GenerationConfig, TextGenerationPipeline
 
@@ -22,6 +23,7 @@ __all__ = [
     "GenerationConfig",
     "TextGenerationPipeline",
     "KVCache",
+    "PagedKVCache",
     "LlamaModelWithHead",
     "GPTNeoXModelWithHead",
     "GemmaModelWithHead",

@@ -92,6 +92,17 @@ class JxFilterArgs(ctypes.Structure):
                 ("top_k", I), ("top_p", F), ("min_p", F)]
 
 
+class JxKv4Cache(ctypes.Structure):
+    _fields_ = [("pages", P), ("table", P), ("lengths", P), ("counts", P), ("refs", P), ("status", P),
+                ("num_layers", I), ("num_pages", I), ("num_rows", I), ("row_pages", I), ("num_kv_heads", I),
+                ("head_dim", I)]
+
+
+class JxLogProbsArgs(ctypes.Structure):
+    _fields_ = [("rows", I), ("V", I), ("logits", P), ("ld", LL), ("dtype", I), ("top_n", I), ("ids", P),
+                ("log_probs", P), ("entropy", P), ("top_log_probs", P), ("top_ids", P)]
+
+
 class JxStepArgs(ctypes.Structure):
     _fields_ = [("M", I), ("L", I), ("d", I), ("Hq", I), ("Hkv", I), ("hd", I), ("F", I), ("V", I), ("vocab", I),
                 ("T", I), ("rd", I), ("max_pos", I), ("Np_qkv", LL), ("Np_d", LL), ("Np_gu", LL), ("Np_v", LL),
@@ -129,6 +140,17 @@ _PROTOS = {
     "jx_prefill_attention": (I, [ctypes.POINTER(JxPAttnArgs), I, P]),
     "jx_sample": (I, [ctypes.POINTER(JxSampleArgs), I, P]),
     "jx_filter_logits": (I, [ctypes.POINTER(JxFilterArgs), P]),
+    "jx_kv4_append": (I, [ctypes.POINTER(JxKv4Cache), I, I, P, LL, LL, LL, P, LL, LL, LL, I, P]),
+    "jx_kv4_read": (I, [ctypes.POINTER(JxKv4Cache), I, P, I, I, P, P, I, P]),
+    "jx_kv4_attend_workspace": (I, [ctypes.POINTER(JxKv4Cache), I, I, I, ctypes.POINTER(LL)]),
+    "jx_kv4_attend": (I, [ctypes.POINTER(JxKv4Cache), I, I, I, P, LL, LL, LL, P, F, I, P, LL, I, P]),
+    "jx_kv4_workspace_ints": (I, [ctypes.POINTER(JxKv4Cache), ctypes.POINTER(LL)]),
+    "jx_kv4_extend": (I, [ctypes.POINTER(JxKv4Cache), P, I, P, LL, P]),
+    "jx_kv4_fork": (I, [ctypes.POINTER(JxKv4Cache), P, P]),
+    "jx_kv4_rollback": (I, [ctypes.POINTER(JxKv4Cache), P, I, P]),
+    "jx_kv4_free": (I, [ctypes.POINTER(JxKv4Cache), P, P]),
+    "jx_kv4_compact": (I, [ctypes.POINTER(JxKv4Cache), P, P, LL, P]),
+    "jx_token_log_probs": (I, [ctypes.POINTER(JxLogProbsArgs), P]),
     "jx_decode_step": (I, [ctypes.POINTER(JxStepArgs), P]),
     "jx_set_decode_step_lookahead": (I, [I]),
     "jx_sample_finalize": (I, [ctypes.POINTER(JxSampleArgs), P, I, P]),

@@ -379,3 +379,160 @@ int jx_allreduce_f32(void* const* bases, int rank, int world, long long max_floa
 }
 
 }  // extern "C"
+
+// ------------------------------------------------------------------------------------------------
+// paged 4-bit KV cache and scoring
+// ------------------------------------------------------------------------------------------------
+namespace jxb {
+int run_kv4_append(const jx_kv4_cache& c, int layer, int S, const void* k, const void* v, const long long* ks,
+                   const long long* vs, int dtype, cudaStream_t s);
+int run_kv4_read(const jx_kv4_cache& c, int layer, const int* start, int start_add, int n, void* k, void* v, int dtype,
+                 cudaStream_t s);
+long long kv4_workspace_ints(int rows, int pages);
+int run_kv4_extend(const jx_kv4_cache& c, const int* counts, int count, int* ws, cudaStream_t s);
+int run_kv4_compact(const jx_kv4_cache& c, int* used, int* ws, cudaStream_t s);
+int run_kv4_fork(const jx_kv4_cache& c, const int* parents, cudaStream_t s);
+int run_kv4_shorten(const jx_kv4_cache& c, const unsigned char* rows, const int* n, int n_all, cudaStream_t s);
+long long kv4_attend_workspace(const jx_kv4_cache& c, int S, int Hq, int dtype);
+int run_kv4_attend(const jx_kv4_cache& c, int layer, int S, int Hq, const void* q, const long long* qs, void* out,
+                   float scale, int window, void* ws, int dtype, cudaStream_t s);
+int run_token_log_probs(const jx_log_probs_args& a, cudaStream_t s);
+
+// The checks every call on a cache makes; a message on failure.
+static const char* kv4_bad(const jx_kv4_cache* c, int* code) {
+  *code = JX_ERR_ARG;
+  if (!c) return "null cache";
+  if (!c->pages || !c->table || !c->lengths || !c->counts || !c->refs || !c->status) return "null cache pointer";
+  if ((uintptr_t)c->pages & 15) return "pages must be 16-byte aligned";
+  *code = JX_ERR_SHAPE;
+  if (c->num_layers <= 0 || c->num_pages <= 0 || c->num_rows <= 0 || c->row_pages <= 0 || c->num_kv_heads <= 0)
+    return "cache sizes must be positive";
+  if (c->num_rows > 8192) return "at most 8192 rows";
+  if (c->row_pages > (1 << 24)) return "at most 2^24 pages per row";
+  if (c->num_pages > (1 << 28) || c->num_kv_heads > 4096) return "at most 2^28 pages and 4096 KV heads";
+  if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return "head_dim must be 64, 128 or 256";
+  return nullptr;
+}
+
+static int kv4_fail(int code, const char* where, const char* msg) {
+  snprintf(g_err, sizeof(g_err), "%s: %s", where, msg);
+  return code;
+}
+
+static int kv4_done(int rc, const char* where) { return rc == JX_ERR_CUDA ? note_cuda(where) : rc; }
+}  // namespace jxb
+
+#define KV4_CHECK(where)                                                   \
+  int bad_code;                                                            \
+  if (const char* bad_msg = kv4_bad(cache, &bad_code)) return kv4_fail(bad_code, where, bad_msg)
+
+extern "C" {
+
+int jx_kv4_append(const jx_kv4_cache* cache, int layer, int S, const void* k, long long k_row, long long k_tok,
+                  long long k_head, const void* v, long long v_row, long long v_tok, long long v_head, int dtype,
+                  void* stream) {
+  KV4_CHECK("jx_kv4_append");
+  if (!k || !v) return fail(JX_ERR_ARG, "jx_kv4_append: null keys or values");
+  if (layer < 0 || layer >= cache->num_layers || S <= 0) return fail(JX_ERR_SHAPE, "jx_kv4_append: layer out of range, or S < 1");
+  if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_append: float32 or bfloat16");
+  const uintptr_t size = dtype == JX_BF16 ? 2 : 4;
+  if ((uintptr_t)k % size || (uintptr_t)v % size) return fail(JX_ERR_ARG, "jx_kv4_append: misaligned keys or values");
+  const long long ks[3] = {k_row, k_tok, k_head}, vs[3] = {v_row, v_tok, v_head};
+  return kv4_done(run_kv4_append(*cache, layer, S, k, v, ks, vs, dtype, (cudaStream_t)stream), "jx_kv4_append");
+}
+
+int jx_kv4_read(const jx_kv4_cache* cache, int layer, const int* start, int start_add, int n, void* k, void* v, int dtype,
+                void* stream) {
+  KV4_CHECK("jx_kv4_read");
+  if (!k || !v || ((uintptr_t)k & 15) || ((uintptr_t)v & 15))
+    return fail(JX_ERR_ARG, "jx_kv4_read: outputs must be 16-byte aligned");
+  if (layer < 0 || layer >= cache->num_layers || n <= 0) return fail(JX_ERR_SHAPE, "jx_kv4_read: layer out of range, or n < 1");
+  if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_read: float32 or bfloat16");
+  return kv4_done(run_kv4_read(*cache, layer, start, start_add, n, k, v, dtype, (cudaStream_t)stream), "jx_kv4_read");
+}
+
+int jx_kv4_attend_workspace(const jx_kv4_cache* cache, int S, int Hq, int dtype, long long* bytes) {
+  KV4_CHECK("jx_kv4_attend_workspace");
+  if (!bytes) return fail(JX_ERR_ARG, "jx_kv4_attend_workspace: null output");
+  if (S <= 0 || Hq <= 0 || Hq % cache->num_kv_heads)
+    return fail(JX_ERR_SHAPE, "jx_kv4_attend_workspace: S >= 1, Hq a multiple of the KV heads");
+  *bytes = kv4_attend_workspace(*cache, S, Hq, dtype);
+  return JX_OK;
+}
+
+int jx_kv4_attend(const jx_kv4_cache* cache, int layer, int S, int Hq, const void* q, long long q_row, long long q_tok,
+                  long long q_head, void* out, float scale, int window, void* ws, long long ws_bytes, int dtype,
+                  void* stream) {
+  KV4_CHECK("jx_kv4_attend");
+  if (!q || !out || !ws || ((uintptr_t)out & 15) || ((uintptr_t)ws & 15))
+    return fail(JX_ERR_ARG, "jx_kv4_attend: null pointer, or out / ws not 16-byte aligned");
+  if (layer < 0 || layer >= cache->num_layers || S <= 0 || window < 0)
+    return fail(JX_ERR_SHAPE, "jx_kv4_attend: layer out of range, S < 1 or window < 0");
+  if (Hq <= 0 || Hq % cache->num_kv_heads || Hq > 65535)
+    return fail(JX_ERR_SHAPE, "jx_kv4_attend: Hq must be a multiple of the KV heads, at most 65535");
+  if ((long long)cache->num_rows * S > 0x7FFFFFFF) return fail(JX_ERR_SHAPE, "jx_kv4_attend: rows * S must be below 2^31");
+  if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_attend: float32 or bfloat16");
+  if ((uintptr_t)q % (dtype == JX_BF16 ? 2 : 4)) return fail(JX_ERR_ARG, "jx_kv4_attend: misaligned queries");
+  if (!(scale > -1e30f && scale < 1e30f)) return fail(JX_ERR_ARG, "jx_kv4_attend: scale must be finite");
+  if (ws_bytes < kv4_attend_workspace(*cache, S, Hq, dtype)) return fail(JX_ERR_ARG, "jx_kv4_attend: workspace too small");
+  const long long qs[3] = {q_row, q_tok, q_head};
+  return kv4_done(run_kv4_attend(*cache, layer, S, Hq, q, qs, out, scale, window, ws, dtype, (cudaStream_t)stream),
+                  "jx_kv4_attend");
+}
+
+int jx_kv4_workspace_ints(const jx_kv4_cache* cache, long long* ints) {
+  KV4_CHECK("jx_kv4_workspace_ints");
+  if (!ints) return fail(JX_ERR_ARG, "jx_kv4_workspace_ints: null output");
+  *ints = kv4_workspace_ints(cache->num_rows, cache->num_pages);
+  return JX_OK;
+}
+
+int jx_kv4_extend(const jx_kv4_cache* cache, const int* counts, int count, int* ws, long long ws_ints, void* stream) {
+  KV4_CHECK("jx_kv4_extend");
+  if (!counts && count < 0) return fail(JX_ERR_SHAPE, "jx_kv4_extend: count must not be negative");
+  if (!ws || ws_ints < kv4_workspace_ints(cache->num_rows, cache->num_pages))
+    return fail(JX_ERR_ARG, "jx_kv4_extend: workspace too small");
+  return kv4_done(run_kv4_extend(*cache, counts, count, ws, (cudaStream_t)stream), "jx_kv4_extend");
+}
+
+int jx_kv4_fork(const jx_kv4_cache* cache, const int* parents, void* stream) {
+  KV4_CHECK("jx_kv4_fork");
+  if (!parents) return fail(JX_ERR_ARG, "jx_kv4_fork: null parents");
+  return kv4_done(run_kv4_fork(*cache, parents, (cudaStream_t)stream), "jx_kv4_fork");
+}
+
+int jx_kv4_rollback(const jx_kv4_cache* cache, const int* n, int n_all, void* stream) {
+  KV4_CHECK("jx_kv4_rollback");
+  if (!n && n_all < 0) return fail(JX_ERR_SHAPE, "jx_kv4_rollback: n must not be negative");
+  return kv4_done(run_kv4_shorten(*cache, nullptr, n, n_all, (cudaStream_t)stream), "jx_kv4_rollback");
+}
+
+int jx_kv4_free(const jx_kv4_cache* cache, const unsigned char* rows, void* stream) {
+  KV4_CHECK("jx_kv4_free");
+  if (!rows) return fail(JX_ERR_ARG, "jx_kv4_free: null rows");
+  return kv4_done(run_kv4_shorten(*cache, rows, nullptr, 0, (cudaStream_t)stream), "jx_kv4_free");
+}
+
+int jx_kv4_compact(const jx_kv4_cache* cache, int* used, int* ws, long long ws_ints, void* stream) {
+  KV4_CHECK("jx_kv4_compact");
+  if (!used) return fail(JX_ERR_ARG, "jx_kv4_compact: null output");
+  if (!ws || ws_ints < kv4_workspace_ints(cache->num_rows, cache->num_pages))
+    return fail(JX_ERR_ARG, "jx_kv4_compact: workspace too small");
+  return kv4_done(run_kv4_compact(*cache, used, ws, (cudaStream_t)stream), "jx_kv4_compact");
+}
+
+int jx_token_log_probs(const jx_log_probs_args* args, void* stream) {
+  if (!args || !args->logits || !args->ids || !args->log_probs || !args->entropy)
+    return fail(JX_ERR_ARG, "jx_token_log_probs: null pointer");
+  if (args->rows <= 0 || args->V <= 0 || (args->rows > 1 && args->ld < args->V))
+    return fail(JX_ERR_SHAPE, "jx_token_log_probs: sizes must be positive and rows must not overlap");
+  if (args->top_n < 0 || args->top_n > 64 || args->top_n > args->V)
+    return fail(JX_ERR_SHAPE, "jx_token_log_probs: 0 <= top_n <= min(64, V)");
+  if (args->top_n && (!args->top_log_probs || !args->top_ids))
+    return fail(JX_ERR_ARG, "jx_token_log_probs: null pointer for the alternatives");
+  if (args->dtype != JX_F32 && args->dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_token_log_probs: float32 or bfloat16");
+  if ((uintptr_t)args->logits % (args->dtype == JX_BF16 ? 2 : 4)) return fail(JX_ERR_ARG, "jx_token_log_probs: misaligned logits");
+  return kv4_done(run_token_log_probs(*args, (cudaStream_t)stream), "jx_token_log_probs");
+}
+
+}  // extern "C"

@@ -16,6 +16,7 @@ from ._checks import normalize_dtype
 from .config import ModelConfig
 from .decoders import (GemmaDecoder, GemmaMLP, GPTNeoXDecoder, GPTNeoXMLP, LlamaDecoder,  # noqa: F401
                        LlamaMLP)
+from .paged_cache import PagedKVCache
 from .nn import GemmaRMSNorm  # noqa: F401  (models/gemma3.py:89-106 lives in jaxml.models)
 
 # models/__init__.py of the reference: the architecture entry points, in its order
@@ -104,7 +105,8 @@ class _DecoderWithHead:
         in a ``CausalLMOutputWithCache``.  A cache-free call without position ids or hidden states runs on
         the fused prefill runtime; calls with KV caches (a prompt into empty caches, or one token per row
         into populated ones), position ids, ``output_hidden_states`` or ``output_attentions`` run layer by
-        layer through the decoder blocks.  Masks must be right-padded."""
+        layer through the decoder blocks.  Masks must be right-padded.  ``kv_caches`` may also be one
+        ``PagedKVCache`` for all layers: the mask's tokens are added to its rows, whatever these hold."""
         from ._checks import normalize_count
 
         keep = normalize_count("keep_last_n_logits", keep_last_n_logits)
@@ -159,6 +161,9 @@ class _DecoderWithHead:
         use_cache = normalize_bool("use_cache", use_cache)
         output_attentions = normalize_bool("output_attentions", output_attentions)
         output_hidden_states = normalize_bool("output_hidden_states", output_hidden_states)
+        if isinstance(kv_caches, PagedKVCache):
+            return self._paged_stack(params, input_ids, attention_mask, position_ids, kv_caches, use_cache,
+                                     output_attentions, output_hidden_states)
         ids, mask, kv_caches, pos = _prepare_model_inputs(self.config, input_ids, attention_mask, kv_caches,
                                                           position_ids)
         L = self.config.num_layers
@@ -183,6 +188,36 @@ class _DecoderWithHead:
             output_attentions)
         return (h, caches if use_cache else None, states if output_hidden_states else None,
                 weights if output_attentions else None, False)
+
+    def _paged_stack(self, params, input_ids, attention_mask, position_ids, cache, use_cache, output_attentions,
+                     output_hidden_states):
+        """The stack over a ``PagedKVCache``: the mask's tokens of every row (a prompt, a chunk of one, or single
+        tokens, also on rows that hold tokens already) are added to the cache, which changes in place."""
+        from .decoders import layered_forward
+
+        cfg = self.config
+        if position_ids is not None or output_attentions:
+            raise NotImplementedError("position_ids and output_attentions are not implemented over a paged 4-bit cache.")
+        ids, mask, _, _ = _prepare_model_inputs(cfg, input_ids, attention_mask)
+        if not _right_padded(mask):
+            raise NotImplementedError("apply takes right-padded attention masks (the kernels attend to key prefixes).")
+        want = (cfg.num_layers, ids.shape[0], cfg.num_key_value_heads, cfg.head_dim)
+        got = (cache.num_layers, cache.num_rows, cache.num_kv_heads, cache.head_dim)
+        if got != want:
+            raise ValueError("the paged cache must match the model's (layers, batch rows, KV heads, head_dim), got "
+                             f"{got} and expected {want}.")
+        body = self._body(params)
+        dev = body["embed_tokens"]["embedding"].device
+        counts = mask.to(device=dev, dtype=torch.int32).sum(dim=1, dtype=torch.int32)
+        if bool((cache.lengths + counts > cfg.max_position_embeddings).any()):
+            raise ValueError(f"rows of the paged cache must stay within max_position_embeddings={cfg.max_position_embeddings}.")
+        cache.extend(counts)
+        cache.check()
+        h, _, states, _ = layered_forward(
+            self.family, cfg, self.dtype, body, ids.to(dev), mask.to(dev),
+            cache.position_ids(ids.shape[1]) if cfg.use_rope else None,
+            tuple(cache.layer(i) for i in range(cfg.num_layers)), None, self.__dict__["_layered_cache"]["rope"])
+        return h, cache if use_cache else None, states if output_hidden_states else None, None, False
 
     _has_head = True
 

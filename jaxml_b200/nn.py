@@ -35,6 +35,7 @@ from . import _native as N
 from ._checks import normalize_bool, normalize_count, normalize_dtype, normalize_float
 from .cache import KVCache
 from .config import ModelConfig
+from .paged_cache import PagedKVLayer
 
 # nn/__init__.py of the reference, in its order (AttentionOutput, GemmaRMSNorm and initializers are here
 # too, outside the star-import list as there)
@@ -1070,7 +1071,7 @@ class Attention(Block):
         output_attentions = normalize_bool("output_attentions", output_attentions)
         if normalize_bool("use_flash", use_flash):
             raise NotImplementedError("JAX flash attention is not enabled in jaxml yet.")
-        if kv_cache is not None and not isinstance(kv_cache, KVCache):
+        if kv_cache is not None and not isinstance(kv_cache, (KVCache, PagedKVLayer)):
             raise TypeError(f"kv_cache must be a KVCache instance or None, got {type(kv_cache)}.")
         return output_attentions
 
@@ -1081,6 +1082,15 @@ class Attention(Block):
         if window < 0:
             raise ValueError(f"sliding_window must be positive when set, got {window}.")
         B, S = hidden.shape[:2]
+        if isinstance(kv_cache, PagedKVLayer):
+            # the cache's counts say which tokens of the call are there; a mask would say it again
+            if output_attentions:
+                raise NotImplementedError("output_attentions is not implemented over a paged 4-bit cache.")
+            _need_cuda("Attention", q, k, v)
+            out = kv_cache.update_and_attend(q.to(self.dtype), k.to(self.dtype), v.to(self.dtype),
+                                             float(self.attn_scale), window or None)
+            kv_cache.cache.check()
+            return AttentionOutput(attention_output=self.post_mha(variables, out), kv_cache=kv_cache)
         if kv_cache is not None:
             if kv_cache.k is not None and S > 1:
                 raise NotImplementedError("a multi-token call on a populated KV cache (chunked prefill) is not "
@@ -1144,10 +1154,13 @@ class AttentionWithRoPE(Attention):
         self._preflight(output_attentions, use_flash, kv_cache)
         cos, sin = _cos_sin_pair(cos_sin)
         q, k, v = self.qkv(variables, x)
-        if attention_mask is None and kv_cache is not None and kv_cache.mask is not None:
+        paged = isinstance(kv_cache, PagedKVLayer)
+        if attention_mask is None and kv_cache is not None and not paged and kv_cache.mask is not None:
             attention_mask = kv_cache.next_mask
         if position_ids is None:
-            if kv_cache is not None and kv_cache.pos_id is not None:
+            if paged:
+                position_ids = kv_cache.cache.position_ids(k.shape[1])
+            elif kv_cache is not None and kv_cache.pos_id is not None:
                 position_ids = kv_cache.next_pos_id
             else:
                 position_ids = torch.arange(k.shape[1], device=x.device)[None].expand(k.shape[0], -1)

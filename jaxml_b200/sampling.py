@@ -17,12 +17,13 @@ import math
 import numbers
 import operator
 from dataclasses import dataclass
+from typing import NamedTuple
 
 import numpy as np
 
 import torch
 
-from ._checks import normalize_bool
+from ._checks import normalize_bool, normalize_count
 
 logger = logging.getLogger(__name__)
 
@@ -266,6 +267,67 @@ def categorical(rng, logits: torch.Tensor, temp: float) -> torch.Tensor:
     s.status = status.data_ptr()
     N.check(N.load().jx_sample(s, 0, torch.cuda.current_stream(dev).cuda_stream), "jx_sample")
     return tokens.reshape(x.shape[:-1])
+
+
+class TokenLogProbs(NamedTuple):
+    """``token_log_probs``: float32 ``log_probs`` and ``entropy`` of the leading shape, ``top_log_probs`` float32 and
+    ``top_ids`` int32 ``[..., top_n]``."""
+
+    log_probs: torch.Tensor
+    entropy: torch.Tensor
+    top_log_probs: torch.Tensor
+    top_ids: torch.Tensor
+
+
+def token_log_probs(logits: torch.Tensor, token_ids, top_n: int = 0) -> TokenLogProbs:
+    """Log probabilities of ``token_ids`` ``[...]`` under softmax of CUDA float32 / bfloat16 ``logits`` ``[..., V]``, the
+    softmax's entropy, and the ``top_n`` (at most 64) likeliest tokens with their log probabilities, equal logits in the
+    order of their ids: ``jx_token_log_probs``, one reading of the logits, in float32.
+
+    Filtered entries (-inf) have probability 0 and log probability -inf.  A negative id asks for nothing and gives 0;
+    an id of V or more gives NaN, and so do a row's results when it has NaN or +inf logits or no finite one (the
+    device is not synchronised to raise)."""
+    from . import _native as N
+
+    if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":
+        raise RuntimeError("token_log_probs runs on CUDA logits only (the scoring kernel).")
+    dtype = _SCORE_DTYPES.get(logits.dtype)
+    if dtype is None:
+        if not logits.is_floating_point():
+            raise TypeError(f"logits must contain floating point values, got dtype {logits.dtype}.")
+        raise NotImplementedError(f"the scoring kernel takes float32 or bfloat16 logits, got {logits.dtype}.")
+    if logits.ndim == 0 or logits.shape[-1] <= 0:
+        raise ValueError(f"logits must have a non-empty vocabulary axis, got shape {tuple(logits.shape)}.")
+    lead, V, dev = logits.shape[:-1], logits.shape[-1], logits.device
+    if type(top_n) is not int:
+        top_n = normalize_count("top_n", top_n)
+    if not 0 <= top_n <= min(64, V):
+        raise ValueError(f"top_n must be within [0, {min(64, V)}], got {top_n}.")
+    ids = token_ids if isinstance(token_ids, torch.Tensor) else torch.as_tensor(token_ids)
+    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+        raise TypeError(f"token_ids must contain integer token ids, got dtype {ids.dtype}.")
+    if ids.shape != lead:
+        raise ValueError(f"token_ids must have the logits' leading shape {tuple(lead)}, got {tuple(ids.shape)}.")
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, V)          # before the narrowing: a wrapped id would be another token's
+    ids = ids.to(device=dev, dtype=torch.int32).contiguous()
+    lp, ent = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    top_lp = torch.empty(lead + (top_n,), dtype=torch.float32, device=dev)
+    top_ids = torch.empty(lead + (top_n,), dtype=torch.int32, device=dev)
+    rows = lp.numel()
+    if rows == 0:
+        return TokenLogProbs(lp, ent, top_lp, top_ids)
+    x = logits.reshape(rows, V)
+    if x.stride(-1) != 1 or (rows > 1 and x.stride(0) < V):
+        x = x.contiguous()
+    a = N.JxLogProbsArgs(rows, V, x.data_ptr(), x.stride(0) if rows > 1 else V, dtype, top_n, ids.data_ptr(),
+                         lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr())
+    with torch.cuda.device(dev):
+        N.check(N.load().jx_token_log_probs(a, torch.cuda.current_stream(dev).cuda_stream), "jx_token_log_probs")
+    return TokenLogProbs(lp, ent, top_lp, top_ids)
+
+
+_SCORE_DTYPES = {torch.float32: 0, torch.bfloat16: 1}   # JX_F32, JX_BF16
 
 
 def _probs(logits: torch.Tensor) -> torch.Tensor:
