@@ -470,7 +470,7 @@ int jx_kv4_attend(const jx_kv4_cache* cache, int layer, int S, int Hq, const voi
     return fail(JX_ERR_SHAPE, "jx_kv4_attend: layer out of range, S < 1 or window < 0");
   if (Hq <= 0 || Hq % cache->num_kv_heads || Hq > 65535)
     return fail(JX_ERR_SHAPE, "jx_kv4_attend: Hq must be a multiple of the KV heads, at most 65535");
-  if ((long long)cache->num_rows * S > 0x7FFFFFFF) return fail(JX_ERR_SHAPE, "jx_kv4_attend: rows * S must be below 2^31");
+  if ((long long)cache->num_rows * S > 0x7FFFFFFF / Hq) return fail(JX_ERR_SHAPE, "jx_kv4_attend: rows * S * Hq must be below 2^31");
   if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_attend: float32 or bfloat16");
   if ((uintptr_t)q % (dtype == JX_BF16 ? 2 : 4)) return fail(JX_ERR_ARG, "jx_kv4_attend: misaligned queries");
   if (!(scale > -1e30f && scale < 1e30f)) return fail(JX_ERR_ARG, "jx_kv4_attend: scale must be finite");
