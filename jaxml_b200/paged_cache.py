@@ -37,6 +37,7 @@ __all__ = ["PagedKVCache", "PagedKVLayer"]
 
 PAGE_SIZE = 64
 HEAD_DIMS = (64, 128, 256)
+_current_device = torch.cuda.current_device
 _DTYPES = {torch.float32: N.JX_F32, torch.bfloat16: N.JX_BF16}
 
 
@@ -96,6 +97,7 @@ class PagedKVCache:
         self._c = c
         self._ref = ctypes.byref(c)
         self._lib = None
+        self._index = self.device.index
         self._plan_ints = 0
         self._ws_bytes: dict = {}
 
@@ -136,17 +138,17 @@ class PagedKVCache:
 
     def _call(self, name: str, *args):
         """One library call on the cache's device and its current stream."""
-        if self.device.type != "cuda":
-            raise RuntimeError(f"{name}: PagedKVCache runs on a CUDA device (got {self.device}).")
-        if self._lib is None:
-            self._lib = N.load()
-        index = self.device.index
-        fn = getattr(self._lib, name)
-        if index is None or index == torch.cuda.current_device():
-            rc = fn(self._ref, *args, torch.cuda.current_stream(self.device).cuda_stream)
+        lib = self._lib
+        if lib is None:
+            if self.device.type != "cuda":
+                raise RuntimeError(f"{name}: PagedKVCache runs on a CUDA device (got {self.device}).")
+            lib = self._lib = N.load()
+        index = self._index
+        if index == _current_device():
+            rc = getattr(lib, name)(self._ref, *args, N.raw_stream(index))
         else:
             with torch.cuda.device(index):
-                rc = fn(self._ref, *args, torch.cuda.current_stream(self.device).cuda_stream)
+                rc = getattr(lib, name)(self._ref, *args, N.raw_stream(index))
         if rc:
             N.check(rc, name)
 
@@ -170,10 +172,12 @@ class PagedKVCache:
         """An int32 [rows] tensor on the cache's device."""
         if not isinstance(x, torch.Tensor):
             x = torch.as_tensor(x)
-        if x.dtype.is_floating_point or x.dtype.is_complex or x.dtype == torch.bool:
+        if x.dtype == torch.bool or x.dtype.is_floating_point or x.dtype.is_complex:
             raise TypeError(f"{name} must contain integers, got dtype {x.dtype}.")
-        if tuple(x.shape) != (self.num_rows,):
+        if x.shape != self.lengths.shape:
             raise ValueError(f"{name} must have shape ({self.num_rows},), got {tuple(x.shape)}.")
+        if x.dtype == torch.int32 and x.device == self.device and x.is_contiguous():
+            return x
         if x.dtype == torch.int64:
             x = x.clamp(-2 ** 31, 2 ** 31 - 1)
         return x.to(device=self.device, dtype=torch.int32).contiguous()
@@ -225,8 +229,8 @@ class PagedKVCache:
             ptr, add = None, normalize_count("start", start)
             if not 0 <= add < 1 << 31:
                 raise ValueError(f"start must be within [0, 2^31), got {add}.")
-        k, v = (torch.empty(self.num_rows, length, self.num_kv_heads, self.head_dim, dtype=dtype, device=self.device)
-                for _ in range(2))
+        k = torch.empty((self.num_rows, length, self.num_kv_heads, self.head_dim), dtype=dtype, device=self.device)
+        v = torch.empty_like(k)
         self._call("jx_kv4_read", layer, None if ptr is None else ptr.data_ptr(), add, length, k.data_ptr(), v.data_ptr(),
                    _DTYPES[dtype])
         return k, v
@@ -245,7 +249,7 @@ class PagedKVCache:
             raise ValueError(f"q heads must be a multiple of the {self.num_kv_heads} KV heads, got {heads}.")
         scale = self.head_dim ** -0.5 if scale is None else normalize_float("scale", scale)
         window = 0 if sliding_window is None else _positive("sliding_window", sliding_window)
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
         key = (S, heads, q.dtype)
         size = self._ws_bytes.get(key)
         if size is None:

@@ -304,26 +304,34 @@ def token_log_probs(logits: torch.Tensor, token_ids, top_n: int = 0) -> TokenLog
     if not 0 <= top_n <= min(64, V):
         raise ValueError(f"top_n must be within [0, {min(64, V)}], got {top_n}.")
     ids = token_ids if isinstance(token_ids, torch.Tensor) else torch.as_tensor(token_ids)
-    if ids.is_floating_point() or ids.is_complex() or ids.dtype == torch.bool:
+    if ids.dtype == torch.bool or ids.is_floating_point() or ids.is_complex():
         raise TypeError(f"token_ids must contain integer token ids, got dtype {ids.dtype}.")
     if ids.shape != lead:
         raise ValueError(f"token_ids must have the logits' leading shape {tuple(lead)}, got {tuple(ids.shape)}.")
-    if ids.dtype == torch.int64:
-        ids = ids.clamp(-1, V)          # before the narrowing: a wrapped id would be another token's
-    ids = ids.to(device=dev, dtype=torch.int32).contiguous()
-    lp, ent = (torch.empty(lead, dtype=torch.float32, device=dev) for _ in range(2))
+    if ids.dtype != torch.int32 or ids.device != dev or not ids.is_contiguous():
+        if ids.dtype == torch.int64:
+            ids = ids.clamp(-1, V)      # before the narrowing: a wrapped id would be another token's
+        ids = ids.to(device=dev, dtype=torch.int32).contiguous()
+    lp = torch.empty(lead, dtype=torch.float32, device=dev)
+    ent = torch.empty_like(lp)
     top_lp = torch.empty(lead + (top_n,), dtype=torch.float32, device=dev)
-    top_ids = torch.empty(lead + (top_n,), dtype=torch.int32, device=dev)
+    top_ids = torch.empty_like(top_lp, dtype=torch.int32)
     rows = lp.numel()
     if rows == 0:
         return TokenLogProbs(lp, ent, top_lp, top_ids)
-    x = logits.reshape(rows, V)
-    if x.stride(-1) != 1 or (rows > 1 and x.stride(0) < V):
+    x = logits if logits.ndim == 2 else logits.reshape(rows, V)
+    if x.stride(1) != 1 or (rows > 1 and x.stride(0) < V):
         x = x.contiguous()
     a = N.JxLogProbsArgs(rows, V, x.data_ptr(), x.stride(0) if rows > 1 else V, dtype, top_n, ids.data_ptr(),
                          lp.data_ptr(), ent.data_ptr(), top_lp.data_ptr(), top_ids.data_ptr())
-    with torch.cuda.device(dev):
-        N.check(N.load().jx_token_log_probs(a, torch.cuda.current_stream(dev).cuda_stream), "jx_token_log_probs")
+    lib = N.load()
+    if dev.index == torch.cuda.current_device():
+        rc = lib.jx_token_log_probs(a, N.raw_stream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = lib.jx_token_log_probs(a, N.raw_stream(dev.index))
+    if rc:
+        N.check(rc, "jx_token_log_probs")
     return TokenLogProbs(lp, ent, top_lp, top_ids)
 
 
