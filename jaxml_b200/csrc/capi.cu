@@ -410,6 +410,7 @@ static const char* kv4_bad(const jx_kv4_cache* c, int* code) {
   if (c->num_rows > 8192) return "at most 8192 rows";
   if (c->row_pages > (1 << 24)) return "at most 2^24 pages per row";
   if (c->num_pages > (1 << 28) || c->num_kv_heads > 4096) return "at most 2^28 pages and 4096 KV heads";
+  if ((long long)c->num_layers * c->num_pages * c->num_kv_heads > 0x7FFFFFFF) return "layers * pages * KV heads must be below 2^31";
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return "head_dim must be 64, 128 or 256";
   return nullptr;
 }

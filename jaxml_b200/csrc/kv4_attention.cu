@@ -1,20 +1,26 @@
 // Attention over the pages of the 4-bit KV cache (format in kv4.cuh).
 //
 // One pass over the keys with a running maximum m and sum l: for a tile of query rows (a query position and a query
-// head of one KV head) and a page of 64 keys,
+// head of one KV head) and a slice of keys,
 //   S = K Q^T (keys x rows), P = 2^(S c - m'), O = O 2^(m - m') + V^T P (channels x rows), l = l 2^(m - m') + sum P.
 // Both products run on mma.m16n8k16 with the cache as the A operand, so a tile of 8 query rows (the usual decode step:
 // the heads that share a KV head) fills the N side and nothing is padded to 16.  The codes go from shared memory
-// straight into A fragments: a thread's 32-bit word is 8 neighbouring channels of one key; (w >> 4k) & 0x000F000F is the pair
-// (channel k, channel k + 4), a fragment register of K once Q's fragments take the same order, and the same bits of
-// two keys' words merged by a byte permute are the pair (key, key + 1) that V^T needs.  0x4300 | u is bfloat16 128 + u,
-// so u - 8 and its product with the scale are exact.  P changes from the accumulator's layout to the B operand's with
-// movmatrix, without shared memory.
+// straight into A fragments: a thread's 32-bit word is 8 neighbouring channels of one key; (w >> 4k) & 0x000F000F is
+// the pair (channel k, channel k + 4), a fragment register of K once Q's fragments take the same order, and the same
+// bits of two keys' words merged by a byte permute are the pair (key, key + 1) that V^T needs.  0x4300 | u is the
+// bfloat16 128 + u.  P changes from the accumulator's layout to the B operand's with movmatrix, without shared memory.
 //
-// Work is split into pages: all (row, query tile, KV head, page) units in one sequence, cut into equal runs, one for
-// each warp of the grid whatever the rows' lengths are.  A warp streams its run's pages (one bulk copy each: a page's
-// block is contiguous) through its own ring.  A (row, tile, head) that one warp holds whole is written at once; the
-// others leave (m, l, O) for a second kernel, which joins them in order.
+// What bounds a decode step is instructions, not bytes: a page of 64 keys is 9 KB and the multiprocessor has some 400
+// cycles for it at the card's bandwidth.  So with one tile of 8 rows nothing is subtracted or scaled per code:
+//   K   the k side of an MMA pair is one group of 32 channels, fed with 128 + u; the accumulator starts at
+//       -136 sum q of the group and its result times the key's scale is added up in float32;
+//   V   one fused multiply-add gives (128 + u) s - 128 s = u s, exact in bfloat16 (u and s have 4 bits each); the
+//       8 sum p s that u = code + 8 adds comes out of one more MMA with the scales as its A operand.
+// With more rows a code is used often enough that making it exact first costs little, and float32 results need it.
+//
+// A page's block is one tensor-map box of 144 rows of hd / 2 bytes, swizzled by the copy so that ldmatrix gives every
+// thread its words of the key it owns without bank conflicts.
+#include <cudaTypedefs.h>
 #include <math.h>
 
 #include "kv4.cuh"
@@ -37,49 +43,52 @@ struct AttendArgs {
 template <int HD, int NT, typename T>
 struct Cfg {
   static constexpr int kBlock = kPage * HD + kPage * (HD / 32) * 4;
+  static constexpr int kRowBytes = HD / 2;                // a key's codes
+  static constexpr int kGroups = HD / 32;
   static constexpr bool kF32 = sizeof(T) == 4;
+  static constexpr bool kRaw = NT == 1 && !kF32;          // codes enter the MMAs with their offset
   static constexpr int kQParts = kF32 ? 3 : 1;            // a float32 as three bfloat16: 24 significant bits
   static constexpr int kPParts = kF32 ? 3 : 1;
   static constexpr int kRows = 8 * NT;
-  static constexpr int kChunks = HD >= 128 ? HD / 128 : 1;
-  static constexpr int kWords = HD >= 128 ? 4 : 2;        // K words of a key, chunk and thread
   static constexpr int kVWords = HD / 64;                 // V words of a key and thread
   static constexpr int kMT = HD / 16;
-  static constexpr int kKeys = NT == 1 ? 64 : 32;         // keys between two updates of the maximum
   static constexpr bool kQReg = NT * kQParts * HD / 8 <= 32;
-  static constexpr int kQBytes = kQReg ? 0 : NT * kQParts * HD * 16;
-  static constexpr int kBudget = 224 * 1024;
-  static constexpr int kFit = kBudget / (2 * kBlock + kQBytes + 64);   // warps with two pages each
-  static constexpr int kWarps = kFit < 8 ? kFit : 8;
-  static constexpr int kDeep = (kBudget / kWarps - kQBytes - 64) / kBlock;
-  static constexpr int kStages = kDeep < 4 ? kDeep : 4;
-  static constexpr int kThreads = kWarps * 32;
-  static constexpr int kSlot = kRows * (HD + 2);          // floats
-  static constexpr int kSmem = kWarps * (kStages * kBlock + kQBytes + kStages * 16) + (kThreads + 40) * 8;
-  static_assert(kSmem <= 227 * 1024, "shared memory");
+  static constexpr int kQBytes = kQReg ? 0 : NT * kQParts * HD * 16;   // a warp's fragments in shared memory
+  static constexpr int kSlot = kRows * (HD + 2);          // floats of a partial result
 };
 
 // ---- small pieces -------------------------------------------------------------------------------------
-// bfloat16 pair (n_k, n_k+4) - 8 of a word.
-__device__ __forceinline__ __nv_bfloat162 codes(uint32_t w, int k) {
+__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t as_u(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+// bfloat16 pair 128 + u of the nibbles k and k + 4 of a word (or k of two merged words).
+__device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
   uint32_t r;
   asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(r) : "r"(w >> (4 * k)));
-  const uint32_t c = 0x43084308u;   // 136
-  return __hsub2(*reinterpret_cast<__nv_bfloat162*>(&r), *reinterpret_cast<const __nv_bfloat162*>(&c));
+  return r;
 }
-__device__ __forceinline__ uint32_t scaled(uint32_t w, int k, uint32_t s2) {
-  const __nv_bfloat162 r = __hmul2(codes(w, k), *reinterpret_cast<__nv_bfloat162*>(&s2));
-  return *reinterpret_cast<const uint32_t*>(&r);
+__device__ __forceinline__ uint32_t code2(uint32_t w, int k) { return as_u(__hsub2(as_b2(raw2(w, k)), as_b2(0x43084308u))); }
+__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2) { return as_u(__hmul2(as_b2(code2(w, k)), as_b2(s2))); }
+__device__ __forceinline__ void mma_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                      float c0, float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
-  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
 }
 __device__ __forceinline__ float exp2_f(float x) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
+}
+// Where the copy's swizzle puts a byte of a block (16-byte pieces of a 128-byte line exchanged by the line's number).
+template <int HD>
+__device__ __forceinline__ int swz(int o) {
+  return o ^ (((o >> 7) & (HD / 32 - 1)) << 4);
 }
 __device__ __forceinline__ uint32_t lds16(const unsigned char* p) { return *reinterpret_cast<const uint16_t*>(p); }
 
@@ -161,23 +170,394 @@ __device__ __forceinline__ void q_words(const float* p, bool vec, uint4* out) {
   }
 }
 
-// ---- the kernel ---------------------------------------------------------------------------------------------
+// ---- one tile of query rows over slices of a page -----------------------------------------------------------
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(Cfg<HD, NT, T>::kThreads, 1) kv4_attend_kernel(const AttendArgs a) {
+struct Tile {
   using C = Cfg<HD, NT, T>;
-  constexpr int kTiles = C::kKeys / 16;
-  extern __shared__ __align__(16) unsigned char smem[];
-  unsigned char* ring = smem;
-  unsigned char* qs = ring + C::kWarps * C::kStages * C::kBlock;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(qs + C::kWarps * C::kQBytes);
-  int* bad = reinterpret_cast<int*>(bars + C::kWarps * C::kStages);
-  long long* first = reinterpret_cast<long long*>(bad + 2 * C::kWarps * C::kStages);   // [kThreads + 1]
-  long long* sums = first + C::kThreads + 1;                                           // [32]
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  float acc[C::kMT][NT][4], m[NT][2], l[NT][2];
+  float over[C::kRaw ? 4 : 1];                    // sum p s of the thread's group (kRaw)
+  float init[C::kRaw ? C::kGroups : 1][2];        // -136 sum q of a group, columns 2t and 2t + 1 (kRaw)
+  int last[NT][2];                                // last visible key of the thread's columns (-1: none)
+  uint4 q[C::kQReg ? NT : 1][C::kQReg ? C::kQParts : 1][C::kQReg ? C::kGroups : 1];
+  uint4* qs;                                      // the fragments in shared memory otherwise
+
+  __device__ __forceinline__ void begin(const AttendArgs& a, const Item& t, int head, int lane, bool store = true) {
+    const int g = lane >> 2, tq = lane & 3, f0 = t.qt * C::kRows, F = a.S * a.G;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int f = f0 + nt * 8 + 2 * tq + e, s = f / a.G;
+        last[nt][e] = f < F && s < t.cnt ? t.base + s : -1;
+        m[nt][e] = -INFINITY, l[nt][e] = 0.f;
+      }
+      const int f = f0 + nt * 8 + g, s = f / a.G;
+      const bool live = f < F && s < t.cnt;
+      const T* src = static_cast<const T*>(a.q) + t.r * a.q_row + s * a.q_tok + (head * a.G + (f - s * a.G)) * a.q_head;
+#pragma unroll
+      for (int i = 0; i < C::kGroups; ++i) {
+        uint4 x[C::kQParts];
+        if (live) {
+          q_words(src + i * 32 + tq * 8, a.q_vec, x);
+        } else {
+#pragma unroll
+          for (int p = 0; p < C::kQParts; ++p) x[p] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int p = 0; p < C::kQParts; ++p) {
+          if constexpr (C::kQReg) q[nt][p][i] = x[p];
+          else if (store) qs[((nt * C::kQParts + p) * C::kGroups + i) * 32 + lane] = x[p];
+        }
+        if constexpr (C::kRaw) {
+          float v[8], sum = 0.f;
+          unpack8(x[0], v);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) sum += v[k];
+          sum += __shfl_xor_sync(~0u, sum, 1);
+          sum += __shfl_xor_sync(~0u, sum, 2);
+          init[i][0] = -136.f * __shfl_sync(~0u, sum, tq * 8);
+          init[i][1] = -136.f * __shfl_sync(~0u, sum, tq * 8 + 4);
+        }
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < C::kMT; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][nt][e] = 0.f;
+    if constexpr (C::kRaw) over[0] = over[1] = over[2] = over[3] = 0.f;
+  }
+
+  __device__ __forceinline__ uint4 query(int nt, int p, int grp, int lane) const {
+    if constexpr (C::kQReg) return q[nt][p][grp];
+    else return qs[((nt * C::kQParts + p) * C::kGroups + grp) * 32 + lane];
+  }
+
+  // Keys [kb, kb + KT) of the page in `blk` (shared memory, swizzled), whose first key is key0.  all: every row sees them.
+  template <int KT>
+  __device__ __forceinline__ void keys(const AttendArgs& a, const unsigned char* blk, int kb, int key0, bool all, int lane) {
+    constexpr int kTiles = KT / 16;
+    const int g = lane >> 2, t = lane & 3;
+    float sc[kTiles][NT][4];
+    const uint32_t base = smem_u32(blk);
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      // words of keys g and g + 8: group w's is 4 bytes at 16 w + 4 t of the key's codes
+      uint32_t kw[2][C::kGroups];
+      const int k16 = kb + i * 16;
+      if constexpr (HD == 64) {
+        const int key = k16 + ((lane >> 4) << 3) + (lane & 7);
+        ldsm_x4(base + swz<HD>(key * C::kRowBytes + ((lane >> 3) & 1) * 16), kw[0][0], kw[0][1], kw[1][0], kw[1][1]);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int w = 0; w < C::kGroups; w += 4) {
+            const int key = k16 + h * 8 + (lane & 7);
+            ldsm_x4(base + swz<HD>(key * C::kRowBytes + (w + (lane >> 3)) * 16), kw[h][w], kw[h][w + 1], kw[h][w + 2],
+                    kw[h][w + 3]);
+          }
+      }
+      uint32_t ks[2][C::kGroups / 2];   // scales of the two keys, two groups a register
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const unsigned char* p = blk + swz<HD>(kPage * HD + (k16 + h * 8 + g) * (HD / 16));
+        if constexpr (HD == 64) {
+          ks[h][0] = *reinterpret_cast<const uint32_t*>(p);
+        } else if constexpr (HD == 128) {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          ks[h][0] = x.x, ks[h][1] = x.y;
+        } else {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          ks[h][0] = x.x, ks[h][1] = x.y, ks[h][2] = x.z, ks[h][3] = x.w;
+        }
+      }
+#pragma unroll
+      for (int w = 0; w < C::kGroups; ++w) {
+        if constexpr (NT == 1) {
+          float x[4];
+          uint32_t r[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[h][k] = C::kRaw ? raw2(kw[h][w], k) : code2(kw[h][w], k);
+#pragma unroll
+          for (int p = 0; p < C::kQParts; ++p) {
+            const uint4 b = query(0, p, w, lane);
+            if (p == 0) {
+              const float c0 = C::kRaw ? init[w][0] : 0.f, c1 = C::kRaw ? init[w][1] : 0.f;
+              mma_c(x, r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y, c0, c1, c0, c1);
+            } else {
+              mma_bf16(x, r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y);
+            }
+            mma_bf16(x, r[0][2], r[1][2], r[0][3], r[1][3], b.z, b.w);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float s = __uint_as_float(w & 1 ? ks[h][w >> 1] & 0xFFFF0000u : ks[h][w >> 1] << 16);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (w == 0) sc[i][0][2 * h + e] = s * x[2 * h + e];
+              else sc[i][0][2 * h + e] = fmaf(s, x[2 * h + e], sc[i][0][2 * h + e]);
+            }
+          }
+        } else {
+          uint32_t r[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t s2 = __byte_perm(ks[h][w >> 1], 0, w & 1 ? 0x3232 : 0x1010);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) r[h][k] = scaled2(kw[h][w], k, s2);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int p = 0; p < C::kQParts; ++p) {
+              const uint4 b = query(nt, p, w, lane);
+              if (w == 0 && p == 0) mma_c(sc[i][nt], r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y, 0.f, 0.f, 0.f, 0.f);
+              else mma_bf16(sc[i][nt], r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y);
+              mma_bf16(sc[i][nt], r[0][2], r[1][2], r[0][3], r[1][3], b.z, b.w);
+            }
+        }
+      }
+    }
+    // softmax over the keys: registers 0, 1 are key g, 2, 3 key g + 8, of columns 2t and 2t + 1
+    uint32_t pf[kTiles][NT][C::kPParts][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x = sc[i][nt][2 * h + e] * a.scale_log2;
+            if (!all) {
+              const int key = key0 + kb + i * 16 + h * 8 + g;
+              if (key > last[nt][e] || (a.window > 0 && key <= last[nt][e] - a.window)) x = -INFINITY;
+            }
+            sc[i][nt][2 * h + e] = x;
+            mx = fmaxf(mx, x);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
+        mx = fmaxf(mx, m[nt][e]);
+        const float use = mx == -INFINITY ? 0.f : mx;      // nothing visible yet: every term is 2^-inf
+        f[e] = exp2_f(m[nt][e] - use);
+        m[nt][e] = mx;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = exp2_f(sc[i][nt][2 * h + e] - use);
+            sc[i][nt][2 * h + e] = x;
+            sum += x;
+          }
+        l[nt][e] = fmaf(l[nt][e], f[e], sum);
+      }
+      if (__any_sync(~0u, f[0] != 1.f || f[1] != 1.f)) {      // seldom, once a row's maximum has settled
+#pragma unroll
+        for (int i = 0; i < C::kMT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][nt][e] *= f[e & 1];
+        if constexpr (C::kRaw) over[0] *= f[0], over[1] *= f[1];
+      }
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x0 = sc[i][nt][2 * h], x1 = sc[i][nt][2 * h + 1];
+#pragma unroll
+          for (int p = 0; p < C::kPParts; ++p) {
+            // probabilities rounded to bfloat16 (half a step: 2^-9 of their binade's top) for bfloat16 results, split in
+            // three for float32 ones
+            pf[i][nt][p][h] = transpose8x8(pack_bf16x2(x0, x1));
+            if (p + 1 < C::kPParts) x0 -= rnd<bf16>(x0), x1 -= rnd<bf16>(x1);
+          }
+        }
+    }
+    const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;   // the thread's channels are of one group
+#pragma unroll
+    for (int i = 0; i < kTiles; ++i) {
+      const int k16 = kb + i * 16;
+      uint32_t vw[4][C::kVWords], s2[2];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k16 + 2 * t + (j & 1) + (j >> 1) * 8;
+        const unsigned char* p = blk + swz<HD>(kPage * C::kRowBytes + key * C::kRowBytes + g * (C::kVWords * 4));
+        if constexpr (C::kVWords == 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          vw[j][0] = x.x, vw[j][1] = x.y, vw[j][2] = x.z, vw[j][3] = x.w;
+        } else if constexpr (C::kVWords == 2) {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          vw[j][0] = x.x, vw[j][1] = x.y;
+        } else {
+          vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int o = kPage * HD + kPage * (HD / 16) + (k16 + 2 * t + h * 8) * (HD / 16) + vg * 2;
+        const uint32_t s = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
+        // NaN and infinity to finite: a key that a row does not see has P = 0 there, and 0 * NaN would reach it.  Rows that
+        // do see one get NaN in nan_values.  2^120 is above every scale that the format has.
+        s2[h] = as_u(__hmin2(__hmax2(as_b2(s), as_b2(0u)), as_b2(0x7B807B80u)));
+      }
+      uint32_t c2[2];
+      if constexpr (C::kRaw) {
+        c2[0] = as_u(__hmul2(as_b2(s2[0]), as_b2(0xC300C300u)));   // -128 s
+        c2[1] = as_u(__hmul2(as_b2(s2[1]), as_b2(0xC300C300u)));
+        mma_bf16(over, s2[0], 0u, s2[1], 0u, pf[i][0][0][0], pf[i][0][0][1]);
+      }
+#pragma unroll
+      for (int wd = 0; wd < C::kVWords; ++wd) {
+        const uint32_t lo0 = __byte_perm(vw[0][wd], vw[1][wd], 0x5410), hi0 = __byte_perm(vw[0][wd], vw[1][wd], 0x7632);
+        const uint32_t lo1 = __byte_perm(vw[2][wd], vw[3][wd], 0x5410), hi1 = __byte_perm(vw[2][wd], vw[3][wd], 0x7632);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t a0, a1, a2, a3;
+          if constexpr (C::kRaw) {
+            a0 = as_u(__hfma2(as_b2(raw2(lo0, k)), as_b2(s2[0]), as_b2(c2[0])));
+            a1 = as_u(__hfma2(as_b2(raw2(hi0, k)), as_b2(s2[0]), as_b2(c2[0])));
+            a2 = as_u(__hfma2(as_b2(raw2(lo1, k)), as_b2(s2[1]), as_b2(c2[1])));
+            a3 = as_u(__hfma2(as_b2(raw2(hi1, k)), as_b2(s2[1]), as_b2(c2[1])));
+          } else {
+            a0 = scaled2(lo0, k, s2[0]), a1 = scaled2(hi0, k, s2[0]);
+            a2 = scaled2(lo1, k, s2[1]), a3 = scaled2(hi1, k, s2[1]);
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int p = 0; p < C::kPParts; ++p)
+              mma_bf16(acc[wd * 4 + k][nt], a0, a1, a2, a3, pf[i][nt][p][0], pf[i][nt][p][1]);
+        }
+      }
+    }
+  }
+
+  // Where a value scale of keys [kb, kb + KT) is NaN, the rows that see its key get NaN in its channels.
+  template <int KT>
+  __device__ __forceinline__ void nan_values(const AttendArgs& a, const unsigned char* blk, int kb, int key0, int lane) {
+    constexpr int kV = KT * (HD / 32) / 2;   // 32-bit words of value scales
+    const int at = kPage * HD + kPage * (HD / 16), g = lane >> 2;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < (kV + 31) / 32; ++i) {
+      const uint32_t x = i * 32 + lane < kV
+                             ? *reinterpret_cast<const uint32_t*>(blk + swz<HD>(at + kb * (HD / 16) + (i * 32 + lane) * 4)) : 0u;
+      nan |= (x & 0x7FFFu) >= 0x7F80u || (x & 0x7FFF0000u) >= 0x7F800000u;
+    }
+    if (!__any_sync(~0u, nan)) return;
+    const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;
+    for (int key = kb; key < kb + KT; ++key) {
+      if ((lds16(blk + swz<HD>(at + key * (HD / 16) + vg * 2)) & 0x7FFFu) < 0x7F80u) continue;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (key0 + key <= last[nt][e] && (a.window <= 0 || key0 + key > last[nt][e] - a.window)) {
+#pragma unroll
+            for (int i = 0; i < C::kMT; ++i) acc[i][nt][e] = acc[i][nt][2 + e] = __uint_as_float(0x7FC00000u);
+          }
+    }
+    __syncwarp();
+  }
+
+  // Whether every key of a page is seen by every row of the tile (all of them there).
+  static __device__ __forceinline__ bool sees_all(const AttendArgs& a, const Item& t, int key0) {
+    const int f0 = t.qt * C::kRows, f1 = f0 + C::kRows;
+    return f1 <= t.cnt * a.G && key0 + kPage - 1 <= t.base + f0 / a.G &&
+           (a.window <= 0 || key0 > t.base + (f1 - 1) / a.G - a.window);
+  }
+
+  // The column's sum over the warp; the 8 kVWords channels of the thread and column.
+  __device__ __forceinline__ float sum(int nt, int e) const {
+    float x = l[nt][e];
+    x += __shfl_xor_sync(~0u, x, 4);
+    x += __shfl_xor_sync(~0u, x, 8);
+    return x + __shfl_xor_sync(~0u, x, 16);
+  }
+  __device__ __forceinline__ float value(int wd, int k, int nt, int e) const {   // channel k of word wd
+    float x = acc[wd * 4 + (k & 3)][nt][(k >> 2) * 2 + e];
+    if constexpr (C::kRaw) x = fmaf(-8.f, over[e], x);
+    return x;
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void store_row8(T* o, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                              pack_bf16x2(x[6], x[7]));
+  }
+}
+template <int HD, typename T>
+__device__ __forceinline__ T* out_row(const AttendArgs& a, int r, int head, int f) {
+  const int s = f / a.G;
+  return static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
+}
+
+// Brings the block of a page into shared memory; a page id out of range is reported and its stage marked.
+template <int HD>
+__device__ __forceinline__ void fetch(const AttendArgs& a, const CUtensorMap* map, int id, int head, unsigned char* to,
+                                      uint64_t* bar, int* bad) {
+  const bool ok = id >= 0 && id < a.c.num_pages;
+  *bad = !ok;
+  if (ok) {
+    mbar_arrive_expect_tx(bar, Cfg<HD, 1, bf16>::kBlock);
+    tma_load_3d(to, map, 0, 0, (a.layer * a.c.num_pages + id) * a.c.num_kv_heads + head, bar);
+  } else {
+    set_status(a.c.status, JX_ERR_RANGE);
+    mbar_arrive(bar);
+  }
+}
+
+// ---- equal runs of pages for every warp ------------------------------------------------------------------------
+// All (row, query tile, KV head, page) units in one sequence, cut into equal runs, one for each warp of the grid whatever
+// the rows' lengths are.  A warp streams its run's pages through its own ring.  A (row, tile, head) that one warp holds
+// whole is written at once; the others leave (m, l, O) for kv4_join_kernel, which joins them in order.
+template <int HD, int NT, typename T>
+struct Runs {
+  using C = Cfg<HD, NT, T>;
+  static constexpr int kKeys = NT == 1 ? 64 : 32;          // keys between two updates of the maximum
+  static constexpr int kBudget = 223 * 1024;
+  static constexpr int kMost = NT == 1 && !C::kF32 && HD <= 128 ? 12 : 8;   // by the registers of a thread
+  static constexpr int kFit = kBudget / (2 * C::kBlock + C::kQBytes + 64);  // warps with two pages each
+  static constexpr int kWarps = kFit < kMost ? kFit : kMost;
+  static constexpr int kDeep = (kBudget / kWarps - C::kQBytes - 64) / C::kBlock;
+  static constexpr int kStages = kDeep < 4 ? kDeep : 4;
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kSmem = kWarps * (kStages * C::kBlock + C::kQBytes + kStages * 16) + (kThreads + 40) * 8 + 1024;
+  static_assert(kSmem <= 227 * 1024 && C::kBlock % (HD * 4) == 0, "shared memory, swizzle alignment");
+};
+
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
+    kv4_attend_runs_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap map) {
+  using C = Cfg<HD, NT, T>;
+  using R = Runs<HD, NT, T>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* qs = ring + R::kWarps * R::kStages * C::kBlock;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(qs + R::kWarps * C::kQBytes);
+  int* bad = reinterpret_cast<int*>(bars + R::kWarps * R::kStages);
+  long long* first = reinterpret_cast<long long*>(bad + 2 * R::kWarps * R::kStages);   // [kThreads + 1]
+  long long* sums = first + R::kThreads + 1;                                           // [32]
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const jx_kv4_cache& c = a.c;
+  if (tid == 0) prefetch_tmap(&map);
 
   // units before each thread's share of the items, and all of them
-  const int each = (a.items + C::kThreads - 1) / C::kThreads;
+  const int each = (a.items + R::kThreads - 1) / R::kThreads;
   const int i0 = min(a.items, tid * each), i1 = min(a.items, i0 + each);
   long long mine = 0;
   for (int i = i0; i < i1; ++i) mine += (long long)item_at<C::kRows>(a, i).n * c.num_kv_heads;
@@ -188,18 +568,17 @@ __global__ void __launch_bounds__(Cfg<HD, NT, T>::kThreads, 1) kv4_attend_kernel
     if (lane >= d) v += o;
   }
   if (lane == 31) sums[warp] = v;
-  if (tid < C::kWarps * C::kStages) mbar_init(&bars[tid], 1);
-  if (tid == 0) fence_barrier_init();
+  if (tid < R::kWarps * R::kStages) mbar_init(&bars[tid], 1);
+  fence_barrier_init();
   __syncthreads();
   long long before = 0, units = 0;
 #pragma unroll
-  for (int w = 0; w < C::kWarps; ++w) {
+  for (int w = 0; w < R::kWarps; ++w) {
     if (w < warp) before += sums[w];
     units += sums[w];
   }
   first[tid] = before + v - mine;
-  if (tid == C::kThreads - 1) first[C::kThreads] = units;
-  const long long warps = min((long long)gridDim.x * C::kWarps, max(units, 1ll));
+  const long long warps = min((long long)gridDim.x * R::kWarps, max(units, 1ll));
   if (blockIdx.x == 0) {
     long long u = before + v - mine;
     for (int i = i0; i < i1; ++i) {
@@ -218,7 +597,7 @@ __global__ void __launch_bounds__(Cfg<HD, NT, T>::kThreads, 1) kv4_attend_kernel
   Walk rd;
   long long seg_first;   // first unit of the (item, head) at hand
   {
-    int lo = 0, hi = C::kThreads - 1;   // last share that begins at or before u0
+    int lo = 0, hi = R::kThreads - 1;   // last share that begins at or before u0
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (first[mid] <= u0) lo = mid;
@@ -237,324 +616,78 @@ __global__ void __launch_bounds__(Cfg<HD, NT, T>::kThreads, 1) kv4_attend_kernel
     rd.page = (int)((u0 - u) - (long long)rd.head * rd.t.n);
     seg_first = u0 - rd.page;
   }
-  unsigned char* my_ring = ring + warp * C::kStages * C::kBlock;
-  uint64_t* my_bar = bars + warp * C::kStages;
-  int* my_bad = bad + warp * C::kStages;
-  uint4* my_q = reinterpret_cast<uint4*>(qs + warp * C::kQBytes);
+  unsigned char* my_ring = ring + warp * R::kStages * C::kBlock;
+  uint64_t* my_bar = bars + warp * R::kStages;
+  int* my_bad = bad + warp * R::kStages;
 
   // ahead: the walk of the copies, its next page's id read one step early
   Walk ahead = rd;
   long long ua = u0;
   int next_id = c.table[(long long)ahead.t.r * c.row_pages + ahead.t.p0 + ahead.page];
   auto issue = [&](int stage) {
-    const int id = next_id;
-    const bool ok = id >= 0 && id < c.num_pages;
-    if (lane == 0) {
-      my_bad[stage] = !ok;
-      if (ok) {
-        mbar_arrive_expect_tx(&my_bar[stage], C::kBlock);
-        bulk_g2s(my_ring + stage * C::kBlock, kv4_block(c, a.layer, id, ahead.head), C::kBlock, &my_bar[stage]);
-      } else {
-        set_status(c.status, JX_ERR_RANGE);
-        mbar_arrive(&my_bar[stage]);
-      }
-    }
+    if (lane == 0) fetch<HD>(a, &map, next_id, ahead.head, my_ring + stage * C::kBlock, &my_bar[stage], &my_bad[stage]);
     if (++ua < u1) {
       ahead.next<C::kRows>(a);
       next_id = c.table[(long long)ahead.t.r * c.row_pages + ahead.t.p0 + ahead.page];
     }
   };
 #pragma unroll
-  for (int s = 0; s < C::kStages; ++s)
+  for (int s = 0; s < R::kStages; ++s)
     if (ua < u1) issue(s);
 
-  float acc[C::kMT][NT][4], m[NT][2], l[NT][2];
-  int last[NT][2];                       // last visible key of the thread's columns (-1: none)
-  uint4 q[C::kQReg ? NT : 1][C::kQReg ? C::kQParts : 1][C::kQReg ? HD / 32 : 1];
+  Tile<HD, NT, T> tile;
+  tile.qs = reinterpret_cast<uint4*>(qs + warp * C::kQBytes);
   bool fresh = true;
   int stage = 0;
   uint32_t phase = 0;
-
   for (long long u = u0; u < u1; ++u) {
-    if (fresh) {
-      fresh = false;
-      const int f0 = rd.t.qt * C::kRows, F = a.S * a.G;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int f = f0 + nt * 8 + 2 * t + e, s = f / a.G;
-          last[nt][e] = f < F && s < rd.t.cnt ? rd.t.base + s : -1;
-          m[nt][e] = -INFINITY, l[nt][e] = 0.f;
-        }
-        const int f = f0 + nt * 8 + g, s = f / a.G;
-        const bool live = f < F && s < rd.t.cnt;
-        const T* src = static_cast<const T*>(a.q) + rd.t.r * a.q_row + s * a.q_tok +
-                       (rd.head * a.G + (f - s * a.G)) * a.q_head;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) {
-          const int d = (i / C::kWords) * 128 + t * (C::kWords * 8) + (i % C::kWords) * 8;
-          uint4 x[C::kQParts];
-          if (live) {
-            q_words(src + d, a.q_vec, x);
-          } else {
-#pragma unroll
-            for (int p = 0; p < C::kQParts; ++p) x[p] = make_uint4(0, 0, 0, 0);
-          }
-#pragma unroll
-          for (int p = 0; p < C::kQParts; ++p) {
-            if constexpr (C::kQReg) q[nt][p][i] = x[p];
-            else my_q[((nt * C::kQParts + p) * (HD / 32) + i) * 32 + lane] = x[p];
-          }
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < C::kMT; ++i)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[i][nt][e] = 0.f;
-    }
+    if (fresh) tile.begin(a, rd.t, rd.head, lane);
+    fresh = false;
     const bool arrived = mbar_wait_bounded(&my_bar[stage], phase);
     if (!__all_sync(~0u, arrived)) {      // give up: no copy of this warp may be in flight when it ends
       if (lane == 0) set_status(c.status, JX_ERR_TIMEOUT);
-      for (int s = 0; s < C::kStages; ++s) mbar_wait_bounded(&my_bar[s], s < stage ? phase ^ 1 : phase);
+      for (int s = 0; s < R::kStages; ++s) mbar_wait_bounded(&my_bar[s], s < stage ? phase ^ 1 : phase);
       return;
     }
     const unsigned char* blk = my_ring + stage * C::kBlock;
     const int key0 = (rd.t.p0 + rd.page) * kPage;
-    const int f_last = min(rd.t.qt * C::kRows + C::kRows, rd.t.cnt * a.G) - 1;
-    const int pos0 = rd.t.base + rd.t.qt * C::kRows / a.G, pos1 = rd.t.base + f_last / a.G;
-    // every key is seen by every row of the tile that is there
-    const bool all = key0 + kPage - 1 <= pos0 && (a.window <= 0 || key0 > pos1 - a.window) &&
-                     rd.t.qt * C::kRows + C::kRows <= rd.t.cnt * a.G;
     if (!my_bad[stage]) {
-#pragma unroll
-      for (int sub = 0; sub < kPage / C::kKeys; ++sub) {
-        const int kb = sub * C::kKeys;
-        float sc[kTiles][NT][4];
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[i][nt][e] = 0.f;
-#pragma unroll
-        for (int ch = 0; ch < C::kChunks; ++ch) {
-          const int group = HD >= 128 ? ch * 4 + t : t >> 1;
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i) {
-            uint32_t kw[2][C::kWords], s2[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int key = kb + i * 16 + h * 8 + g;
-              const unsigned char* p = blk + key * (HD / 2) + ch * 64 + t * (C::kWords * 4);
-              if constexpr (C::kWords == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p);
-                kw[h][0] = x.x, kw[h][1] = x.y, kw[h][2] = x.z, kw[h][3] = x.w;
-              } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                kw[h][0] = x.x, kw[h][1] = x.y;
-              }
-              s2[h] = lds16(blk + kPage * HD + (key * (HD / 32) + group) * 2) * 0x10001u;
-            }
-#pragma unroll
-            for (int wd = 0; wd < C::kWords; ++wd) {
-              uint32_t x[2][4];
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[h][k] = scaled(kw[h][wd], k, s2[h]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int p = 0; p < C::kQParts; ++p) {
-                  uint4 b;
-                  if constexpr (C::kQReg) b = q[nt][p][ch * C::kWords + wd];
-                  else b = my_q[((nt * C::kQParts + p) * (HD / 32) + ch * C::kWords + wd) * 32 + lane];
-                  mma_bf16(sc[i][nt], x[0][0], x[1][0], x[0][1], x[1][1], b.x, b.y);
-                  mma_bf16(sc[i][nt], x[0][2], x[1][2], x[0][3], x[1][3], b.z, b.w);
-                }
-            }
-          }
-        }
-        // softmax over the keys: registers (key g: 0, 1), (key g + 8: 2, 3) of columns 2t, 2t + 1
-        uint32_t pf[kTiles][NT][C::kPParts][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float x = sc[i][nt][2 * h + e] * a.scale_log2;
-                if (!all) {
-                  const int key = key0 + kb + i * 16 + h * 8 + g;
-                  if (key > last[nt][e] || (a.window > 0 && key <= last[nt][e] - a.window)) x = -INFINITY;
-                }
-                sc[i][nt][2 * h + e] = x;
-                mx = fmaxf(mx, x);
-              }
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 4));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
-            mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
-            mx = fmaxf(mx, m[nt][e]);
-            const float use = mx == -INFINITY ? 0.f : mx;      // nothing visible yet: every term is 2^-inf
-            const float f = exp2_f(m[nt][e] - use);
-            m[nt][e] = mx;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float x = exp2_f(sc[i][nt][2 * h + e] - use);
-                sc[i][nt][2 * h + e] = x;
-                sum += x;
-              }
-            l[nt][e] = l[nt][e] * f + sum;
-            if (__any_sync(~0u, f != 1.f)) {      // seldom, once a row's maximum has settled
-#pragma unroll
-              for (int i = 0; i < C::kMT; ++i) acc[i][nt][e] *= f, acc[i][nt][2 + e] *= f;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float x0 = sc[i][nt][2 * h], x1 = sc[i][nt][2 * h + 1];
-#pragma unroll
-              for (int p = 0; p < C::kPParts; ++p) {
-                // probabilities rounded to bfloat16 (2^-9) for bfloat16 results, split in three for float32 ones
-                const uint32_t r = pack_bf16x2(x0, x1);
-                pf[i][nt][p][h] = transpose8x8(r);
-                if (p + 1 < C::kPParts) x0 -= rnd<bf16>(x0), x1 -= rnd<bf16>(x1);
-              }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < kTiles; ++i) {
-          const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;   // the thread's channels are of one group
-          uint32_t vw[4][C::kVWords], s2[2];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = kb + i * 16 + 2 * t + (j & 1) + (j >> 1) * 8;
-            const unsigned char* p = blk + kPage * (HD / 2) + key * (HD / 2) + g * (C::kVWords * 4);
-            if constexpr (C::kVWords == 4) {
-              const uint4 x = *reinterpret_cast<const uint4*>(p);
-              vw[j][0] = x.x, vw[j][1] = x.y, vw[j][2] = x.z, vw[j][3] = x.w;
-            } else if constexpr (C::kVWords == 2) {
-              const uint2 x = *reinterpret_cast<const uint2*>(p);
-              vw[j][0] = x.x, vw[j][1] = x.y;
-            } else {
-              vw[j][0] = *reinterpret_cast<const uint32_t*>(p);
-            }
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const unsigned char* p = blk + kPage * HD + kPage * (HD / 32) * 2 + ((kb + i * 16 + 2 * t + h * 8) * (HD / 32) + vg) * 2;
-            uint32_t s = lds16(p) | (lds16(p + (HD / 32) * 2) << 16);
-            // NaN and infinity to 0: a key that a row does not see has P = 0 there, and 0 * NaN would reach it.  Rows that
-            // do see one get NaN below.
-            const uint32_t zero = 0u, most = 0x7F7F7F7Fu;
-            __nv_bfloat162 b = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&s), *reinterpret_cast<const __nv_bfloat162*>(&zero));
-            b = __hmin2(b, *reinterpret_cast<const __nv_bfloat162*>(&most));
-            s2[h] = *reinterpret_cast<uint32_t*>(&b);
-          }
-#pragma unroll
-          for (int wd = 0; wd < C::kVWords; ++wd) {
-            const uint32_t lo0 = __byte_perm(vw[0][wd], vw[1][wd], 0x5410), hi0 = __byte_perm(vw[0][wd], vw[1][wd], 0x7632);
-            const uint32_t lo1 = __byte_perm(vw[2][wd], vw[3][wd], 0x5410), hi1 = __byte_perm(vw[2][wd], vw[3][wd], 0x7632);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t a0 = scaled(lo0, k, s2[0]), a1 = scaled(hi0, k, s2[0]);
-              const uint32_t a2 = scaled(lo1, k, s2[1]), a3 = scaled(hi1, k, s2[1]);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int p = 0; p < C::kPParts; ++p)
-                  mma_bf16(acc[wd * 4 + k][nt], a0, a1, a2, a3, pf[i][nt][p][0], pf[i][nt][p][1]);
-            }
-          }
-        }
-      }
-      // a NaN scale of values: the rows that see its key get NaN in its channels
-      constexpr int kV = kPage * (HD / 32) / 2;   // 32-bit words of value scales
-      const uint32_t* vs = reinterpret_cast<const uint32_t*>(blk + kPage * HD + kPage * (HD / 32) * 2);
-      bool nan = false;
-#pragma unroll
-      for (int i = 0; i < kV / 32; ++i) {
-        const uint32_t x = vs[i * 32 + lane];
-        nan |= (x & 0x7FFFu) >= 0x7F80u || (x & 0x7FFF0000u) >= 0x7F800000u;
-      }
-      if (__any_sync(~0u, nan)) {
-        const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;
-        for (int key = 0; key < kPage; ++key) {
-          if ((lds16(reinterpret_cast<const unsigned char*>(vs) + (key * (HD / 32) + vg) * 2) & 0x7FFFu) < 0x7F80u) continue;
-          const int at = key0 + key;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (at <= last[nt][e] && (a.window <= 0 || at > last[nt][e] - a.window)) {
-#pragma unroll
-                for (int i = 0; i < C::kMT; ++i) acc[i][nt][e] = acc[i][nt][2 + e] = __uint_as_float(0x7FC00000u);
-              }
-        }
-        __syncwarp();
-      }
+      const bool all = Tile<HD, NT, T>::sees_all(a, rd.t, key0);
+#pragma unroll 1
+      for (int kb = 0; kb < kPage; kb += R::kKeys) tile.template keys<R::kKeys>(a, blk, kb, key0, all, lane);
+      tile.template nan_values<kPage>(a, blk, 0, key0, lane);
     }
     __syncwarp();
     if (ua < u1) issue(stage);
-    if (++stage == C::kStages) stage = 0, phase ^= 1;
+    if (++stage == R::kStages) stage = 0, phase ^= 1;
 
     const bool seg_end = rd.page + 1 == rd.t.n;
     if (seg_end || u + 1 == u1) {
       const bool whole = seg_end && seg_first >= u0;
-      const int f0 = rd.t.qt * C::kRows, F = a.S * a.G;
+      const int f0 = rd.t.qt * C::kRows, F = a.S * a.G, g = lane >> 2, t = lane & 3;
       float* slot = a.part + (w * 2 + (seg_first >= u0 ? 1 : 0)) * C::kSlot;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float sum = l[nt][e];
-          sum += __shfl_xor_sync(~0u, sum, 4);
-          sum += __shfl_xor_sync(~0u, sum, 8);
-          sum += __shfl_xor_sync(~0u, sum, 16);
+          const float sum = tile.sum(nt, e);
           const int j = nt * 8 + 2 * t + e, f = f0 + j;
-          if (f >= F) continue;
-          if (whole) {
-            const int s = f / a.G;
-            T* o = static_cast<T*>(a.out) +
-                   (((long long)rd.t.r * a.S + s) * a.Hq + rd.head * a.G + (f - s * a.G)) * HD + g * (C::kVWords * 8);
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+          if (f < F) {
+            const float inv = !whole ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+            T* o = out_row<HD, T>(a, rd.t.r, rd.head, f) + g * (C::kVWords * 8);
+            float* p = slot + j * HD + g * (C::kVWords * 8);
 #pragma unroll
             for (int wd = 0; wd < C::kVWords; ++wd) {
               float x[8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) x[k] = acc[wd * 4 + k][nt][e] * inv, x[4 + k] = acc[wd * 4 + k][nt][2 + e] * inv;
-              if constexpr (C::kF32) {
-                reinterpret_cast<float4*>(o + wd * 8)[0] = make_float4(x[0], x[1], x[2], x[3]);
-                reinterpret_cast<float4*>(o + wd * 8)[1] = make_float4(x[4], x[5], x[6], x[7]);
-              } else {
-                *reinterpret_cast<uint4*>(o + wd * 8) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
-                                                                   pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
-              }
+              for (int k = 0; k < 8; ++k) x[k] = tile.value(wd, k, nt, e) * inv;
+              if (whole) store_row8<T>(o + wd * 8, x);
+              else store_row8<float>(p + wd * 8, x);
             }
-          } else {
-            float* o = slot + j * HD + g * (C::kVWords * 8);
-#pragma unroll
-            for (int wd = 0; wd < C::kVWords; ++wd) {
-              *reinterpret_cast<float4*>(o + wd * 8) = make_float4(acc[wd * 4][nt][e], acc[wd * 4 + 1][nt][e],
-                                                                   acc[wd * 4 + 2][nt][e], acc[wd * 4 + 3][nt][e]);
-              *reinterpret_cast<float4*>(o + wd * 8 + 4) =
-                  make_float4(acc[wd * 4][nt][2 + e], acc[wd * 4 + 1][nt][2 + e], acc[wd * 4 + 2][nt][2 + e],
-                              acc[wd * 4 + 3][nt][2 + e]);
-            }
-            if (g == 0) slot[C::kRows * HD + 2 * j] = m[nt][e], slot[C::kRows * HD + 2 * j + 1] = sum;
+            if (!whole && g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e], slot[C::kRows * HD + 2 * j + 1] = sum;
           }
         }
+      __syncwarp();
     }
     if (u + 1 < u1) {
       if (seg_end) seg_first = u + 1, fresh = true;
@@ -617,18 +750,132 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendA
   }
 }
 
+// ---- one CTA for every (row, query tile, KV head) -----------------------------------------------------------------
+// Slices of 16 keys go round the CTA's warps and their results meet in shared memory: one launch, and the shortest way
+// from the page table to the result.
+template <int HD, int NT, typename T>
+struct Group {
+  using C = Cfg<HD, NT, T>;
+  static constexpr int kWarps = 8, kKeys = 16, kThreads = kWarps * 32;
+  static constexpr int kPages = HD == 64 ? 8 : 4;          // pages in shared memory at a time
+  static constexpr int kJoin = kWarps * C::kSlot * 4;
+  static constexpr int kRing = kPages * C::kBlock > kJoin ? kPages * C::kBlock : kJoin;
+  static constexpr int kSmem = kRing + C::kQBytes + kPages * 16 + 1024;
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+template <int HD, int NT, typename T>
+__global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
+    kv4_attend_group_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap map) {
+  using C = Cfg<HD, NT, T>;
+  using R = Group<HD, NT, T>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* qs = ring + R::kRing;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(qs + C::kQBytes);
+  int* bad = reinterpret_cast<int*>(bars + R::kPages);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const jx_kv4_cache& c = a.c;
+  const int item = blockIdx.x / c.num_kv_heads, head = blockIdx.x - item * c.num_kv_heads;
+  const Item t = item_at<C::kRows>(a, item);
+  const int f0 = t.qt * C::kRows, rows = min(C::kRows, a.S * a.G - f0);
+  if (tid == 0) {
+    prefetch_tmap(&map);
+    if (c.counts[t.r] > a.S) set_status(c.status, JX_ERR_RANGE);
+  }
+  if (t.n == 0) {
+    for (int i = tid; i < rows * HD; i += R::kThreads) out_row<HD, T>(a, t.r, head, f0 + i / HD)[i % HD] = from_f<T>(0.f);
+    return;
+  }
+  int id = -1;
+  if (tid < R::kPages) {
+    mbar_init(&bars[tid], 1);
+    fence_barrier_init();
+    if (tid < t.n) {
+      id = c.table[(long long)t.r * c.row_pages + t.p0 + tid];
+      fetch<HD>(a, &map, id, head, ring + tid * C::kBlock, &bars[tid], &bad[tid]);
+    }
+  }
+  Tile<HD, NT, T> tile;
+  tile.qs = reinterpret_cast<uint4*>(qs);   // one copy for all warps
+  tile.begin(a, t, head, lane, warp == 0);
+  __syncthreads();
+  bool dead = false;
+  for (int first = 0, phase = 0; first < t.n; first += R::kPages, phase ^= 1) {
+    const int here = min(R::kPages, t.n - first);
+    for (int sl = warp; sl < here * (kPage / R::kKeys); sl += R::kWarps) {
+      const int page = sl / (kPage / R::kKeys), kb = sl % (kPage / R::kKeys) * R::kKeys;
+      if (!dead && !__all_sync(~0u, mbar_wait_bounded(&bars[page], phase))) {
+        dead = true;
+        mbar_wait_bounded(&bars[page], phase);   // no copy may be in flight when the CTA ends
+        if (lane == 0) set_status(c.status, JX_ERR_TIMEOUT);
+      }
+      const unsigned char* blk = ring + page * C::kBlock;
+      const int key0 = (t.p0 + first + page) * kPage;
+      if (!dead && !bad[page]) {
+        tile.template keys<R::kKeys>(a, blk, kb, key0, Tile<HD, NT, T>::sees_all(a, t, key0), lane);
+        tile.template nan_values<R::kKeys>(a, blk, kb, key0, lane);
+      }
+    }
+    __syncthreads();
+    if (tid < R::kPages && first + R::kPages + tid < t.n) {
+      id = c.table[(long long)t.r * c.row_pages + t.p0 + first + R::kPages + tid];
+      mbar_wait_bounded(&bars[tid], phase);   // passed already, unless a warp gave up on it
+      fetch<HD>(a, &map, id, head, ring + tid * C::kBlock, &bars[tid], &bad[tid]);
+    }
+    if (first + R::kPages < t.n) __syncthreads();
+  }
+  float* slots = reinterpret_cast<float*>(ring);
+  {
+    float* slot = slots + warp * C::kSlot;
+    const int g = lane >> 2, tq = lane & 3;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float sum = tile.sum(nt, e);
+        const int j = nt * 8 + 2 * tq + e;
+        if (j < rows) {
+#pragma unroll
+          for (int wd = 0; wd < C::kVWords; ++wd) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = tile.value(wd, k, nt, e);
+            store_row8<float>(slot + j * HD + (g * C::kVWords + wd) * 8, x);
+          }
+          if (g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e], slot[C::kRows * HD + 2 * j + 1] = sum;
+        }
+      }
+  }
+  __syncthreads();
+  const int busy = min(R::kWarps, t.n * (kPage / R::kKeys));   // warps that had a slice
+  for (int i = tid; i < rows * (HD / 8); i += R::kThreads) {
+    const int j = i / (HD / 8), d = i % (HD / 8) * 8;
+    float mx = -INFINITY, sum = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int w = 0; w < busy; ++w) mx = fmaxf(mx, slots[w * C::kSlot + C::kRows * HD + 2 * j]);
+    const float use = mx == -INFINITY ? 0.f : mx;
+    for (int w = 0; w < busy; ++w) {
+      const float* slot = slots + w * C::kSlot;
+      const float f = exp2_f(slot[C::kRows * HD + 2 * j] - use);
+      sum = fmaf(slot[C::kRows * HD + 2 * j + 1], f, sum);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = fmaf(slot[j * HD + d + k], f, x[k]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] *= inv;
+    store_row8<T>(out_row<HD, T>(a, t.r, head, f0 + j) + d, x);
+  }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------------
 // Query rows are taken in tiles of 8, 16 or 32: the smallest that holds all S * G rows of a KV head, or 32 (16 where the
 // accumulators of 32 rows would not fit the registers), which then reads every page once per tile.
-int n_tiles_of(int hd, int dtype, int rows) {
+int n_tiles_of(int hd, int dtype, long long rows) {
   const int most = hd == 256 || dtype == JX_F32 ? 2 : 4;
   return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
 }
 
-struct Layout {
-  int nt, tiles;
-  long long items, first_at, total_at, part_at, bytes;
-};
 int sm_count() {
   static int n[64] = {0};
   int dev = 0;
@@ -636,37 +883,86 @@ int sm_count() {
   if (!n[dev] && (cudaDeviceGetAttribute(&n[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n[dev] <= 0)) n[dev] = 148;
   return n[dev];
 }
-constexpr int kMostCtas = 160, kMostWarps = 8;
+
+struct Layout {
+  int nt, tiles;
+  bool group;            // one CTA per (row, tile, head)
+  long long items, first_at, part_at, bytes;
+};
+constexpr int kGroupPages = 16;
+constexpr int kMostCtas = 160, kMostWarps = 12;
 Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int dtype) {
   Layout l;
   const int G = Hq / c.num_kv_heads;
   const long long rows = (long long)S * G;
-  l.nt = n_tiles_of(c.head_dim, dtype, rows > 64 ? 64 : (int)rows);
+  l.nt = n_tiles_of(c.head_dim, dtype, rows);
   l.tiles = (int)((rows + 8 * l.nt - 1) / (8 * l.nt));
   l.items = (long long)c.num_rows * l.tiles;
-  l.total_at = 0;
+  l.group = l.nt <= 2 && c.row_pages <= kGroupPages;
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;
-  l.bytes = l.part_at + (long long)kMostCtas * kMostWarps * 2 * (8 * l.nt) * (c.head_dim + 2) * 4;
+  l.bytes = l.group ? 16 : l.part_at + (long long)kMostCtas * kMostWarps * 2 * (8 * l.nt) * (c.head_dim + 2) * 4;
   return l;
 }
 
-template <int HD, int NT, typename T>
-int launch(AttendArgs& a, cudaStream_t s) {
-  using C = Cfg<HD, NT, T>;
-  static_assert(C::kWarps <= kMostWarps, "workspace");
-  static bool ready[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !ready[dev]) {
-    if (cudaFuncSetAttribute(kv4_attend_kernel<HD, NT, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
-      return JX_ERR_CUDA;
-    if (dev >= 0 && dev < 64) ready[dev] = true;
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  if (!fn) {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
   }
+  return fn;
+}
+
+// The pool as [blocks][144 rows][hd / 2 bytes]; a box is one block, a row as wide as the swizzle.
+int make_map(CUtensorMap* map, const jx_kv4_cache& c) {
+  auto enc = encoder();
+  if (!enc) return JX_ERR_CUDA;
+  const cuuint64_t blocks = (cuuint64_t)c.num_layers * c.num_pages * c.num_kv_heads;
+  const cuuint64_t dims[3] = {(cuuint64_t)c.head_dim / 2, 144, blocks};
+  const cuuint64_t strides[2] = {(cuuint64_t)c.head_dim / 2, (cuuint64_t)kv4_block_bytes(c.head_dim)};
+  const cuuint32_t box[3] = {(cuuint32_t)c.head_dim / 2, 144, 1}, one[3] = {1, 1, 1};
+  const CUtensorMapSwizzle sw = c.head_dim == 64    ? CU_TENSOR_MAP_SWIZZLE_32B
+                                : c.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                    : CU_TENSOR_MAP_SWIZZLE_128B;
+  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pages, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? JX_OK : JX_ERR_ARG;
+}
+
+// Allows a kernel its shared memory, once per device.
+template <typename K>
+int allow(K kernel, int bytes, bool (&ready)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return JX_ERR_CUDA;
+  if (dev >= 0 && dev < 64 && ready[dev]) return JX_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return JX_ERR_CUDA;
+  if (dev >= 0 && dev < 64) ready[dev] = true;
+  return JX_OK;
+}
+
+template <int HD, int NT, typename T>
+int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
+  if constexpr (NT <= 2) {
+    if (l.group) {
+      using R = Group<HD, NT, T>;
+      static bool ready[64];
+      if (const int rc = allow(kv4_attend_group_kernel<HD, NT, T>, R::kSmem, ready)) return rc;
+      kv4_attend_group_kernel<HD, NT, T><<<a.items * a.c.num_kv_heads, R::kThreads, R::kSmem, s>>>(a, map);
+      return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+    }
+  }
+  using R = Runs<HD, NT, T>;
+  static_assert(R::kWarps <= kMostWarps, "workspace");
+  static bool ready[64];
+  if (const int rc = allow(kv4_attend_runs_kernel<HD, NT, T>, R::kSmem, ready)) return rc;
   const long long most = (long long)a.items * a.c.row_pages * a.c.num_kv_heads;   // units there can be
   int grid = sm_count() < kMostCtas ? sm_count() : kMostCtas;
   if (most < grid) grid = (int)most;
-  kv4_attend_kernel<HD, NT, T><<<grid, C::kThreads, C::kSmem, s>>>(a);
+  kv4_attend_runs_kernel<HD, NT, T><<<grid, R::kThreads, R::kSmem, s>>>(a, map);
   if (cudaPeekAtLastError() != cudaSuccess) return JX_ERR_CUDA;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.items * (long long)a.c.num_kv_heads), (unsigned)(a.tiles > 1 || a.S * a.G >= 8 * NT ? 8 * NT : a.S * a.G));
@@ -676,22 +972,22 @@ int launch(AttendArgs& a, cudaStream_t s) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, (const AttendArgs)a, C::kRows) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, a, Cfg<HD, NT, T>::kRows) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
 template <int HD, typename T>
-int launch_nt(int nt, AttendArgs& a, cudaStream_t s) {
-  if (nt == 1) return launch<HD, 1, T>(a, s);
+int launch_nt(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
+  if (l.nt == 1) return launch<HD, 1, T>(l, a, map, s);
   if constexpr (HD < 256 && sizeof(T) == 2)
-    if (nt == 4) return launch<HD, 4, T>(a, s);
-  return launch<HD, 2, T>(a, s);
+    if (l.nt == 4) return launch<HD, 4, T>(l, a, map, s);
+  return launch<HD, 2, T>(l, a, map, s);
 }
 
 template <typename T>
-int launch_hd(int nt, AttendArgs& a, cudaStream_t s) {
-  if (a.c.head_dim == 64) return launch_nt<64, T>(nt, a, s);
-  if (a.c.head_dim == 128) return launch_nt<128, T>(nt, a, s);
-  return launch_nt<256, T>(nt, a, s);
+int launch_hd(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
+  if (a.c.head_dim == 64) return launch_nt<64, T>(l, a, map, s);
+  if (a.c.head_dim == 128) return launch_nt<128, T>(l, a, map, s);
+  return launch_nt<256, T>(l, a, map, s);
 }
 
 }  // namespace
@@ -708,10 +1004,12 @@ int run_kv4_attend(const jx_kv4_cache& c, int layer, int S, int Hq, const void* 
   const int unit = dtype == JX_BF16 ? 8 : 4;
   a.q_vec = !((uintptr_t)q & 15) && !(qs[0] % unit) && !(qs[1] % unit) && !(qs[2] % unit);
   unsigned char* b = static_cast<unsigned char*>(ws);
-  a.total = reinterpret_cast<long long*>(b + l.total_at);
+  a.total = reinterpret_cast<long long*>(b);
   a.item_first = reinterpret_cast<long long*>(b + l.first_at);
   a.part = reinterpret_cast<float*>(b + l.part_at);
-  return dtype == JX_BF16 ? launch_hd<bf16>(l.nt, a, s) : launch_hd<float>(l.nt, a, s);
+  CUtensorMap map;
+  if (const int rc = make_map(&map, c)) return rc;
+  return dtype == JX_BF16 ? launch_hd<bf16>(l, a, map, s) : launch_hd<float>(l, a, map, s);
 }
 
 }  // namespace jxb

@@ -4,7 +4,10 @@ Writing and reading are exact: every value equals the restatement's.  Page manag
 64-bit softmax attention over the same dequantised values; its tolerance counts, with A = sum p |v| of the output element,
   bfloat16: half a step of the output (2^-8 |o|) and of every probability before its product with v (2^-8 A);
   both:     float32 sums of hd terms in a score, each product and sum off by at most 2^-23 of what has been summed
-            (e = hd 2^-23 scale sum |q k|, twice: numerator and normaliser), and of the row's keys (T 2^-23 A).
+            (e = hd 2^-23 scale sum |q k|, twice: numerator and normaliser), and of the row's keys (T 2^-23 A);
+  bfloat16: the kernels sum codes with an offset and take it off again.  A key's group enters as 128 + u with u <= 15 and
+            -136 sum q: what is summed is at most 143 s |q| a channel, over 33 terms (2 * 33 * 2^-23 scale sum 143 s |q|
+            for A).  A value enters as u s and leaves 8 sum p s: at most 15 s each (2 T 2^-23 15 sum p s).
 """
 import random
 
@@ -24,6 +27,14 @@ def _cache(layers, pages, rows, max_len, heads, hd, fill=None):
     if fill is not None:
         c.pages.fill_(fill)
     return c
+
+
+class _Rows(list):
+    """Dequantised rows, and their scales spread over the channels."""
+
+    def __init__(self, xs):
+        super().__init__(K.dequantised(x) for x in xs)
+        self.scale = [K.quantise(x)[1].repeat_interleave(32, -1) for x in xs]
 
 
 def _rand(shape, dtype, seed, scale=1.0):
@@ -116,14 +127,14 @@ def test_append_special_values():
 
 
 # -- attention ----------------------------------------------------------------------------------------------------
-def _filled(rows, lens, counts, heads, hd, seed, fill=0xFF, extra=3, peaky=1.0):
+def _filled(rows, lens, counts, heads, hd, seed, fill=0xFF, extra=3, peaky=1.0, room=0):
     """A cache whose rows hold lens tokens, the last counts of them the current call's; unused pages and slots hold NaN
-    scales.  Returns it and the rows' dequantised keys and values."""
-    width = max(1, -(-max(lens) // PAGE))
+    scales; tables have room for that many pages more than the rows need (long tables take another kernel).  Returns it
+    and the rows' dequantised keys and values."""
+    width = max(1, -(-max(lens) // PAGE)) + room
     c = _cache(1, sum(-(-n // PAGE) for n in lens) + extra, rows, width * PAGE, heads, hd, fill=fill)
     dev = torch.device("cuda")
     older = [n - k for n, k in zip(lens, counts)]
-    kv = [[], []]
     k_all, v_all = _rand((rows, max(lens), heads, hd), torch.float32, seed, peaky), _rand((rows, max(lens), heads, hd),
                                                                                           torch.float32, seed + 1)
     for first, n in ((torch.zeros(rows, dtype=torch.int64), older), (torch.tensor(older), counts)):
@@ -138,10 +149,7 @@ def _filled(rows, lens, counts, heads, hd, seed, fill=0xFF, extra=3, peaky=1.0):
         c.append(0, pick(k_all), pick(v_all))
     c.check()
     assert c.lengths.tolist() == list(lens) and c.counts.tolist() == list(counts)
-    for r in range(rows):
-        kv[0].append(K.dequantised(k_all[r, :lens[r]]))
-        kv[1].append(K.dequantised(v_all[r, :lens[r]]))
-    return c, kv[0], kv[1]
+    return c, _Rows([k_all[r, :lens[r]] for r in range(rows)]), _Rows([v_all[r, :lens[r]] for r in range(rows)])
 
 
 def _check_attend(got, q, ks, vs, lens, counts, scale, window=0):
@@ -160,7 +168,10 @@ def _check_attend(got, q, ks, vs, lens, counts, scale, window=0):
         e = 2 * hd * 2.0 ** -23 * abs(scale) * big[..., None] + lens[r] * 2.0 ** -23
         tol = A[:n] * e + 1e-30
         if q.dtype == torch.bfloat16:
-            tol = tol + 2.0 ** -8 * (want[:n].abs() + A[:n])
+            spread = torch.einsum("shd,thd->sht", q[r, :n].double().abs(), ks.scale[r].repeat_interleave(G, 1)).amax(-1)
+            ps = K.attend(q[r].double(), ks[r], vs.scale[r], lens[r], counts[r], scale, window)[:n]
+            tol = tol + 2.0 ** -8 * (want[:n].abs() + A[:n]) + A[:n] * 2 * 33 * 2.0 ** -23 * abs(scale) * 143 * spread[..., None]
+            tol = tol + 2 * lens[r] * 2.0 ** -23 * 15 * ps
         err = (got[r, :n] - want[:n]).abs()
         assert (err <= tol).all(), (r, (err / tol).max())
 
@@ -172,10 +183,11 @@ SHAPES = [  # heads, kv heads, hd
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("heads,kv,hd", SHAPES)
-@pytest.mark.parametrize("lens", [[1], [64, 1, 63, 65], [0, 129, 700], [130] * 9])
-def test_single_token_attention(dtype, heads, kv, hd, lens):
+@pytest.mark.parametrize("lens,room", [([1], 0), ([64, 1, 63, 65], 0), ([0, 129, 700], 0), ([130] * 9, 0), ([1], 500),
+                                       ([0, 129, 700, 1], 500)])
+def test_single_token_attention(dtype, heads, kv, hd, lens, room):
     counts = [min(1, n) for n in lens]
-    c, ks, vs = _filled(len(lens), lens, counts, kv, hd, seed=heads)
+    c, ks, vs = _filled(len(lens), lens, counts, kv, hd, seed=heads, room=room)
     q = _rand((len(lens), 1, heads, hd), dtype, 5, 1.5)
     got = c.attend(0, q.cuda())
     assert got.dtype == dtype and got.shape == q.shape
@@ -187,8 +199,9 @@ def test_single_token_attention(dtype, heads, kv, hd, lens):
 @pytest.mark.parametrize("heads,kv,hd", [(8, 2, 128), (4, 4, 64), (16, 8, 256), (6, 1, 64)])
 @pytest.mark.parametrize("S,lens,counts", [(2, [2, 66], [2, 1]), (7, [7, 64, 200, 5], [7, 0, 6, 3]), (64, [64, 128], [64, 64]),
                                            (33, [300, 33], [33, 17]), (150, [150, 410], [149, 150])])
-def test_chunks(dtype, heads, kv, hd, S, lens, counts):
-    c, ks, vs = _filled(len(lens), lens, counts, kv, hd, seed=S)
+@pytest.mark.parametrize("room", [0, 500])
+def test_chunks(dtype, heads, kv, hd, S, lens, counts, room):
+    c, ks, vs = _filled(len(lens), lens, counts, kv, hd, seed=S, room=room)
     q = _rand((len(lens), S, heads, hd), dtype, 5)
     for r, n in enumerate(counts):
         q[r, n:] = float("nan")                # padding is not read into anything
@@ -200,10 +213,11 @@ def test_chunks(dtype, heads, kv, hd, S, lens, counts):
 @pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 300, 5000])
 def test_sliding_window(dtype, window):
     for S, lens, counts in ((1, [1, 500, 64], [1, 1, 1]), (70, [70, 333, 100], [70, 69, 0])):
-        c, ks, vs = _filled(3, lens, counts, 2, 64, seed=window)
-        q = _rand((3, S, 6, 64), dtype, 5)
-        got = c.attend(0, q.cuda(), sliding_window=window)
-        _check_attend(got, q, ks, vs, lens, counts, 64 ** -0.5, window)
+        for room in (0, 500):
+            c, ks, vs = _filled(3, lens, counts, 2, 64, seed=window, room=room)
+            q = _rand((3, S, 6, 64), dtype, 5)
+            got = c.attend(0, q.cuda(), sliding_window=window)
+            _check_attend(got, q, ks, vs, lens, counts, 64 ** -0.5, window)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -239,43 +253,57 @@ def test_long_row_is_split_and_joined():
         _check_attend(c.attend(0, q.cuda()), q, ks, vs, lens, counts, 128 ** -0.5)
 
 
-def test_many_rows():
+@pytest.mark.parametrize("room", [0, 500])
+def test_many_rows(room):
     """More rows than multiprocessors, most of them of one or two pages, some empty."""
     rng = random.Random(1)
     lens = [rng.choice([0, 1, 60, 64, 100, 140]) for _ in range(300)]
     counts = [min(1, n) if i % 7 else 0 for i, n in enumerate(lens)]
-    c, ks, vs = _filled(300, lens, counts, 2, 64, seed=8)
+    c, ks, vs = _filled(300, lens, counts, 2, 64, seed=8, room=room)
     q = _rand((300, 1, 4, 64), torch.bfloat16, 5)
     _check_attend(c.attend(0, q.cuda()), q, ks, vs, lens, counts, 64 ** -0.5)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_a_visible_nan_is_seen_and_a_hidden_one_is_not(dtype):
+@pytest.mark.parametrize("max_len,group", [(128, 1), (40000, 1), (128, 2), (40000, 4), (40000, 8)])
+def test_a_visible_nan_is_seen_and_a_hidden_one_is_not(dtype, max_len, group):
     """A key or value group that decodes to NaN reaches the queries that see it, and no other row or query."""
     hd, heads = 64, 2
-    c = _cache(1, 8, 2, 128, heads, hd, fill=0xFF)
+    c = _cache(1, 8, 2, max_len, heads, hd, fill=0xFF)
     k, v = _rand((2, 70, heads, hd), torch.float32, 1), _rand((2, 70, heads, hd), torch.float32, 2)
     k[0, 50, 1, 3] = float("nan")
     v[1, 69, 0, 40] = float("inf")
     c.extend(70)
     c.append(0, k.cuda(), v.cuda())
-    q = _rand((2, 70, 4, hd), dtype, 3)
+    q = _rand((2, 70, heads * group, hd), dtype, 3)
     got = torch.isnan(c.attend(0, q.cuda())).cpu()
     want = torch.zeros_like(got)
-    want[0, 50:, 2:] = True                     # its score is NaN: the whole softmax is
-    want[1, 69, :2, 32:] = True                 # its value is NaN in one group of channels
+    want[0, 50:, group:] = True                 # its score is NaN: the whole softmax is
+    want[1, 69, :group, 32:] = True             # its value is NaN in one group of channels
     assert torch.equal(got, want)
     got = torch.isnan(c.attend(0, q.cuda(), sliding_window=5)).cpu()
     want[0, 55:] = False
     assert torch.equal(got, want)
+    got = torch.isnan(c.attend(0, q[:, -1:].cuda())).cpu()        # one query at a time: counts[r] tokens, the first here
+    assert int(c.status.item()) == 4            # fewer queries than tokens is reported, and nothing is out of range
+    c.status.zero_()
+    c.rollback(1)
+    c.extend(1)
+    c.append(0, k[:, 69:].cuda(), v[:, 69:].cuda())
+    got = torch.isnan(c.attend(0, q[:, -1:].cuda())).cpu()
+    want = torch.zeros_like(got)
+    want[0, 0, group:], want[1, 0, :group, 32:] = True, True
+    assert torch.equal(got, want)
 
 
-def test_page_ids_out_of_range_are_skipped_and_reported():
-    c, ks, vs = _filled(2, [130, 130], [1, 1], 2, 64, seed=4)
+@pytest.mark.parametrize("room", [0, 500])
+def test_page_ids_out_of_range_are_skipped_and_reported(room):
+    c, ks, vs = _filled(2, [130, 130], [1, 1], 2, 64, seed=4, room=room)
     c.table[0, 1], c.table[0, 0] = 1 << 20, -7
     q = _rand((2, 1, 4, 64), torch.bfloat16, 5)
     got = c.attend(0, q.cuda())
-    ks[0], vs[0] = ks[0][128:], vs[0][128:]
+    for x in (ks, vs):
+        x[0], x.scale[0] = x[0][128:], x.scale[0][128:]
     _check_attend(got, q, ks, vs, [2, 130], [1, 1], 0.125)
     with pytest.raises(RuntimeError, match="device status 4"):
         c.check()
@@ -298,8 +326,9 @@ def test_more_tokens_than_queries_is_reported():
         c.check()
 
 
-def test_results_do_not_change_from_run_to_run():
-    c, _, _ = _filled(3, [3000, 40, 700], [1, 1, 1], 4, 128, seed=4)
+@pytest.mark.parametrize("lens", [[3000, 40, 700], [500, 40, 700]])
+def test_results_do_not_change_from_run_to_run(lens):
+    c, _, _ = _filled(3, lens, [1, 1, 1], 4, 128, seed=4)
     q = _rand((3, 1, 16, 128), torch.bfloat16, 5).cuda()
     want = c.attend(0, q)
     for _ in range(20):
