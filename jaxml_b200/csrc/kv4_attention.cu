@@ -31,7 +31,7 @@ namespace {
 struct AttendArgs {
   jx_kv4_cache c;
   int layer, S, Hq, G, window, q_vec, items, tiles;   // tiles: query tiles of a row; items = rows * tiles
-  float scale_log2;
+  float scale_log2, sign;   // |scale| log2(e), at least 1e-30 so that a hidden -inf stays one; its sign, taken into q
   const void* q;
   long long q_row, q_tok, q_head;
   void* out;
@@ -140,7 +140,7 @@ __device__ __forceinline__ long long run_of(long long u, long long units, long l
 
 // ---- loading queries ----------------------------------------------------------------------------------------
 // 8 neighbouring channels as fragment registers (0,4) (1,5) (2,6) (3,7), a float32 split into `parts`.
-__device__ __forceinline__ void q_words(const bf16* p, bool vec, uint4* out) {
+__device__ __forceinline__ void q_words(const bf16* p, bool vec, float sign, uint4* out) {
   uint32_t x[4];
   if (vec) {
     const uint4 u = *reinterpret_cast<const uint4*>(p);
@@ -150,10 +150,12 @@ __device__ __forceinline__ void q_words(const bf16* p, bool vec, uint4* out) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= sign < 0.f ? 0x80008000u : 0u;
   out[0] = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410),
                       __byte_perm(x[1], x[3], 0x7632));
 }
-__device__ __forceinline__ void q_words(const float* p, bool vec, uint4* out) {
+__device__ __forceinline__ void q_words(const float* p, bool vec, float sign, uint4* out) {
   float x[8];
   if (vec) {
     const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
@@ -162,6 +164,8 @@ __device__ __forceinline__ void q_words(const float* p, bool vec, uint4* out) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = p[i];
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= sign;
 #pragma unroll
   for (int part = 0; part < 3; ++part) {
     out[part] = make_uint4(pack_bf16x2(x[0], x[4]), pack_bf16x2(x[1], x[5]), pack_bf16x2(x[2], x[6]), pack_bf16x2(x[3], x[7]));
@@ -180,9 +184,21 @@ struct Tile {
   int last[NT][2];                                // last visible key of the thread's columns (-1: none)
   uint4 q[C::kQReg ? NT : 1][C::kQReg ? C::kQParts : 1][C::kQReg ? C::kGroups : 1];
   uint4* qs;                                      // the fragments in shared memory otherwise
+  int all_hi, all_lo;                             // pages within (all_lo, all_hi] are seen by every row of the tile
+  int k_code, k_scale, v_code[2], v_scale[2];     // the thread's places in a block (swizzled)
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Item& t, int head, int lane, bool store = true) {
     const int g = lane >> 2, tq = lane & 3, f0 = t.qt * C::kRows, F = a.S * a.G;
+    all_hi = f0 + C::kRows <= t.cnt * a.G ? t.base + f0 / a.G : -1;
+    all_lo = a.window > 0 ? t.base + (f0 + C::kRows - 1) / a.G - a.window : -1;
+    // 8 rows of codes are whole periods of the swizzle: what is added to these places below does not change it
+    k_code = HD == 64 ? swz<HD>((((lane >> 4) << 3) + (lane & 7)) * C::kRowBytes + ((lane >> 3) & 1) * 16)
+                      : swz<HD>((lane & 7) * C::kRowBytes + (lane >> 3) * 16);
+    v_code[0] = swz<HD>(2 * tq * C::kRowBytes + g * (C::kVWords * 4)) + kPage * C::kRowBytes;
+    v_code[1] = swz<HD>((2 * tq + 1) * C::kRowBytes + g * (C::kVWords * 4)) + kPage * C::kRowBytes;
+    k_scale = kPage * HD + g * (HD / 16);
+    v_scale[0] = kPage * HD + kPage * (HD / 16) + 2 * tq * (HD / 16) + (HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g) * 2;
+    v_scale[1] = v_scale[0] + 8 * (HD / 16);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -198,7 +214,7 @@ struct Tile {
       for (int i = 0; i < C::kGroups; ++i) {
         uint4 x[C::kQParts];
         if (live) {
-          q_words(src + i * 32 + tq * 8, a.q_vec, x);
+          q_words(src + i * 32 + tq * 8, a.q_vec, a.sign, x);
         } else {
 #pragma unroll
           for (int p = 0; p < C::kQParts; ++p) x[p] = make_uint4(0, 0, 0, 0);
@@ -248,22 +264,19 @@ struct Tile {
       uint32_t kw[2][C::kGroups];
       const int k16 = kb + i * 16;
       if constexpr (HD == 64) {
-        const int key = k16 + ((lane >> 4) << 3) + (lane & 7);
-        ldsm_x4(base + swz<HD>(key * C::kRowBytes + ((lane >> 3) & 1) * 16), kw[0][0], kw[0][1], kw[1][0], kw[1][1]);
+        ldsm_x4(base + k_code + k16 * C::kRowBytes, kw[0][0], kw[0][1], kw[1][0], kw[1][1]);
       } else {
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int w = 0; w < C::kGroups; w += 4) {
-            const int key = k16 + h * 8 + (lane & 7);
-            ldsm_x4(base + swz<HD>(key * C::kRowBytes + (w + (lane >> 3)) * 16), kw[h][w], kw[h][w + 1], kw[h][w + 2],
+          for (int w = 0; w < C::kGroups; w += 4)   // groups 4..7: the fourth bit of the swizzled piece
+            ldsm_x4(base + ((k_code + (k16 + h * 8) * C::kRowBytes) ^ (w * 16)), kw[h][w], kw[h][w + 1], kw[h][w + 2],
                     kw[h][w + 3]);
-          }
       }
       uint32_t ks[2][C::kGroups / 2];   // scales of the two keys, two groups a register
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const unsigned char* p = blk + swz<HD>(kPage * HD + (k16 + h * 8 + g) * (HD / 16));
+        const unsigned char* p = blk + swz<HD>(k_scale + (k16 + h * 8) * (HD / 16));
         if constexpr (HD == 64) {
           ks[h][0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (HD == 128) {
@@ -335,7 +348,7 @@ struct Tile {
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            float x = sc[i][nt][2 * h + e] * a.scale_log2;
+            float x = sc[i][nt][2 * h + e];
             if (!all) {
               const int key = key0 + kb + i * 16 + h * 8 + g;
               if (key > last[nt][e] || (a.window > 0 && key <= last[nt][e] - a.window)) x = -INFINITY;
@@ -347,15 +360,15 @@ struct Tile {
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
         mx = fmaxf(mx, m[nt][e]);
-        const float use = mx == -INFINITY ? 0.f : mx;      // nothing visible yet: every term is 2^-inf
-        f[e] = exp2_f(m[nt][e] - use);
+        const float use = mx == -INFINITY ? 0.f : -mx * a.scale_log2;      // nothing visible yet: every term is 2^-inf
+        f[e] = exp2_f(fmaf(m[nt][e], a.scale_log2, use));
         m[nt][e] = mx;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float x = exp2_f(sc[i][nt][2 * h + e] - use);
+            const float x = exp2_f(fmaf(sc[i][nt][2 * h + e], a.scale_log2, use));
             sc[i][nt][2 * h + e] = x;
             sum += x;
           }
@@ -382,15 +395,13 @@ struct Tile {
           }
         }
     }
-    const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;   // the thread's channels are of one group
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) {
       const int k16 = kb + i * 16;
       uint32_t vw[4][C::kVWords], s2[2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int key = k16 + 2 * t + (j & 1) + (j >> 1) * 8;
-        const unsigned char* p = blk + swz<HD>(kPage * C::kRowBytes + key * C::kRowBytes + g * (C::kVWords * 4));
+      for (int j = 0; j < 4; ++j) {   // keys 2t, 2t + 1, 2t + 8, 2t + 9
+        const unsigned char* p = blk + v_code[j & 1] + (k16 + (j >> 1) * 8) * C::kRowBytes;
         if constexpr (C::kVWords == 4) {
           const uint4 x = *reinterpret_cast<const uint4*>(p);
           vw[j][0] = x.x, vw[j][1] = x.y, vw[j][2] = x.z, vw[j][3] = x.w;
@@ -402,12 +413,9 @@ struct Tile {
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int o = kPage * HD + kPage * (HD / 16) + (k16 + 2 * t + h * 8) * (HD / 16) + vg * 2;
-        const uint32_t s = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
-        // NaN and infinity to finite: a key that a row does not see has P = 0 there, and 0 * NaN would reach it.  Rows that
-        // do see one get NaN in nan_values.  2^120 is above every scale that the format has.
-        s2[h] = as_u(__hmin2(__hmax2(as_b2(s), as_b2(0u)), as_b2(0x7B807B80u)));
+      for (int h = 0; h < 2; ++h) {   // the thread's channels are of one group
+        const int o = v_scale[h] + k16 * (HD / 16);
+        s2[h] = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
       }
       uint32_t c2[2];
       if constexpr (C::kRaw) {
@@ -441,40 +449,57 @@ struct Tile {
     }
   }
 
-  // Where a value scale of keys [kb, kb + KT) is NaN, the rows that see its key get NaN in its channels.
+  // Where a value scale of keys [kb, kb + KT) is not finite, the rows that see its key get NaN in its channels, and the scale
+  // in shared memory becomes 0: a row that does not see the key has P = 0 there, and 0 * NaN would reach it.  Runs before
+  // keys().
   template <int KT>
-  __device__ __forceinline__ void nan_values(const AttendArgs& a, const unsigned char* blk, int kb, int key0, int lane) {
-    constexpr int kV = KT * (HD / 32) / 2;   // 32-bit words of value scales
-    const int at = kPage * HD + kPage * (HD / 16), g = lane >> 2;
-    bool nan = false;
+  __device__ __forceinline__ void nan_values(const AttendArgs& a, unsigned char* blk, int kb, int key0, int lane) {
+    constexpr int kBytes = KT * (HD / 16), kEach = kBytes >= 512 ? 16 : kBytes >= 256 ? 8 : 4;
+    const int at = kPage * HD + kPage * (HD / 16) + kb * (HD / 16), g = lane >> 2;
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < (kV + 31) / 32; ++i) {
-      const uint32_t x = i * 32 + lane < kV
-                             ? *reinterpret_cast<const uint32_t*>(blk + swz<HD>(at + kb * (HD / 16) + (i * 32 + lane) * 4)) : 0u;
-      nan |= (x & 0x7FFFu) >= 0x7F80u || (x & 0x7FFF0000u) >= 0x7F800000u;
+    for (int i = 0; i < kBytes; i += kEach * 32) {
+      const int o = i + lane * kEach;
+      if (o < kBytes) {
+        const uint32_t* x = reinterpret_cast<const uint32_t*>(blk + swz<HD>(at + o));
+        uint32_t w[4] = {0, 0, 0, 0};
+        if constexpr (kEach == 16) {
+          const uint4 v = *reinterpret_cast<const uint4*>(x);
+          w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else if constexpr (kEach == 8) {
+          const uint2 v = *reinterpret_cast<const uint2*>(x);
+          w[0] = v.x, w[1] = v.y;
+        } else {
+          w[0] = *x;
+        }
+#pragma unroll
+        for (int j = 0; j < kEach / 4; ++j) top |= (w[j] & 0x7F807F80u) + 0x00800080u;   // an exponent of ones carries
+      }
     }
-    if (!__any_sync(~0u, nan)) return;
+    if (!__any_sync(~0u, top & 0x80008000u)) return;
     const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;
-    for (int key = kb; key < kb + KT; ++key) {
+    for (int key = 0; key < KT; ++key) {
       if ((lds16(blk + swz<HD>(at + key * (HD / 16) + vg * 2)) & 0x7FFFu) < 0x7F80u) continue;
+      const int pos = key0 + kb + key;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (key0 + key <= last[nt][e] && (a.window <= 0 || key0 + key > last[nt][e] - a.window)) {
+          if (pos <= last[nt][e] && (a.window <= 0 || pos > last[nt][e] - a.window)) {
 #pragma unroll
             for (int i = 0; i < C::kMT; ++i) acc[i][nt][e] = acc[i][nt][2 + e] = __uint_as_float(0x7FC00000u);
           }
     }
     __syncwarp();
+    for (int i = lane; i < kBytes / 2; i += 32) {
+      uint16_t* s = reinterpret_cast<uint16_t*>(blk + swz<HD>(at + i * 2));
+      if ((*s & 0x7FFFu) >= 0x7F80u) *s = 0;
+    }
+    fence_proxy_async();   // the next copy writes here
+    __syncwarp();
   }
 
-  // Whether every key of a page is seen by every row of the tile (all of them there).
-  static __device__ __forceinline__ bool sees_all(const AttendArgs& a, const Item& t, int key0) {
-    const int f0 = t.qt * C::kRows, f1 = f0 + C::kRows;
-    return f1 <= t.cnt * a.G && key0 + kPage - 1 <= t.base + f0 / a.G &&
-           (a.window <= 0 || key0 > t.base + (f1 - 1) / a.G - a.window);
-  }
+  __device__ __forceinline__ bool sees_all(int key0) const { return key0 + kPage - 1 <= all_hi && key0 > all_lo; }
 
   // The column's sum over the warp; the 8 kVWords channels of the thread and column.
   __device__ __forceinline__ float sum(int nt, int e) const {
@@ -649,13 +674,13 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
       for (int s = 0; s < R::kStages; ++s) mbar_wait_bounded(&my_bar[s], s < stage ? phase ^ 1 : phase);
       return;
     }
-    const unsigned char* blk = my_ring + stage * C::kBlock;
+    unsigned char* blk = my_ring + stage * C::kBlock;
     const int key0 = (rd.t.p0 + rd.page) * kPage;
     if (!my_bad[stage]) {
-      const bool all = Tile<HD, NT, T>::sees_all(a, rd.t, key0);
+      const bool all = tile.sees_all(key0);
+      tile.template nan_values<kPage>(a, blk, 0, key0, lane);
 #pragma unroll 1
       for (int kb = 0; kb < kPage; kb += R::kKeys) tile.template keys<R::kKeys>(a, blk, kb, key0, all, lane);
-      tile.template nan_values<kPage>(a, blk, 0, key0, lane);
     }
     __syncwarp();
     if (ua < u1) issue(stage);
@@ -684,7 +709,7 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
               if (whole) store_row8<T>(o + wd * 8, x);
               else store_row8<float>(p + wd * 8, x);
             }
-            if (!whole && g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e], slot[C::kRows * HD + 2 * j + 1] = sum;
+            if (!whole && g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e] * a.scale_log2, slot[C::kRows * HD + 2 * j + 1] = sum;
           }
         }
       __syncwarp();
@@ -810,11 +835,11 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
         mbar_wait_bounded(&bars[page], phase);   // no copy may be in flight when the CTA ends
         if (lane == 0) set_status(c.status, JX_ERR_TIMEOUT);
       }
-      const unsigned char* blk = ring + page * C::kBlock;
+      unsigned char* blk = ring + page * C::kBlock;
       const int key0 = (t.p0 + first + page) * kPage;
       if (!dead && !bad[page]) {
-        tile.template keys<R::kKeys>(a, blk, kb, key0, Tile<HD, NT, T>::sees_all(a, t, key0), lane);
         tile.template nan_values<R::kKeys>(a, blk, kb, key0, lane);
+        tile.template keys<R::kKeys>(a, blk, kb, key0, tile.sees_all(key0), lane);
       }
     }
     __syncthreads();
@@ -843,7 +868,7 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
             for (int k = 0; k < 8; ++k) x[k] = tile.value(wd, k, nt, e);
             store_row8<float>(slot + j * HD + (g * C::kVWords + wd) * 8, x);
           }
-          if (g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e], slot[C::kRows * HD + 2 * j + 1] = sum;
+          if (g == 0) slot[C::kRows * HD + 2 * j] = tile.m[nt][e] * a.scale_log2, slot[C::kRows * HD + 2 * j + 1] = sum;
         }
       }
   }
@@ -999,7 +1024,8 @@ int run_kv4_attend(const jx_kv4_cache& c, int layer, int S, int Hq, const void* 
   const Layout l = layout_of(c, S, Hq, dtype);
   AttendArgs a;
   a.c = c, a.layer = layer, a.S = S, a.Hq = Hq, a.G = Hq / c.num_kv_heads, a.window = window;
-  a.items = (int)l.items, a.tiles = l.tiles, a.scale_log2 = scale * 1.4426950408889634f;
+  a.items = (int)l.items, a.tiles = l.tiles, a.sign = scale < 0.f ? -1.f : 1.f;
+  a.scale_log2 = fmaxf(fabsf(scale) * 1.4426950408889634f, 1e-30f);
   a.q = q, a.q_row = qs[0], a.q_tok = qs[1], a.q_head = qs[2], a.out = out;
   const int unit = dtype == JX_BF16 ? 8 : 4;
   a.q_vec = !((uintptr_t)q & 15) && !(qs[0] % unit) && !(qs[1] % unit) && !(qs[2] % unit);
