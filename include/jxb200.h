@@ -543,8 +543,8 @@ int jx_kv4_compact(const jx_kv4_cache* cache, int* used, int* ws, long long ws_i
 /* ---- scoring (beside the filters and draws of inference_engine/sampling.py:34-188) ----
  * Of every logits row x [V]: log_probs = x[id] - log sum exp x (0 for a negative id, NaN for id >= V), entropy of
  * softmax(x), and the top_n largest entries' ids (equal values: lowest id first) with their log probabilities.  Entries
- * of -inf have probability 0; a row with NaN or +inf, or without a finite entry, has NaN results and the ids that its
- * order gives.  top_n <= 64 and <= V. */
+ * of -inf have probability 0; a row with NaN or +inf, or without a finite entry, has NaN results (ids of -1 where it
+ * has NaN).  top_n <= 64 and <= V, V <= 2^30. */
 typedef struct jx_log_probs_args {
   int rows, V;
   const void* logits;

@@ -527,6 +527,7 @@ int jx_token_log_probs(const jx_log_probs_args* args, void* stream) {
     return fail(JX_ERR_ARG, "jx_token_log_probs: null pointer");
   if (args->rows <= 0 || args->V <= 0 || (args->rows > 1 && args->ld < args->V))
     return fail(JX_ERR_SHAPE, "jx_token_log_probs: sizes must be positive and rows must not overlap");
+  if (args->V > (1 << 30)) return fail(JX_ERR_SHAPE, "jx_token_log_probs: V must be at most 2^30");
   if (args->top_n < 0 || args->top_n > 64 || args->top_n > args->V)
     return fail(JX_ERR_SHAPE, "jx_token_log_probs: 0 <= top_n <= min(64, V)");
   if (args->top_n && (!args->top_log_probs || !args->top_ids))

@@ -2,7 +2,17 @@
 //
 // With m the row's maximum, z = sum exp(x - m) and w = sum exp(x - m) (x - m):
 //   log p(id) = (x[id] - m) - log z,   entropy = log z - w / z.
-// One CTA per row; the alternatives are taken one after the other in the order of (value, lowest id).
+// One reading of the row: a thread keeps its own m, z and w and moves z and w to a new maximum when a batch of its
+// elements brings one (z' = z f, w' = f (w + z (m - m'))).  x - m is formed before anything is scaled, so it is exact near the
+// maximum whatever the logits' offset.
+//
+// The alternatives come from the maxima of the threads and of their batches.  t, the top_n-th largest of the threads'
+// maxima, is a lower bound of every element wanted, and the larger elements lie in batches (whose maxima stay in shared
+// memory) of fewer than top_n threads: only those are read again.  Elements equal to t are taken in the order of their
+// index until top_n are there.
+//
+// What bounds it is the reading of the logits.  Few rows are split over a cluster of CTAs, whose results meet in the
+// first one's shared memory.
 #include <math.h>
 
 #include "common.cuh"
@@ -10,72 +20,464 @@
 namespace jxb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kSlots = 32;        // batch maxima a thread keeps; a batch is 4 vectors times a whole number of rounds
+constexpr int kCand = 1024;       // elements above t that fit; more (all in a few batches) take the slow way
+constexpr int kMostTop = 64;
 
-// Order-preserving integer of a float: -0 equals +0, NaN is above infinity.
+__device__ __forceinline__ float nan_f() { return __uint_as_float(0x7FC00000u); }
+// Order-preserving integer of a float: -0 equals +0.
 __device__ __forceinline__ uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
-
-template <typename V, typename Op>
-__device__ __forceinline__ V block_reduce(V v, V* sh, Op op) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int d = 16; d; d >>= 1) v = op(v, __shfl_xor_sync(~0u, v, d));
-  __syncthreads();
-  if (lane == 0) sh[warp] = v;
-  __syncthreads();
-  V r = sh[0];
-  for (int i = 1; i < kThreads / 32; ++i) r = op(r, sh[i]);
+__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float exp2_f(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
 
+// (m, z, w) of a set of elements.
+struct Sums {
+  float m, z, w;
+};
+// exp(d) for d = m - m' of two maxima, 1 where both are the same (also -inf), 0 for an empty side.
+__device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
+  Sums r;
+  r.m = max_nan(a.m, b.m);
+  const float da = a.m == r.m ? 0.f : fmaxf(a.m - r.m, -1e30f), db = b.m == r.m ? 0.f : fmaxf(b.m - r.m, -1e30f);
+  const float fa = exp2_f(da * 1.4426950408889634f), fb = exp2_f(db * 1.4426950408889634f);
+  r.z = a.z * fa + b.z * fb;
+  r.w = fa * (a.w + a.z * da) + fb * (b.w + b.z * db);
+  return r;
+}
+
+// A row's (or a slice's) elements as 16-byte vectors on 16-byte boundaries; what lies outside reads as -inf.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) log_probs_kernel(const jx_log_probs_args a) {
-  __shared__ float sf[kThreads / 32];
-  __shared__ unsigned long long sk[kThreads / 32];
-  const int row = blockIdx.x, tid = threadIdx.x, V = a.V;
-  const T* x = static_cast<const T*>(a.logits) + (long long)row * a.ld;
+struct Row {
+  static constexpr int kE = 16 / sizeof(T);
+  const T* base;       // on a 16-byte boundary, at or before the row
+  int first, last;     // elements of the row are [first, last) of base
+  __device__ __forceinline__ bool inside(int v) const { return v * kE >= first && v * kE + kE <= last; }
+  __device__ __forceinline__ uint4 load(int v) const {
+    if (inside(v)) return __ldcs(reinterpret_cast<const uint4*>(base) + v);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const uint16_t* h = reinterpret_cast<const uint16_t*>(base);
+        const int e = v * kE + 2 * i;
+        w[i] = (e >= first && e < last ? h[e] : 0xFF80u) | (uint32_t)(e + 1 >= first && e + 1 < last ? h[e + 1] : 0xFF80u) << 16;
+      } else {
+        const int e = v * kE + i;
+        w[i] = e >= first && e < last ? reinterpret_cast<const uint32_t*>(base)[e] : 0xFF800000u;
+      }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  // Elements of a vector as floats.
+  static __device__ __forceinline__ void floats(const uint4& u, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      else x[i] = __uint_as_float(w[i]);
+    }
+  }
+  static __device__ __forceinline__ float max_of(const uint4& a, const uint4& b, const uint4& c, const uint4& d) {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[16] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+      uint32_t m = w[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w[i]));
+      return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
+    } else {
+      const uint32_t w[16] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w, d.x, d.y, d.z, d.w};
+      float m = __uint_as_float(w[0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) m = max_nan(m, __uint_as_float(w[i]));
+      return m;
+    }
+  }
+};
+
+struct Shared {
+  uint32_t slot[kSlots][kThreads];              // order keys of the batches' maxima
+  unsigned long long cand[kCand];               // order key << 32 | ~index
+  unsigned long long list[kMostTop];            // this CTA's best, unordered
+  __align__(16) uint32_t best[kThreads];        // order keys of the threads' maxima
+  Sums sums[kWarps];
+  Sums mine;
+  int scan[kWarps + 1];
+  uint32_t bound;
+  int n_cand, n_list;
+};
+
+// Exclusive sum over the CTA's threads.
+__device__ __forceinline__ int block_exclusive(int x, int* sh, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int v = x;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int o = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += o;
+  }
+  __syncthreads();
+  if (lane == 31) sh[warp] = v;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sh[w];
+    all += sh[w];
+  }
+  *total = all;
+  return before + v - x;
+}
+
+// The want-th largest of the maxima of kThreads / kEach groups of neighbouring threads (all threads; 1 <= want <= groups).
+template <int kEach>
+__device__ __forceinline__ uint32_t nth_largest(Shared& s, uint32_t mine, int want) {
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int d = 1; d < kEach; d <<= 1) mine = max(mine, __shfl_xor_sync(~0u, mine, d));
+  if (tid % kEach == 0) s.best[tid / kEach] = mine;
+  __syncthreads();
+  if (tid < kThreads / kEach) {
+    mine = s.best[tid];
+    int above = 0;
+    const uint4* all = reinterpret_cast<const uint4*>(s.best);
+#pragma unroll 4
+    for (int i = 0; i < kThreads / kEach / 4; ++i) {
+      const uint4 k = all[i];
+      // of equal keys the lower place's counts as larger: ranks are distinct
+      above += (k.x > mine || (k.x == mine && 4 * i < tid)) + (k.y > mine || (k.y == mine && 4 * i + 1 < tid)) +
+               (k.z > mine || (k.z == mine && 4 * i + 2 < tid)) + (k.w > mine || (k.w == mine && 4 * i + 3 < tid));
+    }
+    if (above == want - 1) s.bound = mine;
+  }
+  __syncthreads();
+  return s.bound;
+}
+
+// The top_n largest elements of the slice into s.list (all threads); n_list of them.
+template <typename T>
+__device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rounds_per_slot, int slots, int top_n) {
+  constexpr int kE = Row<T>::kE;
+  const int tid = threadIdx.x;
+  const int size = min(v1 * kE, row.last) - max(v0 * kE, row.first);   // elements of the slice
+  const int want = min(top_n, max(size, 0));
+  if (want == 0) return;
+  // a thread without an element has key 0, below that of -inf: with fewer threads at work than elements wanted all count
+  uint32_t mine = 0;
+  for (int i = 0; i < slots; ++i) mine = max(mine, s.slot[i][tid]);
+  // 64 groups are as good a bound for few elements and cost a sixteenth of the comparisons
+  const uint32_t t = want <= 32 ? nth_largest<4>(s, mine, want) : nth_largest<1>(s, mine, want);
+  const int per = rounds_per_slot;
+  auto each = [&](int slot, auto&& f) {   // this thread's elements of a slot
+    for (int r = slot * per; r < slot * per + per; ++r) {
+      uint4 u[4];
+      const int v = v0 + r * 4 * kThreads + tid;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (v + j * kThreads >= v1) continue;
+        float x[kE];
+        Row<T>::floats(u[j], x);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) {
+          const int i = (v + j * kThreads) * kE + e;
+          if (i >= row.first && i < row.last) f(order_key(x[e]), i - row.first);
+        }
+      }
+    }
+  };
+  auto collect = [&](uint32_t from) {     // all elements of that key or above; how many
+    if (tid == 0) s.n_cand = 0;
+    __syncthreads();
+    for (int i = 0; mine >= from && i < slots; ++i)
+      if (s.slot[i][tid] >= from)
+        each(i, [&](uint32_t k, int at) {
+          if (k >= from) {
+            const int p = atomicAdd(&s.n_cand, 1);
+            if (p < kCand) s.cand[p] = ((unsigned long long)k << 32) | (uint32_t)~at;
+          }
+        });
+    __syncthreads();
+    return s.n_cand;
+  };
+  int n = collect(t);
+  if (n > kCand) {          // so many equal to t: those above it, then the equal ones by index
+    __syncthreads();
+    n = collect(t + 1);
+  }
+  if (n > kCand) {
+    // too many above t in a few batches: one after the other
+    unsigned long long below = ~0ull;
+    for (int k = 0; k < want; ++k) {
+      unsigned long long best = 0;
+      for (int i = 0; i < slots; ++i)
+        each(i, [&](uint32_t key, int at) {
+          const unsigned long long c = ((unsigned long long)key << 32) | (uint32_t)~at;
+          if (c < below && c > best) best = c;
+        });
+      for (int d = 16; d; d >>= 1) {
+        const unsigned long long o = __shfl_xor_sync(~0u, best, d);
+        best = o > best ? o : best;
+      }
+      __syncthreads();
+      if ((tid & 31) == 0) s.cand[tid >> 5] = best;
+      __syncthreads();
+      for (int w = 0; w < kWarps; ++w) best = s.cand[w] > best ? s.cand[w] : best;
+      below = best;
+      if (tid == 0) s.list[k] = best, s.n_list = k + 1;
+    }
+    __syncthreads();
+    return;
+  }
+  // the candidates' ranks; the best go to the list
+  for (int i = tid; i < n; i += kThreads) {
+    const unsigned long long c = s.cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += s.cand[j] > c;
+    if (rank < want) s.list[rank] = c;
+  }
+  if (n < want) {   // elements equal to t, by index: rounds in order, in a round the vectors in order
+    int found = n;
+    for (int i = 0; i < slots && found < want; ++i) {
+      const bool holds = s.slot[i][tid] >= t;
+      if (!__syncthreads_or(holds)) continue;
+      for (int r = i * per; r < i * per + per && found < want; ++r)
+        for (int j = 0; j < 4 && found < want; ++j) {
+          const int v = v0 + (r * 4 + j) * kThreads + tid;
+          uint32_t hit = 0;
+          if (holds && v < v1) {
+            float x[kE];
+            Row<T>::floats(row.load(v), x);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+              const int at = v * kE + e;
+              if (at >= row.first && at < row.last && order_key(x[e]) == t) hit |= 1u << e;
+            }
+          }
+          int total, p = found + block_exclusive(__popc(hit), s.scan, &total);
+          for (; hit && p < want; hit &= hit - 1, ++p)
+            s.list[p] = ((unsigned long long)t << 32) | (uint32_t)~(v * kE + __ffs(hit) - 1 - row.first);
+          found += total;
+        }
+    }
+  }
+  if (tid == 0) s.n_list = want;
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 5) log_probs_kernel(const jx_log_probs_args a, int rounds_per_slot) {
+  extern __shared__ __align__(16) unsigned char smem[];
+  Shared& s = *reinterpret_cast<Shared*>(smem);
+  constexpr int kE = Row<T>::kE;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
+  const int r = blockIdx.x / C;
+  const T* x = static_cast<const T*>(a.logits) + (long long)r * a.ld;
+  Row<T> row;
+  row.first = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+  row.base = x - row.first;
+  row.last = row.first + a.V;
+  const int nv = (row.last + kE - 1) / kE;
+  const int v0 = (int)((long long)nv * rank / C), v1 = (int)((long long)nv * (rank + 1) / C);
+  const int rounds = (v1 - v0 + 4 * kThreads - 1) / (4 * kThreads);
+  const int slots = (rounds + rounds_per_slot - 1) / rounds_per_slot;
+
   float m = -INFINITY;
-  for (int i = tid; i < V; i += kThreads) m = fmaxf(m, to_f(x[i]));
-  m = block_reduce(m, sf, [](float p, float q) { return fmaxf(p, q); });
-  float z = 0.f, w = 0.f;
-  for (int i = tid; i < V; i += kThreads) {
-    const float d = to_f(x[i]) - m, e = expf(d);
-    z += e;
-    if (e != 0.f) w += e * d;
+  uint64_t z2 = pack2(0.f, 0.f), w2 = z2;
+  const uint64_t c2 = pack2(1.4426950408889634f, 1.4426950408889634f);
+  const uint4 none = sizeof(T) == 2 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
+                                    : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
+  int round = 0;
+  for (int i = 0; i < slots; ++i) {
+    float slot_max = -INFINITY;
+    bool any = false;
+    for (int k = 0; k < rounds_per_slot && round < rounds; ++k, ++round) {
+      const int v = v0 + round * 4 * kThreads + tid;
+      uint4 u[4];
+      if (v0 + (round + 1) * 4 * kThreads <= v1 && round > 0 && (round + 1 < rounds || row.inside(v1 - 1))) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(row.base) + v + j * kThreads);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : none;
+      }
+      any |= v < v1;
+      const float bm = Row<T>::max_of(u[0], u[1], u[2], u[3]);
+      slot_max = max_nan(slot_max, bm);
+      if (!(bm <= m)) {   // a new maximum (or NaN)
+        if (m != -INFINITY) {
+          const float d = fmaxf(m - bm, -1e30f), f = exp2_f(d * 1.4426950408889634f);
+          w2 = mul2(pack2(f, f), fma2(z2, pack2(d, d), w2));
+          z2 = mul2(pack2(f, f), z2);
+        }
+        m = max_nan(m, bm);
+      }
+      const uint64_t nm = pack2(-m, -m);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float e[kE];
+        Row<T>::floats(u[j], e);
+#pragma unroll
+        for (int p = 0; p < kE; p += 2) {
+          float d0, d1, y0, y1;
+          unpack2(add2(pack2(e[p], e[p + 1]), nm), d0, d1);
+          d0 = fmaxf(d0, -1e30f), d1 = fmaxf(d1, -1e30f);     // -inf (and, with m, NaN): a probability of 0 without 0 * inf
+          const uint64_t d = pack2(d0, d1);
+          unpack2(mul2(d, c2), y0, y1);
+          const uint64_t y = pack2(exp2_f(y0), exp2_f(y1));
+          z2 = add2(z2, y);
+          w2 = fma2(y, d, w2);
+        }
+      }
+    }
+    if (a.top_n) s.slot[i][tid] = any ? order_key(slot_max) : 0u;
   }
-  z = block_reduce(z, sf, [](float p, float q) { return p + q; });
-  w = block_reduce(w, sf, [](float p, float q) { return p + q; });
-  const float lz = logf(z);
+  Sums t;
+  {
+    float a0, a1;
+    t.m = m;
+    unpack2(z2, a0, a1);
+    t.z = a0 + a1;
+    unpack2(w2, a0, a1);
+    t.w = a0 + a1;
+  }
+#pragma unroll
+  for (int d = 16; d; d >>= 1) {
+    Sums o;
+    o.m = __shfl_xor_sync(~0u, t.m, d), o.z = __shfl_xor_sync(~0u, t.z, d), o.w = __shfl_xor_sync(~0u, t.w, d);
+    // the lower lane's first on both sides: one result for the warp
+    t = lane & d ? joined(o, t) : joined(t, o);
+  }
+  if (lane == 0) s.sums[warp] = t;
+  __syncthreads();
+  t = s.sums[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) t = joined(t, s.sums[w]);
+  if (tid == 0) s.mine = t, s.n_list = 0;
+  if (a.top_n) {
+    if (t.m == t.m) select_top<T>(s, row, v0, v1, rounds_per_slot, slots, a.top_n);   // no order with NaN
+  }
+  if (C > 1) {
+    cluster_sync_all();
+    if (rank == 0) {
+      t = s.mine;
+      for (int q = 1; q < C; ++q) {
+        const uint32_t at = dsmem_map(smem_u32(&s.mine), q);
+        Sums o;
+        o.m = dsmem_ld_f32(at), o.z = dsmem_ld_f32(at + 4), o.w = dsmem_ld_f32(at + 8);
+        t = joined(t, o);
+      }
+      // every CTA's list behind the others in the candidates
+      int n = 0;
+      if (a.top_n) {
+        for (int q = 0; q < C; ++q) {
+          const int have = q == 0 ? s.n_list : __float_as_int(dsmem_ld_f32(dsmem_map(smem_u32(&s.n_list), q)));
+          const uint32_t at = dsmem_map(smem_u32(&s.list[0]), q);
+          if (tid < have) {
+            const uint32_t lo = __float_as_uint(dsmem_ld_f32(at + tid * 8)), hi = __float_as_uint(dsmem_ld_f32(at + tid * 8 + 4));
+            s.cand[n + tid] = ((unsigned long long)hi << 32) | lo;
+          }
+          n += have;
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < n; i += kThreads) {
+        const unsigned long long c = s.cand[i];
+        int k = 0;
+        for (int j = 0; j < n; ++j) k += s.cand[j] > c;
+        if (k < a.top_n) s.list[k] = c;
+      }
+      __syncthreads();
+    }
+    cluster_sync_all();      // the others' shared memory is read until here
+    if (rank != 0) return;
+  } else {
+    __syncthreads();
+  }
+  const float lz = logf(t.z);
   if (tid == 0) {
-    const int id = a.ids[row];
-    a.log_probs[row] = id < 0 ? 0.f : id >= V ? __uint_as_float(0x7FC00000u) : (to_f(x[id]) - m) - lz;
-    a.entropy[row] = lz - w / z;
+    const int id = a.ids[r];
+    a.log_probs[r] = id < 0 ? 0.f : id >= a.V || t.m != t.m ? nan_f() : (to_f(x[id]) - t.m) - lz;
+    a.entropy[r] = t.m != t.m ? nan_f() : lz - t.w / t.z;
   }
-  unsigned long long below = ~0ull;
-  for (int n = 0; n < a.top_n; ++n) {
-    unsigned long long best = 0;
-    for (int i = tid; i < V; i += kThreads) {
-      const unsigned long long k = ((unsigned long long)order_key(to_f(x[i])) << 32) | (uint32_t)~i;
-      if (k < below && k > best) best = k;
-    }
-    best = block_reduce(best, sk, [](unsigned long long p, unsigned long long q) { return p > q ? p : q; });
-    below = best;
-    if (tid == 0) {
-      const int id = (int)~(uint32_t)best;
-      a.top_ids[(long long)row * a.top_n + n] = id;
-      a.top_log_probs[(long long)row * a.top_n + n] = (to_f(x[id]) - m) - lz;
-    }
+  if (tid < a.top_n) {
+    const bool fine = t.m == t.m;
+    const unsigned long long c = fine ? s.list[tid] : 0;
+    a.top_ids[(long long)r * a.top_n + tid] = fine ? (int)~(uint32_t)c : -1;
+    a.top_log_probs[(long long)r * a.top_n + tid] = fine ? (key_value((uint32_t)(c >> 32)) - t.m) - lz : nan_f();
   }
+}
+
+template <typename T>
+int launch(const jx_log_probs_args& a, cudaStream_t s) {
+  // CTAs per row: enough for three on every multiprocessor, while a slice keeps two rounds of vectors
+  const int e = 16 / (int)sizeof(T);
+  int C = 1;
+  while (C < 8 && (long long)a.rows * C < 3 * 148 && a.V / (2 * C) >= 2 * kThreads * 4 * e / 4) C *= 2;
+  const long long nv = ((long long)a.V + e - 1) / e + 1;      // a row off its boundary has one vector more
+  const long long per_cta = (nv + C - 1) / C;
+  const long long rounds = (per_cta + 4 * kThreads - 1) / (4 * kThreads);
+  const int per_slot = (int)((rounds + kSlots - 1) / kSlots);
+  const int smem = (int)sizeof(Shared);
+  static bool ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return JX_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(log_probs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return JX_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)a.rows * C);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = C, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, a, per_slot) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
 }  // namespace
 
 int run_token_log_probs(const jx_log_probs_args& a, cudaStream_t s) {
-  if (a.dtype == JX_BF16) log_probs_kernel<bf16><<<a.rows, kThreads, 0, s>>>(a);
-  else log_probs_kernel<float><<<a.rows, kThreads, 0, s>>>(a);
-  return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return a.dtype == JX_BF16 ? launch<bf16>(a, s) : launch<float>(a, s);
 }
 
 }  // namespace jxb

@@ -286,7 +286,7 @@ def token_log_probs(logits: torch.Tensor, token_ids, top_n: int = 0) -> TokenLog
 
     Filtered entries (-inf) have probability 0 and log probability -inf.  A negative id asks for nothing and gives 0;
     an id of V or more gives NaN, and so do a row's results when it has NaN or +inf logits or no finite one (the
-    device is not synchronised to raise)."""
+    device is not synchronised to raise; with NaN its ``top_ids`` are -1)."""
     from . import _native as N
 
     if not isinstance(logits, torch.Tensor) or logits.device.type != "cuda":

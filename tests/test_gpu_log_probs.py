@@ -31,6 +31,7 @@ def _check(x, ids, top_n, got):
     fine = torch.isfinite(x.amax(-1)) & ~torch.isnan(x).any(-1)
     assert torch.isnan(ent[~fine]).all() and torch.isnan(lp[~fine & (ids.cpu() >= 0)]).all()
     ref = torch.log_softmax(x, -1)
+    assert (top_ids[torch.isnan(x).any(-1)] == -1).all() and torch.isnan(top_lp[~fine]).all()
     t = 2.0 ** -22 + (V / 128 + 64) * 2.0 ** -24
     for r in range(N):
         if not fine[r]:
