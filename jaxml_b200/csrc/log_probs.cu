@@ -2,9 +2,11 @@
 //
 // With m the row's maximum, z = sum exp(x - m) and w = sum exp(x - m) (x - m):
 //   log p(id) = (x[id] - m) - log z,   entropy = log z - w / z.
-// One reading of the row: a thread keeps its own m, z and w and moves z and w to a new maximum when a batch of its
-// elements brings one (z' = z f, w' = f (w + z (m - m'))).  x - m is formed before anything is scaled, so it is exact near the
-// maximum whatever the logits' offset.
+// One reading of the row.  A thread keeps a reference K of its own, in units of log2: u = x log2(e) - K is one fused
+// multiply-add, z = sum 2^u and w = sum 2^u u, and both move to the reference of a new maximum when a batch of elements
+// brings one.  K is rounded, but it is the same K for every element: the joined reference enters the results in 64 bits,
+// once a row.  Rows of magnitude above 2^13 (where a rounded K would be far from the maximum in units of u), and rows with NaN
+// or infinity, are read again the careful way: x - m first, which is exact near the maximum.
 //
 // The alternatives come from the maxima of the threads and of their batches.  t, the top_n-th largest of the threads'
 // maxima, is a lower bound of every element wanted, and the larger elements lie in batches (whose maxima stay in shared
@@ -65,15 +67,17 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// (m, z, w) of a set of elements.
+// z and w of a set of elements relative to a reference; m: its maximum (NaN where the set has one).
 struct Sums {
-  float m, z, w;
+  double ref;      // natural units, -inf without elements
+  float m, z, w;   // w in natural units
 };
-// exp(d) for d = m - m' of two maxima, 1 where both are the same (also -inf), 0 for an empty side.
 __device__ __forceinline__ Sums joined(const Sums& a, const Sums& b) {
   Sums r;
   r.m = max_nan(a.m, b.m);
-  const float da = a.m == r.m ? 0.f : fmaxf(a.m - r.m, -1e30f), db = b.m == r.m ? 0.f : fmaxf(b.m - r.m, -1e30f);
+  r.ref = fmax(a.ref, b.ref);
+  const float da = a.ref == r.ref ? 0.f : fmaxf((float)(a.ref - r.ref), -1e30f);
+  const float db = b.ref == r.ref ? 0.f : fmaxf((float)(b.ref - r.ref), -1e30f);
   const float fa = exp2_f(da * 1.4426950408889634f), fb = exp2_f(db * 1.4426950408889634f);
   r.z = a.z * fa + b.z * fb;
   r.w = fa * (a.w + a.z * da) + fb * (b.w + b.z * db);
@@ -129,11 +133,27 @@ struct Row {
   }
 };
 
+// The order key of a batch's maximum: bfloat16 rows need its upper half alone.
+template <typename T>
+struct SlotKey {
+  typedef uint32_t type;
+  static __device__ __forceinline__ uint32_t pack(uint32_t k) { return k; }
+  static __device__ __forceinline__ uint32_t unpack(uint32_t k) { return k; }
+};
+template <>
+struct SlotKey<bf16> {
+  typedef uint16_t type;
+  static __device__ __forceinline__ uint16_t pack(uint32_t k) { return (uint16_t)(k >> 16); }
+  // the lower bits of a bfloat16's key: zeros for a positive value, ones for a negative one; 0 stays 0
+  static __device__ __forceinline__ uint32_t unpack(uint16_t k) { return (uint32_t)k << 16 | (k - 1u < 0x7FFFu ? 0xFFFFu : 0u); }
+};
+
+template <typename T>
 struct Shared {
-  uint32_t slot[kSlots][kThreads];              // order keys of the batches' maxima
-  unsigned long long cand[kCand];               // order key << 32 | ~index
-  unsigned long long list[kMostTop];            // this CTA's best, unordered
-  __align__(16) uint32_t best[kThreads];        // order keys of the threads' maxima
+  typename SlotKey<T>::type slot[kSlots][kThreads];   // order keys of the batches' maxima
+  __align__(16) unsigned long long cand[kCand];       // order key << 32 | ~index
+  unsigned long long list[kMostTop];                  // this CTA's best, in order
+  __align__(16) uint32_t best[kThreads];              // order keys of the threads' maxima
   Sums sums[kWarps];
   Sums mine;
   int scan[kWarps + 1];
@@ -165,16 +185,16 @@ __device__ __forceinline__ int block_exclusive(int x, int* sh, int* total) {
 
 // The want-th largest of the maxima of kThreads / kEach groups of neighbouring threads (all threads; 1 <= want <= groups).
 template <int kEach>
-__device__ __forceinline__ uint32_t nth_largest(Shared& s, uint32_t mine, int want) {
+__device__ __forceinline__ uint32_t nth_largest(uint32_t* best, uint32_t* bound, uint32_t mine, int want) {
   const int tid = threadIdx.x;
 #pragma unroll
   for (int d = 1; d < kEach; d <<= 1) mine = max(mine, __shfl_xor_sync(~0u, mine, d));
-  if (tid % kEach == 0) s.best[tid / kEach] = mine;
+  if (tid % kEach == 0) best[tid / kEach] = mine;
   __syncthreads();
   if (tid < kThreads / kEach) {
-    mine = s.best[tid];
+    mine = best[tid];
     int above = 0;
-    const uint4* all = reinterpret_cast<const uint4*>(s.best);
+    const uint4* all = reinterpret_cast<const uint4*>(best);
 #pragma unroll 4
     for (int i = 0; i < kThreads / kEach / 4; ++i) {
       const uint4 k = all[i];
@@ -182,27 +202,29 @@ __device__ __forceinline__ uint32_t nth_largest(Shared& s, uint32_t mine, int wa
       above += (k.x > mine || (k.x == mine && 4 * i < tid)) + (k.y > mine || (k.y == mine && 4 * i + 1 < tid)) +
                (k.z > mine || (k.z == mine && 4 * i + 2 < tid)) + (k.w > mine || (k.w == mine && 4 * i + 3 < tid));
     }
-    if (above == want - 1) s.bound = mine;
+    if (above == want - 1) *bound = mine;
   }
   __syncthreads();
-  return s.bound;
+  return *bound;
 }
 
 // The top_n largest elements of the slice into s.list (all threads); n_list of them.
 template <typename T>
-__device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rounds_per_slot, int slots, int top_n) {
+__device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0, int v1, int rounds_per_slot, int slots, int top_n,
+                                        uint32_t mine) {
   constexpr int kE = Row<T>::kE;
   const int tid = threadIdx.x;
   const int size = min(v1 * kE, row.last) - max(v0 * kE, row.first);   // elements of the slice
   const int want = min(top_n, max(size, 0));
   if (want == 0) return;
-  // a thread without an element has key 0, below that of -inf: with fewer threads at work than elements wanted all count
-  uint32_t mine = 0;
-  for (int i = 0; i < slots; ++i) mine = max(mine, s.slot[i][tid]);
+  // mine: the order key of the thread's maximum; 0, below that of -inf, without an element: with fewer threads at work than
+  // elements wanted all elements count
   // 64 groups are as good a bound for few elements and cost a sixteenth of the comparisons
-  const uint32_t t = want <= 32 ? nth_largest<4>(s, mine, want) : nth_largest<1>(s, mine, want);
+  const uint32_t t = want <= 32 ? nth_largest<4>(s.best, &s.bound, mine, want) : nth_largest<1>(s.best, &s.bound, mine, want);
   const int per = rounds_per_slot;
-  auto each = [&](int slot, auto&& f) {   // this thread's elements of a slot
+  // this thread's elements of a slot that are at least `from`
+  auto each = [&](int slot, uint32_t from, auto&& f) {
+    const float least = key_value(from);
     for (int r = slot * per; r < slot * per + per; ++r) {
       uint4 u[4];
       const int v = v0 + r * 4 * kThreads + tid;
@@ -214,24 +236,25 @@ __device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rou
         float x[kE];
         Row<T>::floats(u[j], x);
 #pragma unroll
-        for (int e = 0; e < kE; ++e) {
-          const int i = (v + j * kThreads) * kE + e;
-          if (i >= row.first && i < row.last) f(order_key(x[e]), i - row.first);
-        }
+        for (int e = 0; e < kE; ++e)
+          if (from == 0 || x[e] >= least) {
+            const int i = (v + j * kThreads) * kE + e;
+            const uint32_t k = order_key(x[e]);
+            if (k >= from && i >= row.first && i < row.last) f(k, i - row.first);
+          }
       }
     }
   };
   auto collect = [&](uint32_t from) {     // all elements of that key or above; how many
     if (tid == 0) s.n_cand = 0;
     __syncthreads();
-    for (int i = 0; mine >= from && i < slots; ++i)
-      if (s.slot[i][tid] >= from)
-        each(i, [&](uint32_t k, int at) {
-          if (k >= from) {
-            const int p = atomicAdd(&s.n_cand, 1);
-            if (p < kCand) s.cand[p] = ((unsigned long long)k << 32) | (uint32_t)~at;
-          }
-        });
+    uint32_t mask = 0;
+    for (int i = 0; mine >= from && i < slots; ++i) mask |= (uint32_t)(SlotKey<T>::unpack(s.slot[i][tid]) >= from) << i;
+    for (; mask; mask &= mask - 1)        // the lanes of a warp read their own batches at the same time
+      each(__ffs(mask) - 1, from, [&](uint32_t k, int at) {
+        const int p = atomicAdd(&s.n_cand, 1);
+        if (p < kCand) s.cand[p] = ((unsigned long long)k << 32) | (uint32_t)~at;
+      });
     __syncthreads();
     return s.n_cand;
   };
@@ -246,7 +269,7 @@ __device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rou
     for (int k = 0; k < want; ++k) {
       unsigned long long best = 0;
       for (int i = 0; i < slots; ++i)
-        each(i, [&](uint32_t key, int at) {
+        each(i, 0u, [&](uint32_t key, int at) {
           const unsigned long long c = ((unsigned long long)key << 32) | (uint32_t)~at;
           if (c < below && c > best) best = c;
         });
@@ -274,7 +297,7 @@ __device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rou
   if (n < want) {   // elements equal to t, by index: rounds in order, in a round the vectors in order
     int found = n;
     for (int i = 0; i < slots && found < want; ++i) {
-      const bool holds = s.slot[i][tid] >= t;
+      const bool holds = SlotKey<T>::unpack(s.slot[i][tid]) >= t;
       if (!__syncthreads_or(holds)) continue;
       for (int r = i * per; r < i * per + per && found < want; ++r)
         for (int j = 0; j < 4 && found < want; ++j) {
@@ -300,10 +323,113 @@ __device__ void select_top(Shared& s, const Row<T>& row, int v0, int v1, int rou
   __syncthreads();
 }
 
+// Reads the slice: this thread's part of the sums; the batches' maxima where `slot` is given.
+template <typename T, bool kCareful>
+__device__ __forceinline__ Sums stream(const Row<T>& row, int v0, int v1, int rounds, int per_slot, int slots,
+                                       typename SlotKey<T>::type* slot) {
+  constexpr int kE = Row<T>::kE;
+  constexpr float kLog2e = 1.4426950408889634f;
+  const int tid = threadIdx.x;
+  float m = -INFINITY, ref = -INFINITY;     // ref: K, or (careful) m itself
+  uint64_t z2 = pack2(0.f, 0.f), w2 = z2;   // even and odd elements
+  const uint64_t c2 = pack2(kLog2e, kLog2e);
+  uint64_t nr = 0;
+  const uint4 none = sizeof(T) == 2 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
+                                    : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
+  float floor = 0.f;                        // far enough below m: a term of 0, and no infinity in a product with 0
+  uint32_t floor2 = 0;
+  int round = 0;
+  const int fast_to = (v1 - v0) / (4 * kThreads) - !row.inside(v1 - 1);   // rounds of whole vectors, but the first
+  const uint4* p = reinterpret_cast<const uint4*>(row.base) + v0 + tid;
+  for (int i = 0; i < slots; ++i) {
+    float slot_max = -INFINITY;
+    bool any = false;
+    for (int k = 0; k < per_slot && round < rounds; ++k, ++round) {
+      uint4 u[4];
+      if (round > 0 && round < fast_to) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = __ldg(p + j * kThreads);
+        any = true;
+      } else {
+        const int v = v0 + round * 4 * kThreads + tid;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : none;
+        any |= v < v1;
+      }
+      p += 4 * kThreads;
+      const float bm = Row<T>::max_of(u[0], u[1], u[2], u[3]);
+      slot_max = max_nan(slot_max, bm);
+      if (!(bm <= m)) {                     // a new maximum (or NaN)
+        const float old = ref;
+        const bool had = m != -INFINITY;
+        m = max_nan(m, bm);
+        ref = kCareful ? m : m * kLog2e;
+        floor = m - 16384.f;
+        floor2 = pack_bf16x2(floor, floor);
+        nr = pack2(-ref, -ref);
+        if (had) {
+          const float d = fmaxf(old - ref, -1e30f), f = exp2_f(kCareful ? d * kLog2e : d);
+          w2 = mul2(pack2(f, f), fma2(z2, pack2(d, d), w2));
+          z2 = mul2(pack2(f, f), z2);
+        }
+      }
+      if (!kCareful && m == -INFINITY) continue;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float e[kE];
+        if constexpr (kCareful) {
+          Row<T>::floats(u[j], e);
+        } else if constexpr (sizeof(T) == 2) {
+          uint4 x;
+          asm("max.bf16x2 %0, %1, %2;" : "=r"(x.x) : "r"(u[j].x), "r"(floor2));
+          asm("max.bf16x2 %0, %1, %2;" : "=r"(x.y) : "r"(u[j].y), "r"(floor2));
+          asm("max.bf16x2 %0, %1, %2;" : "=r"(x.z) : "r"(u[j].z), "r"(floor2));
+          asm("max.bf16x2 %0, %1, %2;" : "=r"(x.w) : "r"(u[j].w), "r"(floor2));
+          Row<T>::floats(x, e);
+        } else {
+          Row<T>::floats(u[j], e);
+#pragma unroll
+          for (int p = 0; p < kE; ++p) e[p] = fmaxf(e[p], floor);
+        }
+#pragma unroll
+        for (int p = 0; p < kE; p += 2) {
+          float y0, y1;
+          uint64_t d;
+          if constexpr (kCareful) {
+            unpack2(add2(pack2(e[p], e[p + 1]), nr), y0, y1);
+            d = pack2(fmaxf(y0, -1e30f), fmaxf(y1, -1e30f));
+            unpack2(mul2(d, c2), y0, y1);
+          } else {
+            d = fma2(pack2(e[p], e[p + 1]), c2, nr);
+            unpack2(d, y0, y1);
+          }
+          const uint64_t y = pack2(exp2_f(y0), exp2_f(y1));
+          z2 = add2(z2, y);
+          w2 = fma2(y, d, w2);
+        }
+      }
+    }
+    if (slot) slot[i * kThreads + tid] = SlotKey<T>::pack(any ? order_key(slot_max) : 0u);
+  }
+  Sums t;
+  float a0, a1;
+  t.m = m;
+  t.ref = kCareful ? (double)ref : (double)ref * 0.6931471805599453;
+  unpack2(z2, a0, a1);
+  t.z = a0 + a1;
+  unpack2(w2, a0, a1);
+  t.w = kCareful ? a0 + a1 : (a0 + a1) * 0.6931471805599453f;
+  return t;
+}
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 5) log_probs_kernel(const jx_log_probs_args a, int rounds_per_slot) {
+__device__ __noinline__ Sums stream_careful(const Row<T>& row, int v0, int v1, int rounds, int per_slot, int slots) {
+  return stream<T, true>(row, v0, v1, rounds, per_slot, slots, nullptr);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_probs_args a, int rounds_per_slot) {
   extern __shared__ __align__(16) unsigned char smem[];
-  Shared& s = *reinterpret_cast<Shared*>(smem);
+  Shared<T>& s = *reinterpret_cast<Shared<T>*>(smem);
   constexpr int kE = Row<T>::kE;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
@@ -318,90 +444,54 @@ __global__ void __launch_bounds__(kThreads, 5) log_probs_kernel(const jx_log_pro
   const int rounds = (v1 - v0 + 4 * kThreads - 1) / (4 * kThreads);
   const int slots = (rounds + rounds_per_slot - 1) / rounds_per_slot;
 
-  float m = -INFINITY;
-  uint64_t z2 = pack2(0.f, 0.f), w2 = z2;
-  const uint64_t c2 = pack2(1.4426950408889634f, 1.4426950408889634f);
-  const uint4 none = sizeof(T) == 2 ? make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u)
-                                    : make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
-  int round = 0;
-  for (int i = 0; i < slots; ++i) {
-    float slot_max = -INFINITY;
-    bool any = false;
-    for (int k = 0; k < rounds_per_slot && round < rounds; ++k, ++round) {
-      const int v = v0 + round * 4 * kThreads + tid;
-      uint4 u[4];
-      if (v0 + (round + 1) * 4 * kThreads <= v1 && round > 0 && (round + 1 < rounds || row.inside(v1 - 1))) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = __ldcs(reinterpret_cast<const uint4*>(row.base) + v + j * kThreads);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : none;
-      }
-      any |= v < v1;
-      const float bm = Row<T>::max_of(u[0], u[1], u[2], u[3]);
-      slot_max = max_nan(slot_max, bm);
-      if (!(bm <= m)) {   // a new maximum (or NaN)
-        if (m != -INFINITY) {
-          const float d = fmaxf(m - bm, -1e30f), f = exp2_f(d * 1.4426950408889634f);
-          w2 = mul2(pack2(f, f), fma2(z2, pack2(d, d), w2));
-          z2 = mul2(pack2(f, f), z2);
-        }
-        m = max_nan(m, bm);
-      }
-      const uint64_t nm = pack2(-m, -m);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float e[kE];
-        Row<T>::floats(u[j], e);
-#pragma unroll
-        for (int p = 0; p < kE; p += 2) {
-          float d0, d1, y0, y1;
-          unpack2(add2(pack2(e[p], e[p + 1]), nm), d0, d1);
-          d0 = fmaxf(d0, -1e30f), d1 = fmaxf(d1, -1e30f);     // -inf (and, with m, NaN): a probability of 0 without 0 * inf
-          const uint64_t d = pack2(d0, d1);
-          unpack2(mul2(d, c2), y0, y1);
-          const uint64_t y = pack2(exp2_f(y0), exp2_f(y1));
-          z2 = add2(z2, y);
-          w2 = fma2(y, d, w2);
-        }
-      }
-    }
-    if (a.top_n) s.slot[i][tid] = any ? order_key(slot_max) : 0u;
+  // the given token's logit on its way while the row is read
+  int id = -1;
+  float given = 0.f;
+  if (rank == 0 && tid == 0) {
+    id = a.ids[r];
+    if (id >= 0 && id < a.V) given = to_f(x[id]);
   }
-  Sums t;
-  {
-    float a0, a1;
-    t.m = m;
-    unpack2(z2, a0, a1);
-    t.z = a0 + a1;
-    unpack2(w2, a0, a1);
-    t.w = a0 + a1;
-  }
+  Sums t = stream<T, false>(row, v0, v1, rounds, rounds_per_slot, slots, a.top_n ? &s.slot[0][0] : nullptr);
+  if (__syncthreads_or(t.m != -INFINITY && !(fabsf(t.m) <= 8192.f)))
+    t = stream_careful<T>(row, v0, v1, rounds, rounds_per_slot, slots);
+  const uint32_t my_key = v0 + tid < v1 ? order_key(t.m) : 0u;
+  const bool no_order = __syncthreads_or(t.m != t.m);    // NaN
 #pragma unroll
   for (int d = 16; d; d >>= 1) {
     Sums o;
-    o.m = __shfl_xor_sync(~0u, t.m, d), o.z = __shfl_xor_sync(~0u, t.z, d), o.w = __shfl_xor_sync(~0u, t.w, d);
+    o.ref = __shfl_xor_sync(~0u, t.ref, d), o.m = __shfl_xor_sync(~0u, t.m, d);
+    o.z = __shfl_xor_sync(~0u, t.z, d), o.w = __shfl_xor_sync(~0u, t.w, d);
     // the lower lane's first on both sides: one result for the warp
     t = lane & d ? joined(o, t) : joined(t, o);
   }
   if (lane == 0) s.sums[warp] = t;
+  if (tid == 0) s.n_list = 0;
   __syncthreads();
-  t = s.sums[0];
+  if (warp == 0) {
+    t = s.sums[lane & (kWarps - 1)];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) t = joined(t, s.sums[w]);
-  if (tid == 0) s.mine = t, s.n_list = 0;
-  if (a.top_n) {
-    if (t.m == t.m) select_top<T>(s, row, v0, v1, rounds_per_slot, slots, a.top_n);   // no order with NaN
+    for (int d = kWarps / 2; d; d >>= 1) {
+      Sums o;
+      o.ref = __shfl_xor_sync(~0u, t.ref, d), o.m = __shfl_xor_sync(~0u, t.m, d);
+      o.z = __shfl_xor_sync(~0u, t.z, d), o.w = __shfl_xor_sync(~0u, t.w, d);
+      t = lane & d ? joined(o, t) : joined(t, o);
+    }
+    if (lane == 0) s.mine = t;
   }
+  if (a.top_n && !no_order) select_top<T>(s, row, v0, v1, rounds_per_slot, slots, a.top_n, my_key);
   if (C > 1) {
     cluster_sync_all();
     if (rank == 0) {
-      t = s.mine;
-      for (int q = 1; q < C; ++q) {
-        const uint32_t at = dsmem_map(smem_u32(&s.mine), q);
-        Sums o;
-        o.m = dsmem_ld_f32(at), o.z = dsmem_ld_f32(at + 4), o.w = dsmem_ld_f32(at + 8);
-        t = joined(t, o);
+      if (tid == 0) {
+        t = s.mine;
+        for (int q = 1; q < C; ++q) {
+          const uint32_t at = dsmem_map(smem_u32(&s.mine), q);
+          Sums o;
+          o.ref = __hiloint2double(__float_as_int(dsmem_ld_f32(at + 4)), __float_as_int(dsmem_ld_f32(at)));
+          o.m = dsmem_ld_f32(at + 8), o.z = dsmem_ld_f32(at + 12), o.w = dsmem_ld_f32(at + 16);
+          t = joined(t, o);
+        }
+        s.mine = t;
       }
       // every CTA's list behind the others in the candidates
       int n = 0;
@@ -430,17 +520,20 @@ __global__ void __launch_bounds__(kThreads, 5) log_probs_kernel(const jx_log_pro
   } else {
     __syncthreads();
   }
+  // log p = (x - ref) - log z, the difference in 64 bits: the reference is rounded, and may be large beside it
+  t = s.mine;
+  const bool fine = t.m == t.m && fabsf(t.m) != INFINITY;
   const float lz = logf(t.z);
   if (tid == 0) {
-    const int id = a.ids[r];
-    a.log_probs[r] = id < 0 ? 0.f : id >= a.V || t.m != t.m ? nan_f() : (to_f(x[id]) - t.m) - lz;
-    a.entropy[r] = t.m != t.m ? nan_f() : lz - t.w / t.z;
+    a.log_probs[r] = id < 0 ? 0.f : id >= a.V || !fine ? nan_f() : (float)((double)given - t.ref) - lz;
+    a.entropy[r] = fine ? lz - t.w / t.z : nan_f();
   }
   if (tid < a.top_n) {
-    const bool fine = t.m == t.m;
-    const unsigned long long c = fine ? s.list[tid] : 0;
-    a.top_ids[(long long)r * a.top_n + tid] = fine ? (int)~(uint32_t)c : -1;
-    a.top_log_probs[(long long)r * a.top_n + tid] = fine ? (key_value((uint32_t)(c >> 32)) - t.m) - lz : nan_f();
+    const bool order = t.m == t.m;
+    const unsigned long long c = order ? s.list[tid] : 0;
+    a.top_ids[(long long)r * a.top_n + tid] = order ? (int)~(uint32_t)c : -1;
+    a.top_log_probs[(long long)r * a.top_n + tid] =
+        fine ? (float)((double)key_value((uint32_t)(c >> 32)) - t.ref) - lz : nan_f();
   }
 }
 
@@ -454,7 +547,7 @@ int launch(const jx_log_probs_args& a, cudaStream_t s) {
   const long long per_cta = (nv + C - 1) / C;
   const long long rounds = (per_cta + 4 * kThreads - 1) / (4 * kThreads);
   const int per_slot = (int)((rounds + kSlots - 1) / kSlots);
-  const int smem = (int)sizeof(Shared);
+  const int smem = (int)sizeof(Shared<T>);
   static bool ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return JX_ERR_CUDA;
