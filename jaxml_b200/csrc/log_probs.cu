@@ -341,20 +341,26 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int v0, int v1, int ro
   int round = 0;
   const int fast_to = (v1 - v0) / (4 * kThreads) - !row.inside(v1 - 1);   // rounds of whole vectors, but the first
   const uint4* p = reinterpret_cast<const uint4*>(row.base) + v0 + tid;
+  uint4 next[4] = {none, none, none, none};
+  bool ahead = false;
   for (int i = 0; i < slots; ++i) {
     float slot_max = -INFINITY;
     bool any = false;
     for (int k = 0; k < per_slot && round < rounds; ++k, ++round) {
       uint4 u[4];
-      if (round > 0 && round < fast_to) {
+      const int v = v0 + round * 4 * kThreads + tid;
+      if (ahead) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = __ldg(p + j * kThreads);
-        any = true;
+        for (int j = 0; j < 4; ++j) u[j] = next[j];
       } else {
-        const int v = v0 + round * 4 * kThreads + tid;
 #pragma unroll
         for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : none;
-        any |= v < v1;
+      }
+      any |= v < v1;
+      ahead = round + 1 < fast_to;        // the next round's vectors are under way while this one's are summed
+      if (ahead) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) next[j] = __ldg(p + (j + 4) * kThreads);
       }
       p += 4 * kThreads;
       const float bm = Row<T>::max_of(u[0], u[1], u[2], u[3]);
