@@ -22,6 +22,7 @@ namespace jxb {
 
 constexpr int kPage = 64;                        // tokens per page
 constexpr uint32_t kKv4Overflow = 0x7C800000u;   // bits of 2^122
+constexpr uint32_t kKv4BadScale = 0x7B80u;       // bfloat16 2^120: every scale of a finite group is below it
 
 __host__ __device__ __forceinline__ int kv4_block_bytes(int hd) { return kPage * hd + kPage * (hd / 32) * 4; }
 __host__ __device__ __forceinline__ int kv4_scale_offset(int hd, int which) {

@@ -1,0 +1,173 @@
+// What the attention kernels over the 4-bit KV cache share: arguments, the order of work, operand pieces.
+#pragma once
+
+#include <cudaTypedefs.h>
+#include <math.h>
+
+#include "kv4.cuh"
+
+namespace jxb {
+namespace kv4 {
+
+struct AttendArgs {
+  jx_kv4_cache c;
+  int layer, S, Hq, G, window, q_vec, items, tiles;   // tiles: query tiles of a row; items = rows * tiles
+  float scale_log2, sign;   // |scale| log2(e), at least 1e-30 so that a hidden -inf stays one; its sign, taken into q
+  const void* q;
+  long long q_row, q_tok, q_head;
+  void* out;
+  long long* item_first;   // [items] first unit of an item (written by the first CTA)
+  long long* total;        // [2] units, warps
+  float* part;             // [warps][2] slots of 8 * NT rows: O, then m and l
+};
+
+// ---- small pieces -------------------------------------------------------------------------------------
+__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t as_u(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+// bfloat16 pair 128 + u of the nibbles k and k + 4 of a word (or k of two merged words).
+__device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(r) : "r"(w >> (4 * k)));
+  return r;
+}
+__device__ __forceinline__ uint32_t code2(uint32_t w, int k) { return as_u(__hsub2(as_b2(raw2(w, k)), as_b2(0x43084308u))); }
+__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2) { return as_u(__hmul2(as_b2(code2(w, k)), as_b2(s2))); }
+__device__ __forceinline__ void mma_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                      float c0, float c1, float c2, float c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_f(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+// Where the copy's swizzle puts a byte of a block (16-byte pieces of a 128-byte line exchanged by the line's number).
+template <int HD>
+__device__ __forceinline__ int swz(int o) {
+  return o ^ (((o >> 7) & (HD / 32 - 1)) << 4);
+}
+__device__ __forceinline__ uint32_t lds16(const unsigned char* p) { return *reinterpret_cast<const uint16_t*>(p); }
+
+// ---- the order of work ------------------------------------------------------------------------------------
+// Pages [p0, p0 + n) that query tile `qt` of a row sees.
+struct Item {
+  int r, qt, cnt, base, n, p0;   // base: position of query 0
+};
+template <int kRows>
+__device__ __forceinline__ Item item_at(const AttendArgs& a, long long item) {
+  Item t;
+  t.r = (int)(item / a.tiles), t.qt = (int)(item - (long long)t.r * a.tiles);
+  t.cnt = min(a.c.counts[t.r], a.S);
+  const int len = min(a.c.lengths[t.r], a.c.row_pages * kPage);
+  t.base = len - a.c.counts[t.r];
+  const int s0 = t.qt * kRows / a.G, s1 = min(min(t.qt * kRows + kRows, a.S * a.G) - 1, t.cnt * a.G - 1) / a.G;
+  t.n = 0, t.p0 = 0;
+  if (s0 < t.cnt && t.base >= 0) {
+    t.p0 = a.window > 0 ? max(0, t.base + s0 - a.window + 1) / kPage : 0;
+    t.n = (t.base + s1) / kPage - t.p0 + 1;
+  }
+  return t;
+}
+
+struct Walk {
+  Item t;
+  long long item;
+  int head, page;
+  template <int kRows>
+  __device__ __forceinline__ void next(const AttendArgs& a) {
+    if (++page < t.n) return;
+    page = 0;
+    if (++head < a.c.num_kv_heads) return;
+    head = 0;
+    do {
+      ++item;
+      if (item >= a.items) return;
+      t = item_at<kRows>(a, item);
+    } while (t.n == 0);
+  }
+};
+
+// First unit of warp w's run.
+__device__ __forceinline__ long long run_start(long long w, long long units, long long warps) { return w * units / warps; }
+// Warp whose run holds unit u.
+__device__ __forceinline__ long long run_of(long long u, long long units, long long warps) {
+  return ((u + 1) * warps - 1) / units;
+}
+
+// ---- loading queries ----------------------------------------------------------------------------------------
+// 8 neighbouring channels as fragment registers (0,4) (1,5) (2,6) (3,7), a float32 split into `parts`.
+__device__ __forceinline__ void q_words(const bf16* p, bool vec, float sign, uint4* out) {
+  uint32_t x[4];
+  if (vec) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+  } else {
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] ^= sign < 0.f ? 0x80008000u : 0u;
+  out[0] = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410),
+                      __byte_perm(x[1], x[3], 0x7632));
+}
+__device__ __forceinline__ void q_words(const float* p, bool vec, float sign, uint4* out) {
+  float x[8];
+  if (vec) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] *= sign;
+#pragma unroll
+  for (int part = 0; part < 3; ++part) {
+    out[part] = make_uint4(pack_bf16x2(x[0], x[4]), pack_bf16x2(x[1], x[5]), pack_bf16x2(x[2], x[6]), pack_bf16x2(x[3], x[7]));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] -= rnd<bf16>(x[i]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store_row8(T* o, const float* x) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4*>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
+  } else {
+    *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                                              pack_bf16x2(x[6], x[7]));
+  }
+}
+template <int HD, typename T>
+__device__ __forceinline__ T* out_row(const AttendArgs& a, int r, int head, int f) {
+  const int s = f / a.G;
+  return static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
+}
+
+// Brings the block of a page into shared memory; a page id out of range is reported and its stage marked.
+template <int HD>
+__device__ __forceinline__ void fetch(const AttendArgs& a, const CUtensorMap* map, int id, int head, unsigned char* to,
+                                      uint64_t* bar, int* bad) {
+  const bool ok = id >= 0 && id < a.c.num_pages;
+  *bad = !ok;
+  if (ok) {
+    mbar_arrive_expect_tx(bar, kv4_block_bytes(HD));
+    tma_load_3d(to, map, 0, 0, (a.layer * a.c.num_pages + id) * a.c.num_kv_heads + head, bar);
+  } else {
+    set_status(a.c.status, JX_ERR_RANGE);
+    mbar_arrive(bar);
+  }
+}
+
+}  // namespace kv4
+}  // namespace jxb

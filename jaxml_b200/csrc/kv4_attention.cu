@@ -20,25 +20,12 @@
 //
 // A page's block is one tensor-map box of 144 rows of hd / 2 bytes, swizzled by the copy so that ldmatrix gives every
 // thread its words of the key it owns without bank conflicts.
-#include <cudaTypedefs.h>
-#include <math.h>
-
-#include "kv4.cuh"
+#include "kv4_attend.cuh"
 
 namespace jxb {
+int run_kv4_attend_tc(const void* args, const void* map, int sms, cudaStream_t s);   // kv4_attention_tc.cu
+using namespace kv4;
 namespace {
-
-struct AttendArgs {
-  jx_kv4_cache c;
-  int layer, S, Hq, G, window, q_vec, items, tiles;   // tiles: query tiles of a row; items = rows * tiles
-  float scale_log2, sign;   // |scale| log2(e), at least 1e-30 so that a hidden -inf stays one; its sign, taken into q
-  const void* q;
-  long long q_row, q_tok, q_head;
-  void* out;
-  long long* item_first;   // [items] first unit of an item (written by the first CTA)
-  long long* total;        // [2] units, warps
-  float* part;             // [warps][2] slots of 8 * NT rows: O, then m and l
-};
 
 template <int HD, int NT, typename T>
 struct Cfg {
@@ -56,123 +43,6 @@ struct Cfg {
   static constexpr int kQBytes = kQReg ? 0 : NT * kQParts * HD * 16;   // a warp's fragments in shared memory
   static constexpr int kSlot = kRows * (HD + 2);          // floats of a partial result
 };
-
-// ---- small pieces -------------------------------------------------------------------------------------
-__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
-__device__ __forceinline__ uint32_t as_u(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
-// bfloat16 pair 128 + u of the nibbles k and k + 4 of a word (or k of two merged words).
-__device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(r) : "r"(w >> (4 * k)));
-  return r;
-}
-__device__ __forceinline__ uint32_t code2(uint32_t w, int k) { return as_u(__hsub2(as_b2(raw2(w, k)), as_b2(0x43084308u))); }
-__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2) { return as_u(__hmul2(as_b2(code2(w, k)), as_b2(s2))); }
-__device__ __forceinline__ void mma_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
-                                      float c0, float c1, float c2, float c3) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
-  return r;
-}
-__device__ __forceinline__ float exp2_f(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-// Where the copy's swizzle puts a byte of a block (16-byte pieces of a 128-byte line exchanged by the line's number).
-template <int HD>
-__device__ __forceinline__ int swz(int o) {
-  return o ^ (((o >> 7) & (HD / 32 - 1)) << 4);
-}
-__device__ __forceinline__ uint32_t lds16(const unsigned char* p) { return *reinterpret_cast<const uint16_t*>(p); }
-
-// ---- the order of work ------------------------------------------------------------------------------------
-// Pages [p0, p0 + n) that query tile `qt` of a row sees.
-struct Item {
-  int r, qt, cnt, base, n, p0;   // base: position of query 0
-};
-template <int kRows>
-__device__ __forceinline__ Item item_at(const AttendArgs& a, long long item) {
-  Item t;
-  t.r = (int)(item / a.tiles), t.qt = (int)(item - (long long)t.r * a.tiles);
-  t.cnt = min(a.c.counts[t.r], a.S);
-  const int len = min(a.c.lengths[t.r], a.c.row_pages * kPage);
-  t.base = len - a.c.counts[t.r];
-  const int s0 = t.qt * kRows / a.G, s1 = min(min(t.qt * kRows + kRows, a.S * a.G) - 1, t.cnt * a.G - 1) / a.G;
-  t.n = 0, t.p0 = 0;
-  if (s0 < t.cnt && t.base >= 0) {
-    t.p0 = a.window > 0 ? max(0, t.base + s0 - a.window + 1) / kPage : 0;
-    t.n = (t.base + s1) / kPage - t.p0 + 1;
-  }
-  return t;
-}
-
-struct Walk {
-  Item t;
-  long long item;
-  int head, page;
-  template <int kRows>
-  __device__ __forceinline__ void next(const AttendArgs& a) {
-    if (++page < t.n) return;
-    page = 0;
-    if (++head < a.c.num_kv_heads) return;
-    head = 0;
-    do {
-      ++item;
-      if (item >= a.items) return;
-      t = item_at<kRows>(a, item);
-    } while (t.n == 0);
-  }
-};
-
-// First unit of warp w's run.
-__device__ __forceinline__ long long run_start(long long w, long long units, long long warps) { return w * units / warps; }
-// Warp whose run holds unit u.
-__device__ __forceinline__ long long run_of(long long u, long long units, long long warps) {
-  return ((u + 1) * warps - 1) / units;
-}
-
-// ---- loading queries ----------------------------------------------------------------------------------------
-// 8 neighbouring channels as fragment registers (0,4) (1,5) (2,6) (3,7), a float32 split into `parts`.
-__device__ __forceinline__ void q_words(const bf16* p, bool vec, float sign, uint4* out) {
-  uint32_t x[4];
-  if (vec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] ^= sign < 0.f ? 0x80008000u : 0u;
-  out[0] = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410),
-                      __byte_perm(x[1], x[3], 0x7632));
-}
-__device__ __forceinline__ void q_words(const float* p, bool vec, float sign, uint4* out) {
-  float x[8];
-  if (vec) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] *= sign;
-#pragma unroll
-  for (int part = 0; part < 3; ++part) {
-    out[part] = make_uint4(pack_bf16x2(x[0], x[4]), pack_bf16x2(x[1], x[5]), pack_bf16x2(x[2], x[6]), pack_bf16x2(x[3], x[7]));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] -= rnd<bf16>(x[i]);
-  }
-}
 
 // ---- one tile of query rows over slices of a page -----------------------------------------------------------
 template <int HD, int NT, typename T>
@@ -449,7 +319,7 @@ struct Tile {
     }
   }
 
-  // Where a value scale of keys [kb, kb + KT) is not finite, the rows that see its key get NaN in its channels, and the scale
+  // Where a value scale of keys [kb, kb + KT) is none of the format (NaN; 2^120 or more), the rows that see its key get NaN in its channels, and the scale
   // in shared memory becomes 0: a row that does not see the key has P = 0 there, and 0 * NaN would reach it.  Runs before
   // keys().
   template <int KT>
@@ -473,13 +343,13 @@ struct Tile {
           w[0] = *x;
         }
 #pragma unroll
-        for (int j = 0; j < kEach / 4; ++j) top |= (w[j] & 0x7F807F80u) + 0x00800080u;   // an exponent of ones carries
+        for (int j = 0; j < kEach / 4; ++j) top |= (w[j] & 0x7FFF7FFFu) + (0x8000u - kKv4BadScale) * 0x10001u;   // carries into the sign from there on
       }
     }
     if (!__any_sync(~0u, top & 0x80008000u)) return;
     const int vg = HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g;
     for (int key = 0; key < KT; ++key) {
-      if ((lds16(blk + swz<HD>(at + key * (HD / 16) + vg * 2)) & 0x7FFFu) < 0x7F80u) continue;
+      if ((lds16(blk + swz<HD>(at + key * (HD / 16) + vg * 2)) & 0x7FFFu) < kKv4BadScale) continue;
       const int pos = key0 + kb + key;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -493,7 +363,7 @@ struct Tile {
     __syncwarp();
     for (int i = lane; i < kBytes / 2; i += 32) {
       uint16_t* s = reinterpret_cast<uint16_t*>(blk + swz<HD>(at + i * 2));
-      if ((*s & 0x7FFFu) >= 0x7F80u) *s = 0;
+      if ((*s & 0x7FFFu) >= kKv4BadScale) *s = 0;
     }
     fence_proxy_async();   // the next copy writes here
     __syncwarp();
@@ -514,37 +384,6 @@ struct Tile {
     return x;
   }
 };
-
-template <typename T>
-__device__ __forceinline__ void store_row8(T* o, const float* x) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(o)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(o)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    *reinterpret_cast<uint4*>(o) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                                              pack_bf16x2(x[6], x[7]));
-  }
-}
-template <int HD, typename T>
-__device__ __forceinline__ T* out_row(const AttendArgs& a, int r, int head, int f) {
-  const int s = f / a.G;
-  return static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
-}
-
-// Brings the block of a page into shared memory; a page id out of range is reported and its stage marked.
-template <int HD>
-__device__ __forceinline__ void fetch(const AttendArgs& a, const CUtensorMap* map, int id, int head, unsigned char* to,
-                                      uint64_t* bar, int* bad) {
-  const bool ok = id >= 0 && id < a.c.num_pages;
-  *bad = !ok;
-  if (ok) {
-    mbar_arrive_expect_tx(bar, Cfg<HD, 1, bf16>::kBlock);
-    tma_load_3d(to, map, 0, 0, (a.layer * a.c.num_pages + id) * a.c.num_kv_heads + head, bar);
-  } else {
-    set_status(a.c.status, JX_ERR_RANGE);
-    mbar_arrive(bar);
-  }
-}
 
 // ---- equal runs of pages for every warp ------------------------------------------------------------------------
 // All (row, query tile, KV head, page) units in one sequence, cut into equal runs, one for each warp of the grid whatever
@@ -721,31 +560,31 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
   }
 }
 
-// Joins what several warps hold of one (row, tile, head): a CTA for every query row of it.  Rows without a visible key are
-// zero.
+// Joins what several runs hold of one (row, tile, head).  A CTA takes kJoinWarps / kEach query rows, kEach warps each: one
+// where a row has a few parts, all of them where one row may be spread over the whole grid.  Rows without a visible key
+// are zero.
 constexpr int kJoinWarps = 8;
-template <int HD, typename T>
+template <int HD, typename T, int kEach>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendArgs a, int rows) {
   pdl_wait();
-  __shared__ float sh[kJoinWarps][HD + 2];
+  __shared__ float sh[kEach > 1 ? kJoinWarps : 1][HD + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, Hkv = a.c.num_kv_heads;
-  const long long seg = blockIdx.x;
-  const long long item = seg / Hkv;
-  const int head = (int)(seg - item * Hkv), j = blockIdx.y;
+  const int item = blockIdx.x / Hkv, head = blockIdx.x - item * Hkv, j = blockIdx.y * (kJoinWarps / kEach) + warp / kEach;
   const long long units = a.total[0], warps = a.total[1];
   const long long first = a.item_first[item], end = item + 1 < a.items ? a.item_first[item + 1] : units;
   const long long n = (end - first) / Hkv, u0 = first + head * n, u1 = u0 + n;
   const long long w0 = n ? run_of(u0, units, warps) : 0, w1 = n ? run_of(u1 - 1, units, warps) : 0;
   if (n && w0 == w1) return;
-  const int r = (int)(item / a.tiles), qt = (int)(item - (long long)r * a.tiles), f = qt * rows + j, s = f / a.G;
-  if (f >= a.S * a.G) return;
-  T* out = static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
-  const int slot_floats = rows * (HD + 2);
+  const int r = item / a.tiles, qt = item - r * a.tiles, f = qt * rows + j;
+  const bool live = j < rows && f < a.S * a.G;
+  if (kEach == 1 && !live) return;
+  const long long slot_floats = (long long)rows * (HD + 2);
   constexpr int kV = HD / 32;
   float m = -INFINITY, l = 0.f, o[kV];
 #pragma unroll
   for (int i = 0; i < kV; ++i) o[i] = 0.f;
-  for (long long w = w0 + warp; n && w <= w1; w += kJoinWarps) {
+  for (long long w = w0 + warp % kEach; live && n && w <= w1; w += kEach) {
+    // the run that the segment begins in holds it in its second slot
     const float* slot = a.part + (w * 2 + (run_start(w, units, warps) <= u0 ? 1 : 0)) * slot_floats;
     const float mw = slot[rows * HD + 2 * j], lw = slot[rows * HD + 2 * j + 1];
     const float mn = fmaxf(m, mw), use = mn == -INFINITY ? 0.f : mn;
@@ -755,24 +594,30 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendA
 #pragma unroll
     for (int i = 0; i < kV; ++i) o[i] = o[i] * fo + slot[j * HD + i * 32 + lane] * fw;
   }
+  if constexpr (kEach > 1) {
 #pragma unroll
-  for (int i = 0; i < kV; ++i) sh[warp][i * 32 + lane] = o[i];
-  if (lane == 0) sh[warp][HD] = m, sh[warp][HD + 1] = l;
-  __syncthreads();
-  float mx = -INFINITY, sum = 0.f;
+    for (int i = 0; i < kV; ++i) sh[warp][i * 32 + lane] = o[i];
+    if (lane == 0) sh[warp][HD] = m, sh[warp][HD + 1] = l;
+    __syncthreads();
+    if (warp || !live) return;
+    m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) mx = fmaxf(mx, sh[w][HD]);
-  const float use = mx == -INFINITY ? 0.f : mx;
-  float fw[kJoinWarps];
+    for (int w = 0; w < kEach; ++w) m = fmaxf(m, sh[w][HD]);
 #pragma unroll
-  for (int w = 0; w < kJoinWarps; ++w) fw[w] = exp2_f(sh[w][HD] - use), sum += sh[w][HD + 1] * fw[w];
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int d = tid; d < HD; d += kJoinWarps * 32) {
-    float x = 0.f;
+    for (int i = 0; i < kV; ++i) o[i] = 0.f;
+    const float use = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < kJoinWarps; ++w) x += sh[w][d] * fw[w];
-    out[d] = from_f<T>(x * inv);
+    for (int w = 0; w < kEach; ++w) {
+      const float fw = exp2_f(sh[w][HD] - use);
+      l += sh[w][HD + 1] * fw;
+#pragma unroll
+      for (int i = 0; i < kV; ++i) o[i] += sh[w][i * 32 + lane] * fw;
+    }
   }
+  T* out = out_row<HD, T>(a, r, head, f);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+  for (int i = 0; i < kV; ++i) out[i * 32 + lane] = from_f<T>(o[i] * inv);
 }
 
 // ---- one CTA for every (row, query tile, KV head) -----------------------------------------------------------------
@@ -912,21 +757,25 @@ int sm_count() {
 struct Layout {
   int nt, tiles;
   bool group;            // one CTA per (row, tile, head)
+  bool tc;               // 128 query rows a tile, on tcgen05
   long long items, first_at, part_at, bytes;
 };
-constexpr int kGroupPages = 16;
+constexpr int kGroupPages = 16, kTcRows = 33;
 constexpr int kMostCtas = 160, kMostWarps = 12;
 Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int dtype) {
   Layout l;
   const int G = Hq / c.num_kv_heads;
   const long long rows = (long long)S * G;
   l.nt = n_tiles_of(c.head_dim, dtype, rows);
-  l.tiles = (int)((rows + 8 * l.nt - 1) / (8 * l.nt));
+  l.tc = dtype == JX_BF16 && rows >= kTcRows;
+  const int tile = l.tc ? 128 : 8 * l.nt;
+  l.tiles = (int)((rows + tile - 1) / tile);
   l.items = (long long)c.num_rows * l.tiles;
-  l.group = l.nt <= 2 && c.row_pages <= kGroupPages;
+  l.group = !l.tc && l.nt <= 2 && c.row_pages <= kGroupPages;
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;
-  l.bytes = l.group ? 16 : l.part_at + (long long)kMostCtas * kMostWarps * 2 * (8 * l.nt) * (c.head_dim + 2) * 4;
+  const long long slots = l.tc ? 2ll * 2 * kMostCtas : 2ll * kMostCtas * kMostWarps;   // two for every run
+  l.bytes = l.group ? 16 : l.part_at + slots * tile * (c.head_dim + 2) * 4;
   return l;
 }
 
@@ -969,6 +818,24 @@ int allow(K kernel, int bytes, bool (&ready)[64]) {
   return JX_OK;
 }
 
+// The second kernel, for tiles of `rows` query rows and that many runs.
+template <int HD, typename T>
+int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
+  const long long segments = a.items * (long long)a.c.num_kv_heads;
+  const int there = a.tiles > 1 || a.S * a.G >= rows ? rows : a.S * a.G;
+  const bool few = runs <= 4 * segments;    // some four parts a segment, if they are alike
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)segments, (unsigned)(few ? (there + kJoinWarps - 1) / kJoinWarps : there));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at, cfg.numAttrs = 1;
+  return (few ? cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, 1>, a, rows)
+              : cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, kJoinWarps>, a, rows)) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+}
+
 template <int HD, int NT, typename T>
 int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
   if constexpr (NT <= 2) {
@@ -989,19 +856,17 @@ int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStr
   if (most < grid) grid = (int)most;
   kv4_attend_runs_kernel<HD, NT, T><<<grid, R::kThreads, R::kSmem, s>>>(a, map);
   if (cudaPeekAtLastError() != cudaSuccess) return JX_ERR_CUDA;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.items * (long long)a.c.num_kv_heads), (unsigned)(a.tiles > 1 || a.S * a.G >= 8 * NT ? 8 * NT : a.S * a.G));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T>, a, Cfg<HD, NT, T>::kRows) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return join<HD, T>(a, Cfg<HD, NT, T>::kRows, grid * R::kWarps, s);
 }
 
 template <int HD, typename T>
 int launch_nt(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2)
+    if (l.tc) {
+      const int sms = sm_count() < kMostCtas ? sm_count() : kMostCtas;
+      if (const int rc = run_kv4_attend_tc(&a, &map, sms, s)) return rc;
+      return join<HD, T>(a, 128, HD == 256 ? sms : 2 * sms, s);
+    }
   if (l.nt == 1) return launch<HD, 1, T>(l, a, map, s);
   if constexpr (HD < 256 && sizeof(T) == 2)
     if (l.nt == 4) return launch<HD, 4, T>(l, a, map, s);

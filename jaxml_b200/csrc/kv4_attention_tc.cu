@@ -1,0 +1,500 @@
+// Attention of many query rows (prompt chunks, long drafts) over the 4-bit KV cache, on tcgen05.
+//
+// A CTA takes 128 query rows of one KV head (positions x the heads that share it) and a run of pages:
+//   warps 4-7  turn a page's codes into bfloat16 operands in shared memory (exact: 4-bit code x 4-bit scale), K as
+//              [64 keys][hd] and V transposed as [hd][64 keys], both K-major without swizzle, two buffers each;
+//   warp 8     issues S = Q K^T and O += P V.  Q and P are A operands in TMEM, so shared memory is read for K and V only:
+//              with Q and P there as well its bandwidth, not the tensor cores, would set the pace;
+//   warps 0-3  own a query row each thread: scores out of TMEM, running maximum and sum, P back over the scores.
+// The maximum that the exponents refer to moves only when a score passes it by 2^8, so O in TMEM is rescaled a few times a
+// row instead of every page; probabilities keep their precision up to that factor, and l is summed in float32.
+// Two CTAs share a multiprocessor (256 TMEM columns each): one's softmax runs under the other's products.
+//
+// Work is split as in kv4_attention.cu: all (row, tile, KV head, page) units cut into equal runs, one a CTA; parts of a
+// (row, tile, head) meet in the join kernel.  What bounds it: per page and 128 rows, 8192 exponentials are 512 cycles of
+// the multiprocessor's units and the products 512 cycles of its tensor cores.
+#include "kv4_attend.cuh"
+
+namespace jxb {
+using namespace kv4;
+namespace {
+
+constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq + 32;
+
+template <int HD>
+struct Tc {
+  static constexpr int kBlock = kPage * HD + kPage * (HD / 32) * 4;
+  static constexpr int kKBytes = kPage * HD * 2;
+  static constexpr int kKSbo = HD / 8 * 128;            // between groups of 8 keys
+  static constexpr int kVSbo = kPage / 8 * 128 + 16;    // between groups of 8 channels; 16 bytes off for the banks
+  static constexpr int kVBytes = HD / 8 * kVSbo;
+  static constexpr int kQCol = 0, kSCol = HD / 2, kOCol = HD / 2 + 64;
+  static constexpr int kCols = kOCol + HD <= 256 ? 256 : 512;
+  static constexpr int kCtas = kCols == 256 ? 2 : 1;
+  static constexpr int kOffK = 2 * kBlock, kOffV = kOffK + 2 * kKBytes, kOffBar = kOffV + 2 * kVBytes;
+  static constexpr int kOffNan = kOffBar + 16 * 8, kOffMisc = kOffNan + 2 * 8 * 8, kOffFirst = kOffMisc + 32;
+  static constexpr int kUsed = kOffFirst + (kThreads + 40) * 8 + 1024;
+  // no third CTA beside two of 256 columns: it would wait for TMEM
+  static constexpr int kSmem = kCtas == 2 ? (kUsed > 80 * 1024 ? kUsed : 80 * 1024) : (kUsed > 116 * 1024 ? kUsed : 116 * 1024);
+  static_assert(kSmem <= 227 * 1024 / kCtas, "shared memory");
+  static_assert(kOffK % 1024 == 0 && kOffV % 16 == 0 && kVBytes % 16 == 0, "alignment");
+};
+
+// D[tmem] (+)= A[tmem] * B[shared]
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// 32 columns of 32-bit cells of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
+      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Code pairs times a scale pair, exact in bfloat16.
+__device__ __forceinline__ uint32_t value2(uint32_t w, int k, uint32_t s2) { return scaled2(w, k, s2); }
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
+    kv4_attend_tc_kernel(const AttendArgs a, const __grid_constant__ CUtensorMap map) {
+  using C = Tc<HD>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* kbuf = smem + C::kOffK;
+  unsigned char* vbuf = smem + C::kOffV;
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t *page_full = bar, *k_ready = bar + 2, *v_ready = bar + 4, *k_free = bar + 6, *v_free = bar + 8, *s_done = bar + 10,
+           *p_ready = bar + 11, *pv_done = bar + 12, *q_ready = bar + 13, *page_free = bar + 14;
+  unsigned char* nan_keys = smem + C::kOffNan;          // [2][8 groups][8 bytes]: keys of the page with a NaN value scale
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* bad = reinterpret_cast<int*>(tmem_slot + 2);     // [4]: whether pages i, i + 1, ... have no block
+  long long* first = reinterpret_cast<long long*>(smem + C::kOffFirst);
+  long long* sums = first + kThreads + 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const jx_kv4_cache& c = a.c;
+
+  if (tid == 0) {
+    prefetch_tmap(&map);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&page_full[i], 1);
+      mbar_init(&k_ready[i], kDeq);
+      mbar_init(&v_ready[i], kDeq);
+      mbar_init(&k_free[i], 1);
+      mbar_init(&v_free[i], 1);
+      mbar_init(&page_free[i], kDeq);
+    }
+    mbar_init(s_done, 1);
+    mbar_init(p_ready, kSoft);
+    mbar_init(pv_done, 1);
+    mbar_init(q_ready, kSoft);
+    *dead = 0;
+    fence_barrier_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, C::kCols);
+    tmem_relinquish();
+  }
+  // units before each thread's share of the items, and all of them
+  const int each = (a.items + kThreads - 1) / kThreads;
+  const int i0 = min(a.items, tid * each), i1 = min(a.items, i0 + each);
+  long long mine = 0;
+  for (int i = i0; i < i1; ++i) mine += (long long)item_at<kRows>(a, i).n * c.num_kv_heads;
+  long long v = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long o = __shfl_up_sync(~0u, v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 31) sums[warp] = v;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  long long before = 0, units = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    units += sums[w];
+  }
+  first[tid] = before + v - mine;
+  const long long runs = min((long long)gridDim.x, max(units, 1ll));
+  if (blockIdx.x == 0) {
+    long long u = before + v - mine;
+    for (int i = i0; i < i1; ++i) {
+      a.item_first[i] = u;
+      if (c.counts[i / a.tiles] > a.S) set_status(c.status, JX_ERR_RANGE);
+      u += (long long)item_at<kRows>(a, i).n * c.num_kv_heads;
+    }
+    if (tid == 0) a.total[0] = units, a.total[1] = runs;
+  }
+  __syncthreads();
+
+  const long long w = blockIdx.x;
+  const bool work = units > 0 && w < runs;
+  if (work) {
+    const long long u0 = run_start(w, units, runs), u1 = run_start(w + 1, units, runs);
+    Walk at;
+    {
+      int lo = 0, hi = kThreads - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (first[mid] <= u0) lo = mid;
+        else hi = mid - 1;
+      }
+      long long u = first[lo];
+      at.item = (long long)lo * each;
+      while (true) {
+        at.t = item_at<kRows>(a, at.item);
+        const long long n = (long long)at.t.n * c.num_kv_heads;
+        if (u0 < u + n) break;
+        u += n;
+        ++at.item;
+      }
+      at.head = (int)((u0 - u) / at.t.n);
+      at.page = (int)((u0 - u) - (long long)at.head * at.t.n);
+    }
+    // every wait is bounded; once one has run out all roles leave
+    auto wait = [&](uint64_t* b, uint32_t parity) {
+      if (mbar_try_wait(b, parity)) return true;
+      const uint64_t t0 = globaltimer_ns();
+      while (!mbar_try_wait(b, parity)) {
+        if (*dead) return false;
+        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+          *dead = 1;
+          set_status(c.status, JX_ERR_TIMEOUT);
+          return false;
+        }
+      }
+      return true;
+    };
+
+    if (warp >= 4 && warp < 8) {
+      // ---------------- pages to bfloat16 operands ----------------
+      const int dt = tid - kSoft, dw = warp - 4;
+      Walk ahead = at;
+      long long ua = u0;
+      int sent = 0;
+      auto issue = [&]() {
+        const int id = c.table[(long long)ahead.t.r * c.row_pages + ahead.t.p0 + ahead.page], b = sent & 1;
+        fetch<HD>(a, &map, id, ahead.head, smem + b * C::kBlock, &page_full[b], &bad[sent & 3]);
+        ++sent;
+        if (++ua < u1) ahead.next<kRows>(a);
+      };
+      if (dt == 0)
+        for (int n = 0; n < 2 && ua < u1; ++n) issue();
+      const int g = lane & 7, t4 = lane >> 3;
+      bool ok = true;
+      int i = 0;
+      for (long long u = u0; u < u1 && ok; ++u, ++i) {
+        const int b = i & 1;
+        const uint32_t use = (i >> 1) & 1;
+        const unsigned char* blk = smem + b * C::kBlock;
+        if (!(ok = wait(&page_full[b], use))) break;
+        if (i >= 2 && !(ok = wait(&k_free[b], use ^ 1))) break;
+        // K: lane (key g of a group of 8, word t4 of a 16-byte piece): a core matrix's rows are 8 neighbouring lanes
+        unsigned char* kd = kbuf + b * C::kKBytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int kg = dw * 2 + h, key = kg * 8 + g;
+#pragma unroll
+          for (int grp = 0; grp < HD / 32; ++grp) {
+            const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(key * (HD / 2) + grp * 16) + t4 * 4);
+            const uint32_t s2 = lds16(blk + swz<HD>(kPage * HD + key * (HD / 16) + grp * 2)) * 0x10001u;
+            *reinterpret_cast<uint4*>(kd + kg * C::kKSbo + (grp * 4 + t4) * 128 + g * 16) =
+                make_uint4(value2(x, 0, s2), value2(x, 1, s2), value2(x, 2, s2), value2(x, 3, s2));
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(&k_ready[b]);
+        if (i >= 2 && !(ok = wait(&v_free[b], use ^ 1))) break;
+        // V: 8 keys x 8 channels a thread, transposed in registers
+        unsigned char* vd = vbuf + b * C::kVBytes;
+        constexpr int kBlocks = HD / 8 * (kPage / 8);
+#pragma unroll
+        for (int n = 0; n < (kBlocks + kDeq - 1) / kDeq; ++n) {
+          const int q = dt + n * kDeq;
+          if (kBlocks >= kDeq || q < kBlocks) {
+            const int ch = q % (HD / 8), j = q / (HD / 8), flip = (lane >> 4) & 1;   // half of the warp reads the odd key first
+            uint32_t x[8], sc[4];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const int key = j * 8 + (e ^ flip);
+              x[e] = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(kPage * (HD / 2) + key * (HD / 2) + ch * 4));
+            }
+            uint32_t nans = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int o = kPage * HD + kPage * (HD / 16) + (j * 8 + 2 * e) * (HD / 16) + (ch >> 2) * 2;
+              uint32_t s0 = lds16(blk + swz<HD>(o)), s1 = lds16(blk + swz<HD>(o + HD / 16));
+              // no scale of the format: 0 for the product (0 * NaN would reach rows that do not see the key), noted for those that do
+              if ((s0 & 0x7FFFu) >= kKv4BadScale) s0 = 0, nans |= 1u << (2 * e);
+              if ((s1 & 0x7FFFu) >= kKv4BadScale) s1 = 0, nans |= 2u << (2 * e);
+              sc[e] = s0 | (s1 << 16);
+            }
+            if ((ch & 3) == 0) nan_keys[(b * 8 + (ch >> 2)) * 8 + j] = (unsigned char)nans;
+            const uint32_t lo_sel = flip ? 0x1054u : 0x5410u, hi_sel = flip ? 0x3276u : 0x7632u;
+            unsigned char* to = vd + ch * C::kVSbo + j * 128;
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              lo[e] = __byte_perm(x[2 * e], x[2 * e + 1], lo_sel);
+              hi[e] = __byte_perm(x[2 * e], x[2 * e + 1], hi_sel);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(value2(lo[0], k, sc[0]), value2(lo[1], k, sc[1]),
+                                                                  value2(lo[2], k, sc[2]), value2(lo[3], k, sc[3]));
+              *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(value2(hi[0], k, sc[0]), value2(hi[1], k, sc[1]),
+                                                                        value2(hi[2], k, sc[2]), value2(hi[3], k, sc[3]));
+            }
+          }
+        }
+        fence_proxy_async();
+        mbar_arrive(&v_ready[b]);
+        mbar_arrive(&page_free[b]);
+        if (dt == 0 && ua < u1 && (ok = wait(&page_free[b], use))) issue();
+        __syncwarp();
+      }
+    } else if (warp == 8) {
+      // ---------------- products ----------------
+      if (lane == 0) {
+        constexpr uint32_t kIdS = umma_idesc_bf16_f32(128, kPage), kIdO = umma_idesc_bf16_f32(128, HD);
+        bool start = true;
+        uint32_t qp = 0;
+        int i = 0;
+        for (long long u = u0; u < u1; ++u, ++i) {
+          const int b = i & 1;
+          const uint32_t use = (i >> 1) & 1;
+          if (start) {
+            if (!wait(q_ready, qp)) break;
+            qp ^= 1;
+          }
+          if (!wait(&k_ready[b], use)) break;
+          if (i > 0 && !wait(pv_done, (i - 1) & 1)) break;     // the scores take P's place
+          tc_fence_after();
+          const uint64_t kd = umma_desc_kmajor(smem_u32(kbuf + b * C::kKBytes), 128, C::kKSbo);
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk)
+            umma_ts(tmem + C::kSCol, tmem + C::kQCol + kk * 8, kd + (uint64_t)(kk * 16), kIdS, kk > 0);
+          umma_commit(s_done);
+          umma_commit(&k_free[b]);
+          if (!wait(&v_ready[b], use)) break;
+          if (!wait(p_ready, i & 1)) break;
+          tc_fence_after();
+          const uint64_t vd = umma_desc_kmajor(smem_u32(vbuf + b * C::kVBytes), 128, C::kVSbo);
+#pragma unroll
+          for (int kk = 0; kk < kPage / 16; ++kk)
+            umma_ts(tmem + C::kOCol, tmem + C::kSCol + kk * 8, vd + (uint64_t)(kk * 16), kIdO, !start || kk > 0);
+          umma_commit(pv_done);
+          umma_commit(&v_free[b]);
+          start = at.page + 1 == at.t.n;
+          if (u + 1 < u1) at.next<kRows>(a);
+        }
+      }
+      __syncwarp();
+    } else if (warp < 4) {
+      // ---------------- softmax: one query row a thread ----------------
+      const uint32_t mine_at = tmem + ((uint32_t)(warp * 32) << 16);
+      const float c2 = a.scale_log2;
+      long long seg_first = u0 - at.page;
+      bool start = true;
+      float m = -INFINITY, l = 0.f;
+      int hi = -1, lo = 0, all_hi = -1, all_lo = -1, f = 0;
+      uint32_t nan_groups = 0;
+      int i = 0;
+      for (long long u = u0; u < u1; ++u, ++i) {
+        const int b = i & 1;
+        if (start) {
+          start = false;
+          const int f0 = at.t.qt * kRows, F = a.S * a.G;
+          f = f0 + tid;
+          const int s = f / a.G;
+          const bool live = f < F && s < at.t.cnt;
+          hi = live ? at.t.base + s : -1;
+          lo = live && a.window > 0 ? max(0, hi - a.window + 1) : 0;
+          all_hi = f0 + kRows <= at.t.cnt * a.G ? at.t.base + f0 / a.G : -1;
+          all_lo = a.window > 0 ? at.t.base + (f0 + kRows - 1) / a.G - a.window : -1;
+          m = -INFINITY, l = 0.f, nan_groups = 0;
+          const bf16* src = static_cast<const bf16*>(a.q) + at.t.r * a.q_row + s * a.q_tok + (at.head * a.G + (f - s * a.G)) * a.q_head;
+#pragma unroll
+          for (int part = 0; part < HD / 64; ++part) {
+            uint32_t r[32];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint4 x = make_uint4(0, 0, 0, 0);
+              if (live) q_words(src + part * 64 + k * 8, a.q_vec, a.sign, &x);
+              r[4 * k] = x.x, r[4 * k + 1] = x.y, r[4 * k + 2] = x.z, r[4 * k + 3] = x.w;
+            }
+            __syncwarp();
+            tmem_st32(mine_at + C::kQCol + part * 32, r);
+          }
+          tmem_wait_st();
+          tc_fence_before();
+          mbar_arrive(q_ready);
+        }
+        bool ok = wait(s_done, i & 1);
+        if (!__all_sync(~0u, ok)) break;
+        tc_fence_after();
+        uint32_t x[64];
+        tmem_ld32(mine_at + C::kSCol, x);
+        tmem_ld32(mine_at + C::kSCol + 32, x + 32);
+        tmem_wait_ld();
+        const int key0 = (at.t.p0 + at.page) * kPage;
+        const bool all = key0 + kPage - 1 <= all_hi && key0 > all_lo && !bad[i & 3];
+        if (!all) {
+          const int from = bad[i & 3] ? kPage : lo - key0, to = hi - key0;      // keys [from, to] of the page
+#pragma unroll
+          for (int k = 0; k < 64; ++k)
+            if (k < from || k > to) x[k] = 0xFF800000u;
+        }
+        float mx = __uint_as_float(x[0]);
+#pragma unroll
+        for (int k = 1; k < 64; ++k) mx = fmaxf(mx, __uint_as_float(x[k]));
+        const bool moves = (mx - m) * c2 > 8.f;           // also from -inf, when there is nothing to rescale
+        const bool scales = moves && m != -INFINITY;
+        if (__any_sync(~0u, scales)) {
+          const float fo = scales ? exp2_f((m - mx) * c2) : 1.f;
+          l *= fo;
+#pragma unroll 1
+          for (int part = 0; part < HD / 32; ++part) {
+            uint32_t r[32];
+            tmem_ld32(mine_at + C::kOCol + part * 32, r);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * fo);
+            tmem_st32(mine_at + C::kOCol + part * 32, r);
+          }
+          tmem_wait_st();
+        }
+        if (moves) m = mx;
+        const float ref = m == -INFINITY ? 0.f : -m * c2;
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float p0 = exp2_f(fmaf(__uint_as_float(x[2 * k]), c2, ref)), p1 = exp2_f(fmaf(__uint_as_float(x[2 * k + 1]), c2, ref));
+          s0 += p0, s1 += p1;
+          x[k] = pack_bf16x2(p0, p1);       // probabilities in bfloat16: half a step, 2^-9 of their binade's top
+        }
+        l += s0 + s1;
+        tmem_st32(mine_at + C::kSCol, x);
+        tmem_wait_st();
+        tc_fence_before();
+        ok = wait(&v_ready[b], (i >> 1) & 1);
+        if (!__all_sync(~0u, ok)) break;
+        {
+          const unsigned long long* nk = reinterpret_cast<const unsigned long long*>(nan_keys + b * 64);
+          unsigned long long any = 0;
+#pragma unroll
+          for (int grp = 0; grp < HD / 32; ++grp) any |= nk[grp];
+          if (any && !bad[i & 3]) {
+            const int from = max(lo - key0, 0), to = min(hi - key0, kPage - 1);
+            if (from <= to) {
+              const unsigned long long sees = (~0ull << from) & (~0ull >> (63 - to));
+              for (int grp = 0; grp < HD / 32; ++grp)
+                if (nk[grp] & sees) nan_groups |= 1u << grp;
+            }
+          }
+        }
+        mbar_arrive(p_ready);
+
+        const bool seg_end = at.page + 1 == at.t.n;
+        if (seg_end || u + 1 == u1) {
+          ok = wait(pv_done, i & 1);
+          if (!__all_sync(~0u, ok)) break;
+          tc_fence_after();
+          const bool whole = seg_end && seg_first >= u0, there = f < a.S * a.G;
+          float* slot = a.part + (w * 2 + (seg_first >= u0 ? 1 : 0)) * (long long)(kRows * (HD + 2));
+          const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+          bf16* o = there ? out_row<HD, bf16>(a, at.t.r, at.head, f) : nullptr;
+#pragma unroll 1
+          for (int part = 0; part < HD / 32; ++part) {
+            uint32_t r[32];
+            tmem_ld32(mine_at + C::kOCol + part * 32, r);
+            tmem_wait_ld();
+            if (there) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  y[e] = (nan_groups >> part) & 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float(r[k + e]) * inv;
+                if (whole) store_row8<bf16>(o + part * 32 + k, y);
+                else store_row8<float>(slot + tid * HD + part * 32 + k, y);
+              }
+            }
+            __syncwarp();
+          }
+          if (!whole && there) slot[kRows * HD + 2 * tid] = m * c2, slot[kRows * HD + 2 * tid + 1] = l;
+          tc_fence_before();
+        }
+        if (u + 1 < u1) {
+          if (seg_end) seg_first = u + 1, start = true;
+          at.next<kRows>(a);
+        }
+      }
+    }
+  }
+  // after a wait that ran out: what was issued gets as long again to finish before its memory goes
+  __syncthreads();
+  if (*dead && tid == 0) {
+    const uint64_t t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < kWaitLimitNs) {
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+template <int HD>
+int launch(const AttendArgs& a, const CUtensorMap& map, int sms, cudaStream_t s) {
+  using C = Tc<HD>;
+  static bool ready[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return JX_ERR_CUDA;
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    if (cudaFuncSetAttribute(kv4_attend_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem) != cudaSuccess)
+      return JX_ERR_CUDA;
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  kv4_attend_tc_kernel<HD><<<sms * C::kCtas, kThreads, C::kSmem, s>>>(a, map);
+  return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+}
+
+}  // namespace
+
+int run_kv4_attend_tc(const void* args, const void* map, int sms, cudaStream_t s) {
+  const AttendArgs& a = *static_cast<const AttendArgs*>(args);
+  const CUtensorMap& m = *static_cast<const CUtensorMap*>(map);
+  if (a.c.head_dim == 64) return launch<64>(a, m, sms, s);
+  if (a.c.head_dim == 128) return launch<128>(a, m, sms, s);
+  return launch<256>(a, m, sms, s);
+}
+
+}  // namespace jxb
