@@ -3,9 +3,10 @@
 // A CTA takes 128 query rows of one KV head (positions x the heads that share it) and a run of pages:
 //   warps 4-7  turn a page's codes into bfloat16 operands in shared memory (exact: 4-bit code x 4-bit scale), K as
 //              [64 keys][hd] and V transposed as [hd][64 keys], both K-major without swizzle, two buffers each;
-//   warp 8     issues S = Q K^T and O += P V.  Q and P are A operands in TMEM, so shared memory is read for K and V only:
-//              with Q and P there as well its bandwidth, not the tensor cores, would set the pace;
-//   warps 0-3  own a query row each thread: scores out of TMEM, running maximum and sum, P back over the scores.
+//   warps 0-3  own a query row each thread: scores out of TMEM, running maximum and sum, P back over the scores; one of
+//              their threads issues S = Q K^T and O += P V, at times when its warp would wait for them anyway.
+// Q and P are A operands in TMEM, so shared memory is read for K and V only: with Q and P there as well its bandwidth, not
+// the tensor cores, would set the pace.
 // The maximum that the exponents refer to moves only when a score passes it by 2^8, so O in TMEM is rescaled a few times a
 // row instead of every page; probabilities keep their precision up to that factor, and l is summed in float32.
 // Two CTAs share a multiprocessor (256 TMEM columns each): one's softmax runs under the other's products.
@@ -19,7 +20,7 @@ namespace jxb {
 using namespace kv4;
 namespace {
 
-constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq + 32;
+constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq;
 
 template <int HD>
 struct Tc {
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
     *dead = 0;
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 4) {
     tmem_alloc(tmem_slot, C::kCols);
     tmem_relinquish();
   }
@@ -191,7 +192,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
       return true;
     };
 
-    if (warp >= 4 && warp < 8) {
+    if (warp >= 4) {
       // ---------------- pages to bfloat16 operands ----------------
       const int dt = tid - kSoft, dw = warp - 4;
       Walk ahead = at;
@@ -278,49 +279,15 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
         if (dt == 0 && ua < u1 && (ok = wait(&page_free[b], use))) issue();
         __syncwarp();
       }
-    } else if (warp == 8) {
-      // ---------------- products ----------------
-      if (lane == 0) {
-        constexpr uint32_t kIdS = umma_idesc_bf16_f32(128, kPage), kIdO = umma_idesc_bf16_f32(128, HD);
-        bool start = true;
-        uint32_t qp = 0;
-        int i = 0;
-        for (long long u = u0; u < u1; ++u, ++i) {
-          const int b = i & 1;
-          const uint32_t use = (i >> 1) & 1;
-          if (start) {
-            if (!wait(q_ready, qp)) break;
-            qp ^= 1;
-          }
-          if (!wait(&k_ready[b], use)) break;
-          if (i > 0 && !wait(pv_done, (i - 1) & 1)) break;     // the scores take P's place
-          tc_fence_after();
-          const uint64_t kd = umma_desc_kmajor(smem_u32(kbuf + b * C::kKBytes), 128, C::kKSbo);
-#pragma unroll
-          for (int kk = 0; kk < HD / 16; ++kk)
-            umma_ts(tmem + C::kSCol, tmem + C::kQCol + kk * 8, kd + (uint64_t)(kk * 16), kIdS, kk > 0);
-          umma_commit(s_done);
-          umma_commit(&k_free[b]);
-          if (!wait(&v_ready[b], use)) break;
-          if (!wait(p_ready, i & 1)) break;
-          tc_fence_after();
-          const uint64_t vd = umma_desc_kmajor(smem_u32(vbuf + b * C::kVBytes), 128, C::kVSbo);
-#pragma unroll
-          for (int kk = 0; kk < kPage / 16; ++kk)
-            umma_ts(tmem + C::kOCol, tmem + C::kSCol + kk * 8, vd + (uint64_t)(kk * 16), kIdO, !start || kk > 0);
-          umma_commit(pv_done);
-          umma_commit(&v_free[b]);
-          start = at.page + 1 == at.t.n;
-          if (u + 1 < u1) at.next<kRows>(a);
-        }
-      }
-      __syncwarp();
-    } else if (warp < 4) {
-      // ---------------- softmax: one query row a thread ----------------
+    } else {
+      // ---------------- softmax: one query row a thread; the products ----------------
+      constexpr uint32_t kIdS = umma_idesc_bf16_f32(128, kPage), kIdO = umma_idesc_bf16_f32(128, HD);
+      const uint64_t kd0 = umma_desc_kmajor(smem_u32(kbuf), 128, C::kKSbo), vd0 = umma_desc_kmajor(smem_u32(vbuf), 128, C::kVSbo);
+      uint32_t qp = 0;
       const uint32_t mine_at = tmem + ((uint32_t)(warp * 32) << 16);
       const float c2 = a.scale_log2;
       long long seg_first = u0 - at.page;
-      bool start = true;
+      bool start = true, fresh = true;      // fresh: the segment's first page
       float m = -INFINITY, l = 0.f;
       int hi = -1, lo = 0, all_hi = -1, all_lo = -1, f = 0;
       uint32_t nan_groups = 0;
@@ -328,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
       for (long long u = u0; u < u1; ++u, ++i) {
         const int b = i & 1;
         if (start) {
-          start = false;
+          start = false, fresh = true;
           const int f0 = at.t.qt * kRows, F = a.S * a.G;
           f = f0 + tid;
           const int s = f / a.G;
@@ -355,7 +322,22 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           tc_fence_before();
           mbar_arrive(q_ready);
         }
-        bool ok = wait(s_done, i & 1);
+        bool ok = true;
+        if (tid == 0) {
+          // Q of a new segment stored, K ready, and P V of the page before done: the scores take P's place
+          ok = (!fresh || wait(q_ready, qp)) && wait(&k_ready[b], (i >> 1) & 1) && (i == 0 || wait(pv_done, (i - 1) & 1));
+          if (ok) {
+            tc_fence_after();
+            const uint64_t kd = kd0 + (uint64_t)(b * (C::kKBytes >> 4));
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk)
+              umma_ts(tmem + C::kSCol, tmem + C::kQCol + kk * 8, kd + (uint64_t)(kk * 16), kIdS, kk > 0);
+            umma_commit(s_done);
+            umma_commit(&k_free[b]);
+          }
+          qp ^= fresh;
+        }
+        ok = __shfl_sync(~0u, ok, 0) && wait(s_done, i & 1);
         if (!__all_sync(~0u, ok)) break;
         tc_fence_after();
         uint32_t x[64];
@@ -419,6 +401,20 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           }
         }
         mbar_arrive(p_ready);
+        if (tid == 0) {
+          ok = wait(p_ready, i & 1);     // V is ready: this thread has waited for it
+          if (ok) {
+            tc_fence_after();
+            const uint64_t vd = vd0 + (uint64_t)(b * (C::kVBytes >> 4));
+#pragma unroll
+            for (int kk = 0; kk < kPage / 16; ++kk)
+              umma_ts(tmem + C::kOCol, tmem + C::kSCol + kk * 8, vd + (uint64_t)(kk * 16), kIdO, !fresh || kk > 0);
+            umma_commit(pv_done);
+            umma_commit(&v_free[b]);
+          }
+        }
+        if (!__shfl_sync(~0u, ok, 0)) break;
+        fresh = false;
 
         const bool seg_end = at.page + 1 == at.t.n;
         if (seg_end || u + 1 == u1) {
@@ -466,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, C::kCols);
   }
