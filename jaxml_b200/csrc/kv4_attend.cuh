@@ -154,6 +154,16 @@ __device__ __forceinline__ T* out_row(const AttendArgs& a, int r, int head, int 
   return static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
 }
 
+// A bounded wait on the clock counter: reading the global timer between polls costs more than most waits here last.
+constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
+__device__ __forceinline__ bool wait_cycles(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(bar, parity))
+    if (clock64() - t0 > kWaitCycles) return false;
+  return true;
+}
+
 // Brings the block of a page into shared memory; a page id out of range is reported and its stage marked.
 template <int HD>
 __device__ __forceinline__ void fetch(const AttendArgs& a, const CUtensorMap* map, int id, int head, unsigned char* to,

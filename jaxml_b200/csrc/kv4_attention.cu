@@ -507,10 +507,10 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
   for (long long u = u0; u < u1; ++u) {
     if (fresh) tile.begin(a, rd.t, rd.head, lane);
     fresh = false;
-    const bool arrived = mbar_wait_bounded(&my_bar[stage], phase);
+    const bool arrived = wait_cycles(&my_bar[stage], phase);
     if (!__all_sync(~0u, arrived)) {      // give up: no copy of this warp may be in flight when it ends
       if (lane == 0) set_status(c.status, JX_ERR_TIMEOUT);
-      for (int s = 0; s < R::kStages; ++s) mbar_wait_bounded(&my_bar[s], s < stage ? phase ^ 1 : phase);
+      for (int s = 0; s < R::kStages; ++s) wait_cycles(&my_bar[s], s < stage ? phase ^ 1 : phase);
       return;
     }
     unsigned char* blk = my_ring + stage * C::kBlock;
@@ -675,9 +675,9 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
     const int here = min(R::kPages, t.n - first);
     for (int sl = warp; sl < here * (kPage / R::kKeys); sl += R::kWarps) {
       const int page = sl / (kPage / R::kKeys), kb = sl % (kPage / R::kKeys) * R::kKeys;
-      if (!dead && !__all_sync(~0u, mbar_wait_bounded(&bars[page], phase))) {
+      if (!dead && !__all_sync(~0u, wait_cycles(&bars[page], phase))) {
         dead = true;
-        mbar_wait_bounded(&bars[page], phase);   // no copy may be in flight when the CTA ends
+        wait_cycles(&bars[page], phase);   // no copy may be in flight when the CTA ends
         if (lane == 0) set_status(c.status, JX_ERR_TIMEOUT);
       }
       unsigned char* blk = ring + page * C::kBlock;
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
     __syncthreads();
     if (tid < R::kPages && first + R::kPages + tid < t.n) {
       id = c.table[(long long)t.r * c.row_pages + t.p0 + first + R::kPages + tid];
-      mbar_wait_bounded(&bars[tid], phase);   // passed already, unless a warp gave up on it
+      wait_cycles(&bars[tid], phase);   // passed already, unless a warp gave up on it
       fetch<HD>(a, &map, id, head, ring + tid * C::kBlock, &bars[tid], &bad[tid]);
     }
     if (first + R::kPages < t.n) __syncthreads();

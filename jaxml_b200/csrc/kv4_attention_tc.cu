@@ -2,14 +2,16 @@
 //
 // A CTA takes 128 query rows of one KV head (positions x the heads that share it) and a run of pages:
 //   warps 4-7  turn a page's codes into bfloat16 operands in shared memory (exact: 4-bit code x 4-bit scale), K as
-//              [64 keys][hd] and V transposed as [hd][64 keys], both K-major without swizzle, two buffers each;
-//   warps 0-3  own a query row each thread: scores out of TMEM, running maximum and sum, P back over the scores; one of
-//              their threads issues S = Q K^T and O += P V, at times when its warp would wait for them anyway.
-// Q and P are A operands in TMEM, so shared memory is read for K and V only: with Q and P there as well its bandwidth, not
-// the tensor cores, would set the pace.
+//              [64 keys][hd] and V transposed as [hd][64 keys], both K-major without swizzle, K a page ahead of V;
+//   warps 0-3  own a query row each thread: scores out of TMEM, running maximum and sum, P back over the scores;
+//   warp 8     issues S = Q K^T and O += P V, warp 9 the copies of the pages.
+// S has two buffers, so the scores of the next page are made while this one's softmax runs: what is left in line is the
+// softmax itself.  P is an A operand in TMEM, and so is Q where two S buffers, O and Q fit (not for hd 128 with two CTAs).
+// What runs for every page is kept short (loops over halves, groups and pieces, not unrolled): 20 KB of instructions in turn
+// on one multiprocessor were fetched again for every page, and that fetching was the bound.
 // The maximum that the exponents refer to moves only when a score passes it by 2^8, so O in TMEM is rescaled a few times a
 // row instead of every page; probabilities keep their precision up to that factor, and l is summed in float32.
-// Two CTAs share a multiprocessor (256 TMEM columns each): one's softmax runs under the other's products.
+// Two CTAs share a multiprocessor (256 TMEM columns each).
 //
 // Work is split as in kv4_attention.cu: all (row, tile, KV head, page) units cut into equal runs, one a CTA; parts of a
 // (row, tile, head) meet in the join kernel.  What bounds it: per page and 128 rows, 8192 exponentials are 512 cycles of
@@ -20,25 +22,28 @@ namespace jxb {
 using namespace kv4;
 namespace {
 
-constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq;
+constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq + 64, kRing = 3;
 
 template <int HD>
 struct Tc {
   static constexpr int kBlock = kPage * HD + kPage * (HD / 32) * 4;
+  static constexpr bool kQTmem = HD != 128;
   static constexpr int kKBytes = kPage * HD * 2;
-  static constexpr int kKSbo = HD / 8 * 128;            // between groups of 8 keys
+  static constexpr int kKSbo = HD / 8 * 128;            // between groups of 8 keys (or query rows)
   static constexpr int kVSbo = kPage / 8 * 128 + 16;    // between groups of 8 channels; 16 bytes off for the banks
   static constexpr int kVBytes = HD / 8 * kVSbo;
-  static constexpr int kQCol = 0, kSCol = HD / 2, kOCol = HD / 2 + 64;
+  static constexpr int kSCol = kQTmem ? HD / 2 : 0, kOCol = kSCol + 2 * kPage;
   static constexpr int kCols = kOCol + HD <= 256 ? 256 : 512;
   static constexpr int kCtas = kCols == 256 ? 2 : 1;
-  static constexpr int kOffK = 2 * kBlock, kOffV = kOffK + 2 * kKBytes, kOffBar = kOffV + 2 * kVBytes;
-  static constexpr int kOffNan = kOffBar + 16 * 8, kOffMisc = kOffNan + 2 * 8 * 8, kOffFirst = kOffMisc + 32;
+  static constexpr int kOffK = kRing * kBlock, kOffV = kOffK + kKBytes, kOffQ = kOffV + 2 * kVBytes;
+  static constexpr int kOffBar = kOffQ + (kQTmem ? 0 : kRows * HD * 2);
+  static constexpr int kOffNan = kOffBar + 16 * 8, kOffMisc = kOffNan + 2 * 8 * 8, kOffFirst = kOffMisc + 80;
   static constexpr int kUsed = kOffFirst + (kThreads + 40) * 8 + 1024;
   // no third CTA beside two of 256 columns: it would wait for TMEM
   static constexpr int kSmem = kCtas == 2 ? (kUsed > 80 * 1024 ? kUsed : 80 * 1024) : (kUsed > 116 * 1024 ? kUsed : 116 * 1024);
-  static_assert(kSmem <= 227 * 1024 / kCtas, "shared memory");
-  static_assert(kOffK % 1024 == 0 && kOffV % 16 == 0 && kVBytes % 16 == 0, "alignment");
+  static_assert(kSmem <= (kCtas == 2 ? 113 : 227) * 1024, "shared memory");
+  static_assert(kOCol + HD <= 512, "TMEM");
+  static_assert(kOffK % 16 == 0 && kOffV % 16 == 0 && kVBytes % 16 == 0 && kOffQ % 16 == 0, "alignment");
 };
 
 // D[tmem] (+)= A[tmem] * B[shared]
@@ -71,11 +76,27 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* r) {
       "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Scores outside [from, to] to -inf.
+__device__ __forceinline__ void hide(uint32_t* x, int from, int to) {
+#pragma unroll
+  for (int k = 0; k < 32; ++k)
+    if (k < from || k > to) x[k] = 0xFF800000u;
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Code pairs times a scale pair, exact in bfloat16.
-__device__ __forceinline__ uint32_t value2(uint32_t w, int k, uint32_t s2) { return scaled2(w, k, s2); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 
 template <int HD>
 __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
@@ -86,12 +107,13 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
   unsigned char* kbuf = smem + C::kOffK;
   unsigned char* vbuf = smem + C::kOffV;
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t *page_full = bar, *k_ready = bar + 2, *v_ready = bar + 4, *k_free = bar + 6, *v_free = bar + 8, *s_done = bar + 10,
-           *p_ready = bar + 11, *pv_done = bar + 12, *q_ready = bar + 13, *page_free = bar + 14;
+  uint64_t *page_full = bar, *page_free = bar + 3, *v_ready = bar + 6, *s_done = bar + 8, *pv_done = bar + 10, *k_ready = bar + 12,
+           *p_ready = bar + 13, *q_ready = bar + 14;
   unsigned char* nan_keys = smem + C::kOffNan;          // [2][8 groups][8 bytes]: keys of the page with a NaN value scale
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* dead = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* bad = reinterpret_cast<int*>(tmem_slot + 2);     // [4]: whether pages i, i + 1, ... have no block
+  int* bad = reinterpret_cast<int*>(tmem_slot + 2);     // [8]: whether pages i, i + 1, ... have no block
+  int* last = bad + 8;                                  // [8]: whether they end a segment
   long long* first = reinterpret_cast<long long*>(smem + C::kOffFirst);
   long long* sums = first + kThreads + 1;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -99,18 +121,18 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
 
   if (tid == 0) {
     prefetch_tmap(&map);
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kRing; ++i) {
       mbar_init(&page_full[i], 1);
-      mbar_init(&k_ready[i], kDeq);
-      mbar_init(&v_ready[i], kDeq);
-      mbar_init(&k_free[i], 1);
-      mbar_init(&v_free[i], 1);
-      mbar_init(&page_free[i], kDeq);
+      mbar_init(&page_free[i], kDeq / 32);
     }
-    mbar_init(s_done, 1);
-    mbar_init(p_ready, kSoft);
-    mbar_init(pv_done, 1);
-    mbar_init(q_ready, kSoft);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&v_ready[i], kDeq / 32);
+      mbar_init(&s_done[i], 1);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(k_ready, kDeq / 32);
+    mbar_init(p_ready, kSoft / 32);
+    mbar_init(q_ready, kSoft / 32);
     *dead = 0;
     fence_barrier_init();
   }
@@ -180,10 +202,10 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
     // every wait is bounded; once one has run out all roles leave
     auto wait = [&](uint64_t* b, uint32_t parity) {
       if (mbar_try_wait(b, parity)) return true;
-      const uint64_t t0 = globaltimer_ns();
+      const long long t0 = clock64();
       while (!mbar_try_wait(b, parity)) {
         if (*dead) return false;
-        if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        if (clock64() - t0 > kWaitCycles) {
           *dead = 1;
           set_status(c.status, JX_ERR_TIMEOUT);
           return false;
@@ -192,110 +214,163 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
       return true;
     };
 
-    if (warp >= 4) {
+    // the warp's writes stand: one arrival
+    auto arrive = [&](uint64_t* b) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(b);
+    };
+
+    if (warp >= 8) {
+      const int pages = (int)(u1 - u0);
+      if (warp == 8 && lane == 0) {
+        // ---------------- products ----------------
+        constexpr uint32_t kIdS = umma_idesc_bf16_f32(128, kPage), kIdO = umma_idesc_bf16_f32(128, HD);
+        const uint64_t kd = umma_desc_kmajor(smem_u32(kbuf), 128, C::kKSbo);
+        const uint64_t qd = umma_desc_kmajor(smem_u32(smem + C::kOffQ), 128, C::kKSbo);
+        uint32_t qp = 0;
+        auto scores = [&](int i, bool start) {
+          // K, Q of a new segment, and the page before last is through with this S buffer
+          const int b = i & 1;
+          if (!wait(k_ready, i & 1) || (start && !wait(q_ready, qp)) || (i >= 2 && !wait(&pv_done[b], ((i - 2) >> 1) & 1)))
+            return false;
+          qp ^= start;
+          tc_fence_after();
+          const uint32_t sd = tmem + C::kSCol + b * kPage;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            if constexpr (C::kQTmem) umma_ts(sd, tmem + kk * 8, kd + (uint64_t)(kk * 16), kIdS, kk > 0);
+            else umma_bf16(sd, qd + (uint64_t)(kk * 16), kd + (uint64_t)(kk * 16), kIdS, kk > 0);
+          }
+          umma_commit(&s_done[b]);
+          return true;
+        };
+        bool ok = scores(0, true), fresh = true;
+        for (int i = 0; i < pages && ok; ++i) {
+          const int b = i & 1;
+          const bool next = i + 1 < pages, start = last[i & 7];   // page i + 1 begins a segment
+          // its scores first, unless they wait for a Q that follows the results of this page
+          if (next && !start && !(ok = scores(i + 1, false))) break;
+          ok = wait(&v_ready[b], (i >> 1) & 1) && wait(p_ready, i & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t vd = umma_desc_kmajor(smem_u32(vbuf + b * C::kVBytes), 128, C::kVSbo);
+#pragma unroll
+          for (int kk = 0; kk < kPage / 16; ++kk)
+            umma_ts(tmem + C::kOCol, tmem + C::kSCol + b * kPage + kk * 8, vd + (uint64_t)(kk * 16), kIdO, !fresh || kk > 0);
+          umma_commit(&pv_done[b]);
+          fresh = start;
+          if (next && start) ok = scores(i + 1, true);
+        }
+      } else if (warp == 9 && lane == 0) {
+        // ---------------- copies ----------------
+        int i = 0;
+        for (; i < pages; ++i) {
+          const int st = i % kRing;
+          const int id = c.table[(long long)at.t.r * c.row_pages + at.t.p0 + at.page];
+          if (i >= kRing && !wait(&page_free[st], (i / kRing - 1) & 1)) break;
+          last[i & 7] = at.page + 1 == at.t.n;
+          fetch<HD>(a, &map, id, at.head, smem + st * C::kBlock, &page_full[st], &bad[i & 7]);
+          if (i + 1 < pages) at.next<kRows>(a);
+        }
+      }
+      __syncwarp();
+    } else if (warp >= 4) {
       // ---------------- pages to bfloat16 operands ----------------
       const int dt = tid - kSoft, dw = warp - 4;
-      Walk ahead = at;
-      long long ua = u0;
-      int sent = 0;
-      auto issue = [&]() {
-        const int id = c.table[(long long)ahead.t.r * c.row_pages + ahead.t.p0 + ahead.page], b = sent & 1;
-        fetch<HD>(a, &map, id, ahead.head, smem + b * C::kBlock, &page_full[b], &bad[sent & 3]);
-        ++sent;
-        if (++ua < u1) ahead.next<kRows>(a);
-      };
-      if (dt == 0)
-        for (int n = 0; n < 2 && ua < u1; ++n) issue();
       const int g = lane & 7, t4 = lane >> 3;
-      bool ok = true;
-      int i = 0;
-      for (long long u = u0; u < u1 && ok; ++u, ++i) {
-        const int b = i & 1;
-        const uint32_t use = (i >> 1) & 1;
-        const unsigned char* blk = smem + b * C::kBlock;
-        if (!(ok = wait(&page_full[b], use))) break;
-        if (i >= 2 && !(ok = wait(&k_free[b], use ^ 1))) break;
-        // K: lane (key g of a group of 8, word t4 of a 16-byte piece): a core matrix's rows are 8 neighbouring lanes
-        unsigned char* kd = kbuf + b * C::kKBytes;
+      const int pages = (int)(u1 - u0);
+      // step i: K of page i, V of page i - 1
+      int st = 0, ring_use = 0, last_st = 0;
+      for (int i = 0; i <= pages; ++i) {
+        if (i < pages) {
+          const unsigned char* blk = smem + st * C::kBlock;
+          const bool ok = wait(&page_full[st], ring_use) && (i == 0 || wait(&s_done[(i - 1) & 1], ((i - 1) >> 1) & 1));
+          if (!__all_sync(~0u, ok)) break;
+          // lane (key g of a group of 8, word t4 of a 16-byte piece): a core matrix's rows are 8 neighbouring lanes
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            const int kg = dw * 2 + h, key = kg * 8 + g;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int kg = dw * 2 + h, key = kg * 8 + g;
-#pragma unroll
-          for (int grp = 0; grp < HD / 32; ++grp) {
-            const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(key * (HD / 2) + grp * 16) + t4 * 4);
-            const uint32_t s2 = lds16(blk + swz<HD>(kPage * HD + key * (HD / 16) + grp * 2)) * 0x10001u;
-            *reinterpret_cast<uint4*>(kd + kg * C::kKSbo + (grp * 4 + t4) * 128 + g * 16) =
-                make_uint4(value2(x, 0, s2), value2(x, 1, s2), value2(x, 2, s2), value2(x, 3, s2));
-          }
-        }
-        fence_proxy_async();
-        mbar_arrive(&k_ready[b]);
-        if (i >= 2 && !(ok = wait(&v_free[b], use ^ 1))) break;
-        // V: 8 keys x 8 channels a thread, transposed in registers
-        unsigned char* vd = vbuf + b * C::kVBytes;
-        constexpr int kBlocks = HD / 8 * (kPage / 8);
-#pragma unroll
-        for (int n = 0; n < (kBlocks + kDeq - 1) / kDeq; ++n) {
-          const int q = dt + n * kDeq;
-          if (kBlocks >= kDeq || q < kBlocks) {
-            const int ch = q % (HD / 8), j = q / (HD / 8), flip = (lane >> 4) & 1;   // half of the warp reads the odd key first
-            uint32_t x[8], sc[4];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int key = j * 8 + (e ^ flip);
-              x[e] = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(kPage * (HD / 2) + key * (HD / 2) + ch * 4));
-            }
-            uint32_t nans = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const int o = kPage * HD + kPage * (HD / 16) + (j * 8 + 2 * e) * (HD / 16) + (ch >> 2) * 2;
-              uint32_t s0 = lds16(blk + swz<HD>(o)), s1 = lds16(blk + swz<HD>(o + HD / 16));
-              // no scale of the format: 0 for the product (0 * NaN would reach rows that do not see the key), noted for those that do
-              if ((s0 & 0x7FFFu) >= kKv4BadScale) s0 = 0, nans |= 1u << (2 * e);
-              if ((s1 & 0x7FFFu) >= kKv4BadScale) s1 = 0, nans |= 2u << (2 * e);
-              sc[e] = s0 | (s1 << 16);
-            }
-            if ((ch & 3) == 0) nan_keys[(b * 8 + (ch >> 2)) * 8 + j] = (unsigned char)nans;
-            const uint32_t lo_sel = flip ? 0x1054u : 0x5410u, hi_sel = flip ? 0x3276u : 0x7632u;
-            unsigned char* to = vd + ch * C::kVSbo + j * 128;
-            uint32_t lo[4], hi[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              lo[e] = __byte_perm(x[2 * e], x[2 * e + 1], lo_sel);
-              hi[e] = __byte_perm(x[2 * e], x[2 * e + 1], hi_sel);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(value2(lo[0], k, sc[0]), value2(lo[1], k, sc[1]),
-                                                                  value2(lo[2], k, sc[2]), value2(lo[3], k, sc[3]));
-              *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(value2(hi[0], k, sc[0]), value2(hi[1], k, sc[1]),
-                                                                        value2(hi[2], k, sc[2]), value2(hi[3], k, sc[3]));
+            for (int grp = 0; grp < HD / 32; ++grp) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(key * (HD / 2) + grp * 16) + t4 * 4);
+              const uint32_t s2 = lds16(blk + swz<HD>(kPage * HD + key * (HD / 16) + grp * 2)) * 0x10001u;
+              *reinterpret_cast<uint4*>(kbuf + kg * C::kKSbo + (grp * 4 + t4) * 128 + g * 16) =
+                  make_uint4(scaled2(x, 0, s2), scaled2(x, 1, s2), scaled2(x, 2, s2), scaled2(x, 3, s2));
             }
           }
+          fence_proxy_async();
+          arrive(k_ready);
         }
-        fence_proxy_async();
-        mbar_arrive(&v_ready[b]);
-        mbar_arrive(&page_free[b]);
-        if (dt == 0 && ua < u1 && (ok = wait(&page_free[b], use))) issue();
-        __syncwarp();
+        if (i > 0) {
+          // V: 8 keys x 8 channels a thread, transposed in registers
+          const int j0 = i - 1, b = j0 & 1;
+          const unsigned char* blk = smem + last_st * C::kBlock;
+          const bool ok = j0 < 2 || wait(&pv_done[b], ((j0 - 2) >> 1) & 1);
+          if (!__all_sync(~0u, ok)) break;
+          unsigned char* vd = vbuf + b * C::kVBytes;
+          constexpr int kBlocks = HD / 8 * (kPage / 8);
+#pragma unroll 1
+          for (int n = 0; n < (kBlocks + kDeq - 1) / kDeq; ++n) {
+            const int q = dt + n * kDeq;
+            if (kBlocks >= kDeq || q < kBlocks) {
+              const int ch = q % (HD / 8), j = q / (HD / 8), flip = (lane >> 4) & 1;   // half of the warp reads the odd key first
+              uint32_t x[8], sc[4];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int key = j * 8 + (e ^ flip);
+                x[e] = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(kPage * (HD / 2) + key * (HD / 2) + ch * 4));
+              }
+              uint32_t nans = 0;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int o = kPage * HD + kPage * (HD / 16) + (j * 8 + 2 * e) * (HD / 16) + (ch >> 2) * 2;
+                uint32_t s0 = lds16(blk + swz<HD>(o)), s1 = lds16(blk + swz<HD>(o + HD / 16));
+                // no scale of the format: 0 for the product (0 * NaN would reach rows that do not see the key), noted for
+                // those that do
+                if ((s0 & 0x7FFFu) >= kKv4BadScale) s0 = 0, nans |= 1u << (2 * e);
+                if ((s1 & 0x7FFFu) >= kKv4BadScale) s1 = 0, nans |= 2u << (2 * e);
+                sc[e] = s0 | (s1 << 16);
+              }
+              if ((ch & 3) == 0) nan_keys[(b * 8 + (ch >> 2)) * 8 + j] = (unsigned char)nans;
+              const uint32_t lo_sel = flip ? 0x1054u : 0x5410u, hi_sel = flip ? 0x3276u : 0x7632u;
+              unsigned char* to = vd + ch * C::kVSbo + j * 128;
+              uint32_t lo[4], hi[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                lo[e] = __byte_perm(x[2 * e], x[2 * e + 1], lo_sel);
+                hi[e] = __byte_perm(x[2 * e], x[2 * e + 1], hi_sel);
+              }
+#pragma unroll 1
+              for (int k = 0; k < 4; ++k) {
+                *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(scaled2(lo[0], k, sc[0]), scaled2(lo[1], k, sc[1]),
+                                                                    scaled2(lo[2], k, sc[2]), scaled2(lo[3], k, sc[3]));
+                *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(scaled2(hi[0], k, sc[0]), scaled2(hi[1], k, sc[1]),
+                                                                          scaled2(hi[2], k, sc[2]), scaled2(hi[3], k, sc[3]));
+              }
+            }
+          }
+          fence_proxy_async();
+          arrive(&v_ready[b]);
+          arrive(&page_free[last_st]);
+        }
+        last_st = st;
+        if (++st == kRing) st = 0, ring_use ^= 1;
       }
     } else {
-      // ---------------- softmax: one query row a thread; the products ----------------
-      constexpr uint32_t kIdS = umma_idesc_bf16_f32(128, kPage), kIdO = umma_idesc_bf16_f32(128, HD);
-      const uint64_t kd0 = umma_desc_kmajor(smem_u32(kbuf), 128, C::kKSbo), vd0 = umma_desc_kmajor(smem_u32(vbuf), 128, C::kVSbo);
-      uint32_t qp = 0;
+      // ---------------- softmax: one query row a thread ----------------
       const uint32_t mine_at = tmem + ((uint32_t)(warp * 32) << 16);
       const float c2 = a.scale_log2;
       long long seg_first = u0 - at.page;
-      bool start = true, fresh = true;      // fresh: the segment's first page
+      bool start = true;
       float m = -INFINITY, l = 0.f;
       int hi = -1, lo = 0, all_hi = -1, all_lo = -1, f = 0;
       uint32_t nan_groups = 0;
       int i = 0;
       for (long long u = u0; u < u1; ++u, ++i) {
         const int b = i & 1;
+        const uint32_t use = (i >> 1) & 1, s_at = mine_at + C::kSCol + b * kPage;
         if (start) {
-          start = false, fresh = true;
+          start = false;
           const int f0 = at.t.qt * kRows, F = a.S * a.G;
           f = f0 + tid;
           const int s = f / a.G;
@@ -306,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           all_lo = a.window > 0 ? at.t.base + (f0 + kRows - 1) / a.G - a.window : -1;
           m = -INFINITY, l = 0.f, nan_groups = 0;
           const bf16* src = static_cast<const bf16*>(a.q) + at.t.r * a.q_row + s * a.q_tok + (at.head * a.G + (f - s * a.G)) * a.q_head;
-#pragma unroll
+#pragma unroll 1
           for (int part = 0; part < HD / 64; ++part) {
             uint32_t r[32];
 #pragma unroll
@@ -316,48 +391,50 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
               r[4 * k] = x.x, r[4 * k + 1] = x.y, r[4 * k + 2] = x.z, r[4 * k + 3] = x.w;
             }
             __syncwarp();
-            tmem_st32(mine_at + C::kQCol + part * 32, r);
-          }
-          tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(q_ready);
-        }
-        bool ok = true;
-        if (tid == 0) {
-          // Q of a new segment stored, K ready, and P V of the page before done: the scores take P's place
-          ok = (!fresh || wait(q_ready, qp)) && wait(&k_ready[b], (i >> 1) & 1) && (i == 0 || wait(pv_done, (i - 1) & 1));
-          if (ok) {
-            tc_fence_after();
-            const uint64_t kd = kd0 + (uint64_t)(b * (C::kKBytes >> 4));
+            if constexpr (C::kQTmem) {
+              tmem_st32(mine_at + part * 32, r);
+            } else {
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk)
-              umma_ts(tmem + C::kSCol, tmem + C::kQCol + kk * 8, kd + (uint64_t)(kk * 16), kIdS, kk > 0);
-            umma_commit(s_done);
-            umma_commit(&k_free[b]);
+              for (int k = 0; k < 8; ++k)
+                *reinterpret_cast<uint4*>(smem + C::kOffQ + (tid >> 3) * C::kKSbo + (part * 8 + k) * 128 + (tid & 7) * 16) =
+                    make_uint4(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]);
+            }
           }
-          qp ^= fresh;
+          if constexpr (C::kQTmem) {
+            tmem_wait_st();
+            tc_fence_before();
+          } else {
+            fence_proxy_async();
+          }
+          arrive(q_ready);
         }
-        ok = __shfl_sync(~0u, ok, 0) && wait(s_done, i & 1);
+        bool ok = wait(&s_done[b], use);
         if (!__all_sync(~0u, ok)) break;
         tc_fence_after();
-        uint32_t x[64];
-        tmem_ld32(mine_at + C::kSCol, x);
-        tmem_ld32(mine_at + C::kSCol + 32, x + 32);
-        tmem_wait_ld();
         const int key0 = (at.t.p0 + at.page) * kPage;
-        const bool all = key0 + kPage - 1 <= all_hi && key0 > all_lo && !bad[i & 3];
-        if (!all) {
-          const int from = bad[i & 3] ? kPage : lo - key0, to = hi - key0;      // keys [from, to] of the page
+        const bool all = key0 + kPage - 1 <= all_hi && key0 > all_lo && !bad[i & 7];
+        const int from = bad[i & 7] ? kPage : lo - key0, to = hi - key0;      // the row sees keys [from, to] of the page
+        float mx = -INFINITY;
+#pragma unroll 1
+        for (int h = 0; h < 64; h += 32) {
+          uint32_t x[32];
+          tmem_ld32(s_at + h, x);
+          tmem_wait_ld();
+          if (!all) hide(x, from - h, to - h);
+          float mz = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
 #pragma unroll
-          for (int k = 0; k < 64; ++k)
-            if (k < from || k > to) x[k] = 0xFF800000u;
+          for (int k = 2; k < 32; k += 4) {
+            mx = max3(mx, __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+            if (k + 2 < 32) mz = max3(mz, __uint_as_float(x[k + 2]), __uint_as_float(x[k + 3]));
+          }
+          mx = fmaxf(mx, mz);
         }
-        float mx = __uint_as_float(x[0]);
-#pragma unroll
-        for (int k = 1; k < 64; ++k) mx = fmaxf(mx, __uint_as_float(x[k]));
         const bool moves = (mx - m) * c2 > 8.f;           // also from -inf, when there is nothing to rescale
         const bool scales = moves && m != -INFINITY;
         if (__any_sync(~0u, scales)) {
+          ok = i == 0 || wait(&pv_done[b ^ 1], ((i - 1) >> 1) & 1);
+          if (!__all_sync(~0u, ok)) break;
+          tc_fence_after();
           const float fo = scales ? exp2_f((m - mx) * c2) : 1.f;
           l *= fo;
 #pragma unroll 1
@@ -374,24 +451,31 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
         if (moves) m = mx;
         const float ref = m == -INFINITY ? 0.f : -m * c2;
         float s0 = 0.f, s1 = 0.f;
+#pragma unroll 1
+        for (int h = 0; h < 64; h += 32) {
+          uint32_t x[32];
+          tmem_ld32(s_at + h, x);
+          tmem_wait_ld();
+          if (!all) hide(x, from - h, to - h);
 #pragma unroll
-        for (int k = 0; k < 32; ++k) {
-          const float p0 = exp2_f(fmaf(__uint_as_float(x[2 * k]), c2, ref)), p1 = exp2_f(fmaf(__uint_as_float(x[2 * k + 1]), c2, ref));
-          s0 += p0, s1 += p1;
-          x[k] = pack_bf16x2(p0, p1);       // probabilities in bfloat16: half a step, 2^-9 of their binade's top
+          for (int k = 0; k < 16; ++k) {
+            const float p0 = exp2_f(fmaf(__uint_as_float(x[2 * k]), c2, ref)), p1 = exp2_f(fmaf(__uint_as_float(x[2 * k + 1]), c2, ref));
+            s0 += p0, s1 += p1;
+            x[k] = pack_bf16x2(p0, p1);       // probabilities in bfloat16: half a step, 2^-9 of their binade's top
+          }
+          tmem_st16(s_at + h / 2, x);         // over scores that have been read
         }
         l += s0 + s1;
-        tmem_st32(mine_at + C::kSCol, x);
         tmem_wait_st();
         tc_fence_before();
-        ok = wait(&v_ready[b], (i >> 1) & 1);
+        ok = wait(&v_ready[b], use);
         if (!__all_sync(~0u, ok)) break;
         {
           const unsigned long long* nk = reinterpret_cast<const unsigned long long*>(nan_keys + b * 64);
           unsigned long long any = 0;
 #pragma unroll
           for (int grp = 0; grp < HD / 32; ++grp) any |= nk[grp];
-          if (any && !bad[i & 3]) {
+          if (any && !bad[i & 7]) {
             const int from = max(lo - key0, 0), to = min(hi - key0, kPage - 1);
             if (from <= to) {
               const unsigned long long sees = (~0ull << from) & (~0ull >> (63 - to));
@@ -400,25 +484,10 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
             }
           }
         }
-        mbar_arrive(p_ready);
-        if (tid == 0) {
-          ok = wait(p_ready, i & 1);     // V is ready: this thread has waited for it
-          if (ok) {
-            tc_fence_after();
-            const uint64_t vd = vd0 + (uint64_t)(b * (C::kVBytes >> 4));
-#pragma unroll
-            for (int kk = 0; kk < kPage / 16; ++kk)
-              umma_ts(tmem + C::kOCol, tmem + C::kSCol + kk * 8, vd + (uint64_t)(kk * 16), kIdO, !fresh || kk > 0);
-            umma_commit(pv_done);
-            umma_commit(&v_free[b]);
-          }
-        }
-        if (!__shfl_sync(~0u, ok, 0)) break;
-        fresh = false;
-
+        arrive(p_ready);
         const bool seg_end = at.page + 1 == at.t.n;
         if (seg_end || u + 1 == u1) {
-          ok = wait(pv_done, i & 1);
+          ok = wait(&pv_done[b], use);
           if (!__all_sync(~0u, ok)) break;
           tc_fence_after();
           const bool whole = seg_end && seg_first >= u0, there = f < a.S * a.G;
@@ -456,8 +525,8 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
   // after a wait that ran out: what was issued gets as long again to finish before its memory goes
   __syncthreads();
   if (*dead && tid == 0) {
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < kWaitLimitNs) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles) {
     }
   }
   tc_fence_before();
