@@ -31,7 +31,15 @@ __device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
   return r;
 }
 __device__ __forceinline__ uint32_t code2(uint32_t w, int k) { return as_u(__hsub2(as_b2(raw2(w, k)), as_b2(0x43084308u))); }
-__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2) { return as_u(__hmul2(as_b2(code2(w, k)), as_b2(s2))); }
+// Code times scale in one fused multiply-add, exact: (128 + u) s - 136 s = (u - 8) s.  136 s is 17 times a 4-bit number, at
+// most 255, times a power of two: a bfloat16.
+__device__ __forceinline__ uint32_t minus136(uint32_t s2) { return as_u(__hmul2(as_b2(s2), as_b2(0xC308C308u))); }
+__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2, uint32_t c2) {
+  return as_u(__hfma2(as_b2(raw2(w, k)), as_b2(s2), as_b2(c2)));
+}
+// Whether a pair of scales has one that the format does not (NaN; 2^120 or more): bits to be or'ed and tested against
+// 0x80008000.
+__device__ __forceinline__ uint32_t bad_scales(uint32_t s2) { return (s2 & 0x7FFF7FFFu) + (0x8000u - kKv4BadScale) * 0x10001u; }
 __device__ __forceinline__ void mma_c(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                       float c0, float c1, float c2, float c3) {
   asm volatile(
@@ -154,12 +162,23 @@ __device__ __forceinline__ T* out_row(const AttendArgs& a, int r, int head, int 
   return static_cast<T*>(a.out) + (((long long)r * a.S + s) * a.Hq + head * a.G + (f - s * a.G)) * HD;
 }
 
-// A bounded wait on the clock counter: reading the global timer between polls costs more than most waits here last.
+// A bounded wait on the clock counter (reading the global timer between polls costs more than most waits here last).  The
+// thread may be suspended until the phase completes, for some microseconds at a time: a polling warp takes issue slots
+// from the others.
 constexpr long long kWaitCycles = 4000000000ll;   // about 2 s
+__device__ __forceinline__ bool try_wait_long(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool wait_cycles(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (try_wait_long(bar, parity)) return true;
   const long long t0 = clock64();
-  while (!mbar_try_wait(bar, parity))
+  while (!try_wait_long(bar, parity))
     if (clock64() - t0 > kWaitCycles) return false;
   return true;
 }

@@ -11,12 +11,11 @@
 // bfloat16 128 + u.  P changes from the accumulator's layout to the B operand's with movmatrix, without shared memory.
 //
 // What bounds a decode step is instructions, not bytes: a page of 64 keys is 9 KB and the multiprocessor has some 400
-// cycles for it at the card's bandwidth.  So with one tile of 8 rows nothing is subtracted or scaled per code:
+// cycles for it at the card's bandwidth.  So with one tile of 8 rows:
 //   K   the k side of an MMA pair is one group of 32 channels, fed with 128 + u; the accumulator starts at
 //       -136 sum q of the group and its result times the key's scale is added up in float32;
-//   V   one fused multiply-add gives (128 + u) s - 128 s = u s, exact in bfloat16 (u and s have 4 bits each); the
-//       8 sum p s that u = code + 8 adds comes out of one more MMA with the scales as its A operand.
-// With more rows a code is used often enough that making it exact first costs little, and float32 results need it.
+//   V   one fused multiply-add a pair gives code times scale exactly (scaled2).
+// With more rows K is made exact the same way; float32 results need its codes exact before the product.
 //
 // A page's block is one tensor-map box of 144 rows of hd / 2 bytes, swizzled by the copy so that ldmatrix gives every
 // thread its words of the key it owns without bank conflicts.
@@ -49,7 +48,6 @@ template <int HD, int NT, typename T>
 struct Tile {
   using C = Cfg<HD, NT, T>;
   float acc[C::kMT][NT][4], m[NT][2], l[NT][2];
-  float over[C::kRaw ? 4 : 1];                    // sum p s of the thread's group (kRaw)
   float init[C::kRaw ? C::kGroups : 1][2];        // -136 sum q of a group, columns 2t and 2t + 1 (kRaw)
   int last[NT][2];                                // last visible key of the thread's columns (-1: none)
   uint4 q[C::kQReg ? NT : 1][C::kQReg ? C::kQParts : 1][C::kQReg ? C::kGroups : 1];
@@ -113,7 +111,6 @@ struct Tile {
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[i][nt][e] = 0.f;
-    if constexpr (C::kRaw) over[0] = over[1] = over[2] = over[3] = 0.f;
   }
 
   __device__ __forceinline__ uint4 query(int nt, int p, int grp, int lane) const {
@@ -190,9 +187,9 @@ struct Tile {
           uint32_t r[2][4];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t s2 = __byte_perm(ks[h][w >> 1], 0, w & 1 ? 0x3232 : 0x1010);
+            const uint32_t s2 = __byte_perm(ks[h][w >> 1], 0, w & 1 ? 0x3232 : 0x1010), c2 = minus136(s2);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) r[h][k] = scaled2(kw[h][w], k, s2);
+            for (int k = 0; k < 4; ++k) r[h][k] = scaled2(kw[h][w], k, s2, c2);
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -249,7 +246,6 @@ struct Tile {
         for (int i = 0; i < C::kMT; ++i)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[i][nt][e] *= f[e & 1];
-        if constexpr (C::kRaw) over[0] *= f[0], over[1] *= f[1];
       }
 #pragma unroll
       for (int i = 0; i < kTiles; ++i)
@@ -287,28 +283,15 @@ struct Tile {
         const int o = v_scale[h] + k16 * (HD / 16);
         s2[h] = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
       }
-      uint32_t c2[2];
-      if constexpr (C::kRaw) {
-        c2[0] = as_u(__hmul2(as_b2(s2[0]), as_b2(0xC300C300u)));   // -128 s
-        c2[1] = as_u(__hmul2(as_b2(s2[1]), as_b2(0xC300C300u)));
-        mma_bf16(over, s2[0], 0u, s2[1], 0u, pf[i][0][0][0], pf[i][0][0][1]);
-      }
+      const uint32_t c2[2] = {minus136(s2[0]), minus136(s2[1])};
 #pragma unroll
       for (int wd = 0; wd < C::kVWords; ++wd) {
         const uint32_t lo0 = __byte_perm(vw[0][wd], vw[1][wd], 0x5410), hi0 = __byte_perm(vw[0][wd], vw[1][wd], 0x7632);
         const uint32_t lo1 = __byte_perm(vw[2][wd], vw[3][wd], 0x5410), hi1 = __byte_perm(vw[2][wd], vw[3][wd], 0x7632);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint32_t a0, a1, a2, a3;
-          if constexpr (C::kRaw) {
-            a0 = as_u(__hfma2(as_b2(raw2(lo0, k)), as_b2(s2[0]), as_b2(c2[0])));
-            a1 = as_u(__hfma2(as_b2(raw2(hi0, k)), as_b2(s2[0]), as_b2(c2[0])));
-            a2 = as_u(__hfma2(as_b2(raw2(lo1, k)), as_b2(s2[1]), as_b2(c2[1])));
-            a3 = as_u(__hfma2(as_b2(raw2(hi1, k)), as_b2(s2[1]), as_b2(c2[1])));
-          } else {
-            a0 = scaled2(lo0, k, s2[0]), a1 = scaled2(hi0, k, s2[0]);
-            a2 = scaled2(lo1, k, s2[1]), a3 = scaled2(hi1, k, s2[1]);
-          }
+          const uint32_t a0 = scaled2(lo0, k, s2[0], c2[0]), a1 = scaled2(hi0, k, s2[0], c2[0]);
+          const uint32_t a2 = scaled2(lo1, k, s2[1], c2[1]), a3 = scaled2(hi1, k, s2[1], c2[1]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -343,7 +326,7 @@ struct Tile {
           w[0] = *x;
         }
 #pragma unroll
-        for (int j = 0; j < kEach / 4; ++j) top |= (w[j] & 0x7FFF7FFFu) + (0x8000u - kKv4BadScale) * 0x10001u;   // carries into the sign from there on
+        for (int j = 0; j < kEach / 4; ++j) top |= bad_scales(w[j]);
       }
     }
     if (!__any_sync(~0u, top & 0x80008000u)) return;
@@ -379,9 +362,7 @@ struct Tile {
     return x + __shfl_xor_sync(~0u, x, 16);
   }
   __device__ __forceinline__ float value(int wd, int k, int nt, int e) const {   // channel k of word wd
-    float x = acc[wd * 4 + (k & 3)][nt][(k >> 2) * 2 + e];
-    if constexpr (C::kRaw) x = fmaf(-8.f, over[e], x);
-    return x;
+    return acc[wd * 4 + (k & 3)][nt][(k >> 2) * 2 + e];
   }
 };
 

@@ -92,6 +92,23 @@ __device__ __forceinline__ void hide(uint32_t* x, int from, int to) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two floats at a time.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -201,9 +218,9 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
     }
     // every wait is bounded; once one has run out all roles leave
     auto wait = [&](uint64_t* b, uint32_t parity) {
-      if (mbar_try_wait(b, parity)) return true;
+      if (try_wait_long(b, parity)) return true;
       const long long t0 = clock64();
-      while (!mbar_try_wait(b, parity)) {
+      while (!try_wait_long(b, parity)) {
         if (*dead) return false;
         if (clock64() - t0 > kWaitCycles) {
           *dead = 1;
@@ -290,12 +307,25 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             const int kg = dw * 2 + h, key = kg * 8 + g;
+            uint32_t ks[HD / 64];        // the key's scales, two groups a register
+            const unsigned char* sp = blk + swz<HD>(kPage * HD + key * (HD / 16));
+            if constexpr (HD == 64) {
+              ks[0] = *reinterpret_cast<const uint32_t*>(sp);
+            } else if constexpr (HD == 128) {
+              const uint2 v2 = *reinterpret_cast<const uint2*>(sp);
+              ks[0] = v2.x, ks[1] = v2.y;
+            } else {
+              const uint4 v4 = *reinterpret_cast<const uint4*>(sp);
+              ks[0] = v4.x, ks[1] = v4.y, ks[2] = v4.z, ks[3] = v4.w;
+            }
+            const int codes = swz<HD>(key * (HD / 2)) + t4 * 4;       // the swizzle exchanges whole pieces: group by xor
+            unsigned char* to = kbuf + kg * C::kKSbo + t4 * 128 + g * 16;
 #pragma unroll
             for (int grp = 0; grp < HD / 32; ++grp) {
-              const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(key * (HD / 2) + grp * 16) + t4 * 4);
-              const uint32_t s2 = lds16(blk + swz<HD>(kPage * HD + key * (HD / 16) + grp * 2)) * 0x10001u;
-              *reinterpret_cast<uint4*>(kbuf + kg * C::kKSbo + (grp * 4 + t4) * 128 + g * 16) =
-                  make_uint4(scaled2(x, 0, s2), scaled2(x, 1, s2), scaled2(x, 2, s2), scaled2(x, 3, s2));
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + (codes ^ (grp * 16)));
+              const uint32_t s2 = __byte_perm(ks[grp >> 1], 0, grp & 1 ? 0x3232 : 0x1010), c2 = minus136(s2);
+              *reinterpret_cast<uint4*>(to + grp * 512) =
+                  make_uint4(scaled2(x, 0, s2, c2), scaled2(x, 1, s2, c2), scaled2(x, 2, s2, c2), scaled2(x, 3, s2, c2));
             }
           }
           fence_proxy_async();
@@ -314,22 +344,31 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
             const int q = dt + n * kDeq;
             if (kBlocks >= kDeq || q < kBlocks) {
               const int ch = q % (HD / 8), j = q / (HD / 8), flip = (lane >> 4) & 1;   // half of the warp reads the odd key first
-              uint32_t x[8], sc[4];
+              uint32_t x[8], sc[4], cc[4];
+              // a word of a key, keys of 8 rows: the swizzle is that of the row alone
+              const unsigned char* vp = blk + kPage * (HD / 2) + j * 8 * (HD / 2);
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
-                const int key = j * 8 + (e ^ flip);
-                x[e] = *reinterpret_cast<const uint32_t*>(blk + swz<HD>(kPage * (HD / 2) + key * (HD / 2) + ch * 4));
+                const int row = e ^ flip;
+                x[e] = *reinterpret_cast<const uint32_t*>(vp + swz<HD>(row * (HD / 2) + ch * 4));
               }
-              uint32_t nans = 0;
+              uint32_t worst = 0;
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const int o = kPage * HD + kPage * (HD / 16) + (j * 8 + 2 * e) * (HD / 16) + (ch >> 2) * 2;
-                uint32_t s0 = lds16(blk + swz<HD>(o)), s1 = lds16(blk + swz<HD>(o + HD / 16));
+                sc[e] = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
+                worst |= bad_scales(sc[e]);
+              }
+              uint32_t nans = 0;
+              if (worst & 0x80008000u) {
                 // no scale of the format: 0 for the product (0 * NaN would reach rows that do not see the key), noted for
                 // those that do
-                if ((s0 & 0x7FFFu) >= kKv4BadScale) s0 = 0, nans |= 1u << (2 * e);
-                if ((s1 & 0x7FFFu) >= kKv4BadScale) s1 = 0, nans |= 2u << (2 * e);
-                sc[e] = s0 | (s1 << 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t bad2 = bad_scales(sc[e]);
+                  if (bad2 & 0x8000u) sc[e] &= 0xFFFF0000u, nans |= 1u << (2 * e);
+                  if (bad2 & 0x80000000u) sc[e] &= 0x0000FFFFu, nans |= 2u << (2 * e);
+                }
               }
               if ((ch & 3) == 0) nan_keys[(b * 8 + (ch >> 2)) * 8 + j] = (unsigned char)nans;
               const uint32_t lo_sel = flip ? 0x1054u : 0x5410u, hi_sel = flip ? 0x3276u : 0x7632u;
@@ -337,15 +376,20 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
               uint32_t lo[4], hi[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
+                cc[e] = minus136(sc[e]);
                 lo[e] = __byte_perm(x[2 * e], x[2 * e + 1], lo_sel);
                 hi[e] = __byte_perm(x[2 * e], x[2 * e + 1], hi_sel);
               }
 #pragma unroll 1
               for (int k = 0; k < 4; ++k) {
-                *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(scaled2(lo[0], k, sc[0]), scaled2(lo[1], k, sc[1]),
-                                                                    scaled2(lo[2], k, sc[2]), scaled2(lo[3], k, sc[3]));
-                *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(scaled2(hi[0], k, sc[0]), scaled2(hi[1], k, sc[1]),
-                                                                          scaled2(hi[2], k, sc[2]), scaled2(hi[3], k, sc[3]));
+                uint32_t r[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  r[e] = scaled2(lo[e], 0, sc[e], cc[e]), r[4 + e] = scaled2(hi[e], 0, sc[e], cc[e]);
+                  lo[e] >>= 4, hi[e] >>= 4;
+                }
+                *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(r[0], r[1], r[2], r[3]);
+                *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(r[4], r[5], r[6], r[7]);
               }
             }
           }
@@ -377,7 +421,8 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           const bool live = f < F && s < at.t.cnt;
           hi = live ? at.t.base + s : -1;
           lo = live && a.window > 0 ? max(0, hi - a.window + 1) : 0;
-          all_hi = f0 + kRows <= at.t.cnt * a.G ? at.t.base + f0 / a.G : -1;
+          // what rows that are not there make of a page does not matter: their results are zeros
+          all_hi = at.t.base + f0 / a.G;
           all_lo = a.window > 0 ? at.t.base + (f0 + kRows - 1) / a.G - a.window : -1;
           m = -INFINITY, l = 0.f, nan_groups = 0;
           const bf16* src = static_cast<const bf16*>(a.q) + at.t.r * a.q_row + s * a.q_tok + (at.head * a.G + (f - s * a.G)) * a.q_head;
@@ -450,7 +495,8 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
         }
         if (moves) m = mx;
         const float ref = m == -INFINITY ? 0.f : -m * c2;
-        float s0 = 0.f, s1 = 0.f;
+        uint64_t sum2 = pair(0.f, 0.f);
+        const uint64_t c22 = pair(c2, c2), ref2 = pair(ref, ref);
 #pragma unroll 1
         for (int h = 0; h < 64; h += 32) {
           uint32_t x[32];
@@ -459,12 +505,16 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           if (!all) hide(x, from - h, to - h);
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
-            const float p0 = exp2_f(fmaf(__uint_as_float(x[2 * k]), c2, ref)), p1 = exp2_f(fmaf(__uint_as_float(x[2 * k + 1]), c2, ref));
-            s0 += p0, s1 += p1;
+            float p0, p1;
+            unpair(fma2(pair(__uint_as_float(x[2 * k]), __uint_as_float(x[2 * k + 1])), c22, ref2), p0, p1);
+            p0 = exp2_f(p0), p1 = exp2_f(p1);
+            sum2 = add2(sum2, pair(p0, p1));
             x[k] = pack_bf16x2(p0, p1);       // probabilities in bfloat16: half a step, 2^-9 of their binade's top
           }
           tmem_st16(s_at + h / 2, x);         // over scores that have been read
         }
+        float s0, s1;
+        unpair(sum2, s0, s1);
         l += s0 + s1;
         tmem_wait_st();
         tc_fence_before();
@@ -492,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           tc_fence_after();
           const bool whole = seg_end && seg_first >= u0, there = f < a.S * a.G;
           float* slot = a.part + (w * 2 + (seg_first >= u0 ? 1 : 0)) * (long long)(kRows * (HD + 2));
+          if (hi < 0) m = -INFINITY, l = 0.f;               // padding
           const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
           bf16* o = there ? out_row<HD, bf16>(a, at.t.r, at.head, f) : nullptr;
 #pragma unroll 1
