@@ -103,11 +103,15 @@ struct Walk {
   }
 };
 
-// First unit of warp w's run.
-__device__ __forceinline__ long long run_start(long long w, long long units, long long warps) { return w * units / warps; }
-// Warp whose run holds unit u.
-__device__ __forceinline__ long long run_of(long long u, long long units, long long warps) {
-  return ((u + 1) * warps - 1) / units;
+// Quotient of two non-negative numbers; most fit 32 bits, where the division is a quarter of the work.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  return (unsigned long long)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+// First unit of run w.
+__device__ __forceinline__ long long run_start(long long w, long long units, long long runs) { return divide(w * units, runs); }
+// The run that holds unit u.
+__device__ __forceinline__ long long run_of(long long u, long long units, long long runs) {
+  return divide((u + 1) * runs - 1, units);
 }
 
 // ---- loading queries ----------------------------------------------------------------------------------------

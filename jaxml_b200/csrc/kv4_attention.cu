@@ -53,7 +53,8 @@ struct Tile {
   uint4 q[C::kQReg ? NT : 1][C::kQReg ? C::kQParts : 1][C::kQReg ? C::kGroups : 1];
   uint4* qs;                                      // the fragments in shared memory otherwise
   int all_hi, all_lo;                             // pages within (all_lo, all_hi] are seen by every row of the tile
-  int k_code, k_scale, v_code[2], v_scale[2];     // the thread's places in a block (swizzled)
+  int k_code, v_code[2];                          // the thread's places in a block's codes (swizzled)
+  int k_scale, v_scale;                           // and among the scales of 8 keys (not yet)
 
   __device__ __forceinline__ void begin(const AttendArgs& a, const Item& t, int head, int lane, bool store = true) {
     const int g = lane >> 2, tq = lane & 3, f0 = t.qt * C::kRows, F = a.S * a.G;
@@ -64,9 +65,8 @@ struct Tile {
                       : swz<HD>((lane & 7) * C::kRowBytes + (lane >> 3) * 16);
     v_code[0] = swz<HD>(2 * tq * C::kRowBytes + g * (C::kVWords * 4)) + kPage * C::kRowBytes;
     v_code[1] = swz<HD>((2 * tq + 1) * C::kRowBytes + g * (C::kVWords * 4)) + kPage * C::kRowBytes;
-    k_scale = kPage * HD + g * (HD / 16);
-    v_scale[0] = kPage * HD + kPage * (HD / 16) + 2 * tq * (HD / 16) + (HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g) * 2;
-    v_scale[1] = v_scale[0] + 8 * (HD / 16);
+    k_scale = g * (HD / 16);
+    v_scale = 2 * tq * (HD / 16) + (HD == 64 ? g >> 2 : HD == 128 ? g >> 1 : g) * 2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -118,11 +118,17 @@ struct Tile {
     else return qs[((nt * C::kQParts + p) * C::kGroups + grp) * 32 + lane];
   }
 
+  // Place in a scale area (which begins on a whole swizzle period) of byte `o` of the scales of the 8 keys from `key` on.
+  static __device__ __forceinline__ int scale_at(int key, int o) {
+    const int first = key * (HD / 16);
+    return (first & ~127) + (((first & 127) + o) ^ (((first >> 7) & (HD / 32 - 1)) << 4));
+  }
+
   // Keys [kb, kb + KT) of the page in `blk` (shared memory, swizzled), whose first key is key0.  all: every row sees them.
   template <int KT>
   __device__ __forceinline__ void keys(const AttendArgs& a, const unsigned char* blk, int kb, int key0, bool all, int lane) {
     constexpr int kTiles = KT / 16;
-    const int g = lane >> 2, t = lane & 3;
+    const int g = lane >> 2;
     float sc[kTiles][NT][4];
     const uint32_t base = smem_u32(blk);
 #pragma unroll
@@ -143,7 +149,8 @@ struct Tile {
       uint32_t ks[2][C::kGroups / 2];   // scales of the two keys, two groups a register
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const unsigned char* p = blk + swz<HD>(k_scale + (k16 + h * 8) * (HD / 16));
+        // keys 16 i + 8 h + g: the line, and with it the swizzle, is known but for g's share of it
+        const unsigned char* p = blk + kPage * HD + scale_at(k16 + h * 8, k_scale);
         if constexpr (HD == 64) {
           ks[h][0] = *reinterpret_cast<const uint32_t*>(p);
         } else if constexpr (HD == 128) {
@@ -280,8 +287,8 @@ struct Tile {
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // the thread's channels are of one group
-        const int o = v_scale[h] + k16 * (HD / 16);
-        s2[h] = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
+        const unsigned char* p = blk + kPage * HD + kPage * (HD / 16);
+        s2[h] = lds16(p + scale_at(k16 + h * 8, v_scale)) | (lds16(p + scale_at(k16 + h * 8, v_scale + HD / 16)) << 16);
       }
       const uint32_t c2[2] = {minus136(s2[0]), minus136(s2[1])};
 #pragma unroll
@@ -541,64 +548,83 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
   }
 }
 
-// Joins what several runs hold of one (row, tile, head).  A CTA takes kJoinWarps / kEach query rows, kEach warps each: one
-// where a row has a few parts, all of them where one row may be spread over the whole grid.  Rows without a visible key
-// are zero.
-constexpr int kJoinWarps = 8;
-template <int HD, typename T, int kEach>
+// Joins what several runs hold of one (row, tile, head).  Where a row has a few parts a warp takes kMany query rows, their
+// loads under way together; where one row may be spread over the whole grid all warps of a CTA share one.  Rows without a
+// visible key are zero.
+constexpr int kJoinWarps = 8, kMany = 4;
+template <int HD, typename T, bool kSpread>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendArgs a, int rows) {
+  constexpr int kR = kSpread ? 1 : kMany, kV = HD / 32;
   pdl_wait();
-  __shared__ float sh[kEach > 1 ? kJoinWarps : 1][HD + 2];
+  __shared__ float sh[kSpread ? kJoinWarps : 1][HD + 2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, Hkv = a.c.num_kv_heads;
-  const int item = blockIdx.x / Hkv, head = blockIdx.x - item * Hkv, j = blockIdx.y * (kJoinWarps / kEach) + warp / kEach;
-  const long long units = a.total[0], warps = a.total[1];
+  const int item = blockIdx.x / Hkv, head = blockIdx.x - item * Hkv;
+  const int j0 = kSpread ? blockIdx.y : (blockIdx.y * kJoinWarps + warp) * kR;
+  const long long units = a.total[0], runs = a.total[1];
   const long long first = a.item_first[item], end = item + 1 < a.items ? a.item_first[item + 1] : units;
-  const long long n = (end - first) / Hkv, u0 = first + head * n, u1 = u0 + n;
-  const long long w0 = n ? run_of(u0, units, warps) : 0, w1 = n ? run_of(u1 - 1, units, warps) : 0;
+  const long long n = divide(end - first, Hkv), u0 = first + head * n, u1 = u0 + n;
+  const long long w0 = n ? run_of(u0, units, runs) : 0, w1 = n ? run_of(u1 - 1, units, runs) : 0;
   if (n && w0 == w1) return;
-  const int r = item / a.tiles, qt = item - r * a.tiles, f = qt * rows + j;
-  const bool live = j < rows && f < a.S * a.G;
-  if (kEach == 1 && !live) return;
+  const int r = item / a.tiles, qt = item - r * a.tiles, f0 = qt * rows + j0;
+  const int live = min(kR, min(rows - j0, a.S * a.G - f0));
+  if (!kSpread && live <= 0) return;
   const long long slot_floats = (long long)rows * (HD + 2);
-  constexpr int kV = HD / 32;
-  float m = -INFINITY, l = 0.f, o[kV];
+  float m[kR], l[kR], o[kR][kV];
 #pragma unroll
-  for (int i = 0; i < kV; ++i) o[i] = 0.f;
-  for (long long w = w0 + warp % kEach; live && n && w <= w1; w += kEach) {
-    // the run that the segment begins in holds it in its second slot
-    const float* slot = a.part + (w * 2 + (run_start(w, units, warps) <= u0 ? 1 : 0)) * slot_floats;
-    const float mw = slot[rows * HD + 2 * j], lw = slot[rows * HD + 2 * j + 1];
-    const float mn = fmaxf(m, mw), use = mn == -INFINITY ? 0.f : mn;
-    const float fo = exp2_f(m - use), fw = exp2_f(mw - use);
-    m = mn;
-    l = l * fo + lw * fw;
+  for (int q = 0; q < kR; ++q) {
+    m[q] = -INFINITY, l[q] = 0.f;
 #pragma unroll
-    for (int i = 0; i < kV; ++i) o[i] = o[i] * fo + slot[j * HD + i * 32 + lane] * fw;
+    for (int i = 0; i < kV; ++i) o[q][i] = 0.f;
   }
-  if constexpr (kEach > 1) {
+  for (long long w = w0 + (kSpread ? warp : 0); n && live > 0 && w <= w1; w += kSpread ? kJoinWarps : 1) {
+    // the run that the segment begins in holds it in its second slot
+    const float* slot = a.part + (w * 2 + (run_start(w, units, runs) <= u0 ? 1 : 0)) * slot_floats;
+    float mw[kR], lw[kR], ow[kR][kV];
 #pragma unroll
-    for (int i = 0; i < kV; ++i) sh[warp][i * 32 + lane] = o[i];
-    if (lane == 0) sh[warp][HD] = m, sh[warp][HD + 1] = l;
-    __syncthreads();
-    if (warp || !live) return;
-    m = -INFINITY, l = 0.f;
+    for (int q = 0; q < kR; ++q) {
+      const int j = j0 + min(q, live - 1);
+      mw[q] = slot[rows * HD + 2 * j], lw[q] = slot[rows * HD + 2 * j + 1];
 #pragma unroll
-    for (int w = 0; w < kEach; ++w) m = fmaxf(m, sh[w][HD]);
+      for (int i = 0; i < kV; ++i) ow[q][i] = slot[j * HD + lane * kV + i];
+    }
 #pragma unroll
-    for (int i = 0; i < kV; ++i) o[i] = 0.f;
-    const float use = m == -INFINITY ? 0.f : m;
+    for (int q = 0; q < kR; ++q) {
+      const float mn = fmaxf(m[q], mw[q]), use = mn == -INFINITY ? 0.f : mn;
+      const float fo = exp2_f(m[q] - use), fw = exp2_f(mw[q] - use);
+      m[q] = mn;
+      l[q] = l[q] * fo + lw[q] * fw;
 #pragma unroll
-    for (int w = 0; w < kEach; ++w) {
-      const float fw = exp2_f(sh[w][HD] - use);
-      l += sh[w][HD + 1] * fw;
-#pragma unroll
-      for (int i = 0; i < kV; ++i) o[i] += sh[w][i * 32 + lane] * fw;
+      for (int i = 0; i < kV; ++i) o[q][i] = o[q][i] * fo + ow[q][i] * fw;
     }
   }
-  T* out = out_row<HD, T>(a, r, head, f);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  if constexpr (kSpread) {
 #pragma unroll
-  for (int i = 0; i < kV; ++i) out[i * 32 + lane] = from_f<T>(o[i] * inv);
+    for (int i = 0; i < kV; ++i) sh[warp][lane * kV + i] = o[0][i];
+    if (lane == 0) sh[warp][HD] = m[0], sh[warp][HD + 1] = l[0];
+    __syncthreads();
+    if (warp || live <= 0) return;
+    m[0] = -INFINITY, l[0] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) m[0] = fmaxf(m[0], sh[w][HD]);
+#pragma unroll
+    for (int i = 0; i < kV; ++i) o[0][i] = 0.f;
+    const float use = m[0] == -INFINITY ? 0.f : m[0];
+#pragma unroll
+    for (int w = 0; w < kJoinWarps; ++w) {
+      const float fw = exp2_f(sh[w][HD] - use);
+      l[0] += sh[w][HD + 1] * fw;
+#pragma unroll
+      for (int i = 0; i < kV; ++i) o[0][i] += sh[w][lane * kV + i] * fw;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kR; ++q) {
+    if (q >= live) continue;
+    T* out = out_row<HD, T>(a, r, head, f0 + q) + lane * kV;
+    const float inv = l[q] == 0.f ? 0.f : 1.f / l[q];
+#pragma unroll
+    for (int i = 0; i < kV; ++i) out[i] = from_f<T>(o[q][i] * inv);
+  }
 }
 
 // ---- one CTA for every (row, query tile, KV head) -----------------------------------------------------------------
@@ -806,15 +832,16 @@ int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
   const int there = a.tiles > 1 || a.S * a.G >= rows ? rows : a.S * a.G;
   const bool few = runs <= 4 * segments;    // some four parts a segment, if they are alike
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)segments, (unsigned)(few ? (there + kJoinWarps - 1) / kJoinWarps : there));
+  const int each = few ? kJoinWarps * kMany : 1;
+  cfg.gridDim = dim3((unsigned)segments, (unsigned)((there + each - 1) / each));
   cfg.blockDim = dim3(kJoinWarps * 32);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return (few ? cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, 1>, a, rows)
-              : cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, kJoinWarps>, a, rows)) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return (few ? cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, false>, a, rows)
+              : cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, true>, a, rows)) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
 template <int HD, int NT, typename T>

@@ -41,44 +41,83 @@ struct AppendArgs {
   long long row[2], tok[2], head[2];   // element strides
 };
 
+// The nibbles of 8 values of a group.  bfloat16 values: the quotient by a product with 1 / s and one step of correction,
+// which is the correctly rounded one where that matters: a quotient that is a half step is represented exactly, so the
+// correction lands on it, and any other is off a half step by at least 2^-9 of itself, far beyond what the step leaves.
+// float32 values, and scales near the ends of the range, take the division.
 template <typename T>
-__global__ void kv4_append_kernel(const AppendArgs a) {
-  const jx_kv4_cache& c = a.c;
-  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per;
-  for (long long t = blockIdx.x; t < (long long)c.num_rows * a.S; t += gridDim.x) {
-    const int r = (int)(t / a.S), i = (int)(t - (long long)r * a.S);
-    const int cnt = c.counts[r];
-    if (i == 0 && cnt > a.S && threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
-    if (i >= cnt) continue;
-    const int pos = c.lengths[r] - cnt + i;
-    int page = -1;
-    if (pos >= 0 && pos < c.row_pages * kPage) page = c.table[(long long)r * c.row_pages + pos / kPage];
-    if (page < 0 || page >= c.num_pages) {
-      if (threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
-      continue;
+__device__ __forceinline__ uint32_t nibbles(const float* x, float s) {
+  uint32_t w = 0;
+  if (sizeof(T) == 2 && s > 1e-30f && s < 1e30f) {
+    const float inv = __frcp_rn(s);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float q0 = x[j] * inv, q = fmaf(fmaf(-q0, s, x[j]), inv, q0);
+      // 1.5 * 2^23 + q rounds to an integer (ties to even) in the lower bits; + 8 makes the nibble.  |q| <= 7.44: no clamp
+      w |= (__float_as_uint(q + 12582920.f) & 15u) << (4 * j);
     }
-    const int slot = pos % kPage;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w |= kv4_nibble(x[j], s) << (4 * j);
+  }
+  return w;
+}
+
+// Each CTA takes kTok neighbouring tokens of a row: their loads are under way together.
+template <typename T, int kTok>
+__global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
+  const jx_kv4_cache& c = a.c;
+  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per, tiles = (a.S + kTok - 1) / kTok;
+  for (long long t = blockIdx.x; t < (long long)c.num_rows * tiles; t += gridDim.x) {
+    const int r = (int)(t / tiles), i0 = (int)(t - (long long)r * tiles) * kTok;
+    const int cnt = c.counts[r];
+    if (i0 == 0 && cnt > a.S && threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
+    if (i0 >= cnt) continue;
+    const int pos0 = c.lengths[r] - cnt + i0;
+    int page[kTok];
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      const int pos = pos0 + j;
+      page[j] = -1;
+      if (i0 + j < min(cnt, a.S)) {
+        if (pos >= 0 && pos < c.row_pages * kPage) page[j] = c.table[(long long)r * c.row_pages + pos / kPage];
+        if (page[j] < 0 || page[j] >= c.num_pages) {
+          page[j] = -1;
+          if (threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
+        }
+      }
+    }
     for (int it = threadIdx.x; it < items; it += blockDim.x) {   // items and blockDim are multiples of 4
       const int which = it >= items / 2, rest = it - which * (items / 2), head = rest / per, ch = rest % per;
-      const T* p = static_cast<const T*>(a.src[which]) + r * a.row[which] + i * a.tok[which] +
+      const T* p = static_cast<const T*>(a.src[which]) + r * a.row[which] + i0 * a.tok[which] +
                    head * a.head[which] + ch * 8;
-      float x[8];
-      load8<T>(p, a.vec, x);
-      uint32_t m = 0;
+      float x[kTok][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(x[j]) & 0x7FFFFFFFu);
-      const unsigned group = 0xFu << (threadIdx.x & 28);
-      m = max(m, __shfl_xor_sync(group, m, 1));
-      m = max(m, __shfl_xor_sync(group, m, 2));
-      const float s = kv4_scale(m);
-      uint32_t w = 0;
+      for (int j = 0; j < kTok; ++j) {
+        if (page[j] >= 0) {
+          load8<T>(p + j * a.tok[which], a.vec, x[j]);
+        } else {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w |= kv4_nibble(x[j], s) << (4 * j);
-      unsigned char* blk = kv4_block(c, a.layer, page, head);
-      *reinterpret_cast<uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4) = w;
-      if ((ch & 3) == 0)
-        *reinterpret_cast<bf16*>(blk + kv4_scale_offset(hd, which) + (slot * (hd / 32) + (ch >> 2)) * 2) =
-            __float2bfloat16_rn(s);
+          for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[j][e]) & 0x7FFFFFFFu);
+        const unsigned group = 0xFu << (threadIdx.x & 28);
+        m = max(m, __shfl_xor_sync(group, m, 1));
+        m = max(m, __shfl_xor_sync(group, m, 2));
+        if (page[j] < 0) continue;
+        const float s = kv4_scale(m);
+        const int slot = (pos0 + j) % kPage;
+        unsigned char* blk = kv4_block(c, a.layer, page[j], head);
+        *reinterpret_cast<uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4) = nibbles<T>(x[j], s);
+        if ((ch & 3) == 0)
+          *reinterpret_cast<bf16*>(blk + kv4_scale_offset(hd, which) + (slot * (hd / 32) + (ch >> 2)) * 2) =
+              __float2bfloat16_rn(s);
+      }
     }
   }
 }
@@ -99,34 +138,48 @@ __device__ __forceinline__ void store8<float>(float* p, const float* x) {
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-template <typename T>
-__global__ void kv4_read_kernel(const jx_kv4_cache c, int layer, const int* start, int start_add, int n, T* k, T* v) {
-  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per;
-  for (long long t = blockIdx.x; t < (long long)c.num_rows * n; t += gridDim.x) {
-    const int r = (int)(t / n), i = (int)(t - (long long)r * n);
-    const long long pos = (long long)(start ? start[r] : 0) + start_add + i;
-    int page = -1;
-    if (pos >= 0 && pos < min(c.lengths[r], c.row_pages * kPage)) {
-      page = c.table[(long long)r * c.row_pages + pos / kPage];
-      if (page < 0 || page >= c.num_pages) {
-        page = -1;
-        if (threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
+template <typename T, int kTok>
+__global__ void __launch_bounds__(256) kv4_read_kernel(const jx_kv4_cache c, int layer, const int* start, int start_add, int n,
+                                                       T* k, T* v) {
+  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per, tiles = (n + kTok - 1) / kTok;
+  for (long long t = blockIdx.x; t < (long long)c.num_rows * tiles; t += gridDim.x) {
+    const int r = (int)(t / tiles), i0 = (int)(t - (long long)r * tiles) * kTok;
+    const long long pos0 = (long long)(start ? start[r] : 0) + start_add + i0;
+    const int len = min(c.lengths[r], c.row_pages * kPage);
+    int page[kTok];
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      page[j] = -1;
+      if (pos0 + j >= 0 && pos0 + j < len) {
+        page[j] = c.table[(long long)r * c.row_pages + (pos0 + j) / kPage];
+        if (page[j] < 0 || page[j] >= c.num_pages) {
+          page[j] = -1;
+          if (threadIdx.x == 0 && i0 + j < n) set_status(c.status, JX_ERR_RANGE);
+        }
       }
     }
-    const int slot = (int)(pos & (kPage - 1));
     for (int it = threadIdx.x; it < items; it += blockDim.x) {
       const int which = it >= items / 2, rest = it - which * (items / 2), head = rest / per, ch = rest % per;
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (page >= 0) {
-        const unsigned char* blk = kv4_block(c, layer, page, head);
-        const uint32_t w =
-            *reinterpret_cast<const uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4);
-        const float s = to_f(*reinterpret_cast<const bf16*>(blk + kv4_scale_offset(hd, which) +
-                                                            (slot * (hd / 32) + (ch >> 2)) * 2));
+      uint32_t w[kTok];
+      float s[kTok];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = (float)((int)((w >> (4 * j)) & 15u) - 8) * s;
+      for (int j = 0; j < kTok; ++j) {
+        w[j] = 0x88888888u, s[j] = 0.f;
+        if (page[j] >= 0) {
+          const unsigned char* blk = kv4_block(c, layer, page[j], head);
+          const int slot = (int)((pos0 + j) & (kPage - 1));
+          w[j] = *reinterpret_cast<const uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4);
+          s[j] = to_f(*reinterpret_cast<const bf16*>(blk + kv4_scale_offset(hd, which) + (slot * (hd / 32) + (ch >> 2)) * 2));
+        }
       }
-      store8<T>((which ? v : k) + (t * c.num_kv_heads + head) * hd + ch * 8, x);
+#pragma unroll
+      for (int j = 0; j < kTok; ++j) {
+        if (i0 + j >= n) continue;
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)((int)((w[j] >> (4 * e)) & 15u) - 8) * s[j];
+        store8<T>((which ? v : k) + ((((long long)r * n + i0 + j) * c.num_kv_heads + head) * hd + ch * 8), x);
+      }
     }
   }
 }
@@ -419,10 +472,16 @@ int run_kv4_append(const jx_kv4_cache& c, int layer, int S, const void* k, const
     if (((uintptr_t)a.src[i] & 15) || a.row[i] % unit || a.tok[i] % unit || a.head[i] % unit) a.vec = 0;
   const int items = 2 * c.num_kv_heads * (c.head_dim / 8);
   const int threads = items < 256 ? (items + 31) / 32 * 32 : 256;
-  const long long tokens = (long long)c.num_rows * S;
-  const int grid = (int)(tokens < 148 * 64 ? tokens : 148 * 64);
-  if (dtype == JX_BF16) kv4_append_kernel<bf16><<<grid, threads, 0, s>>>(a);
-  else kv4_append_kernel<float><<<grid, threads, 0, s>>>(a);
+  const int tok = S >= 4 ? 4 : 1;
+  const long long tiles = (long long)c.num_rows * ((S + tok - 1) / tok);
+  const int grid = (int)(tiles < 148 * 64 ? tiles : 148 * 64);
+  if (dtype == JX_BF16) {
+    if (tok == 4) kv4_append_kernel<bf16, 4><<<grid, threads, 0, s>>>(a);
+    else kv4_append_kernel<bf16, 1><<<grid, threads, 0, s>>>(a);
+  } else {
+    if (tok == 4) kv4_append_kernel<float, 4><<<grid, threads, 0, s>>>(a);
+    else kv4_append_kernel<float, 1><<<grid, threads, 0, s>>>(a);
+  }
   return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
@@ -430,12 +489,16 @@ int run_kv4_read(const jx_kv4_cache& c, int layer, const int* start, int start_a
                  cudaStream_t s) {
   const int items = 2 * c.num_kv_heads * (c.head_dim / 8);
   const int threads = items < 256 ? (items + 31) / 32 * 32 : 256;
-  const long long tokens = (long long)c.num_rows * n;
-  const int grid = (int)(tokens < 148 * 64 ? tokens : 148 * 64);
-  if (dtype == JX_BF16)
-    kv4_read_kernel<bf16><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (bf16*)k, (bf16*)v);
-  else
-    kv4_read_kernel<float><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (float*)k, (float*)v);
+  const int tok = n >= 4 ? 4 : 1;
+  const long long tiles = (long long)c.num_rows * ((n + tok - 1) / tok);
+  const int grid = (int)(tiles < 148 * 64 ? tiles : 148 * 64);
+  if (dtype == JX_BF16) {
+    if (tok == 4) kv4_read_kernel<bf16, 4><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (bf16*)k, (bf16*)v);
+    else kv4_read_kernel<bf16, 1><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (bf16*)k, (bf16*)v);
+  } else {
+    if (tok == 4) kv4_read_kernel<float, 4><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (float*)k, (float*)v);
+    else kv4_read_kernel<float, 1><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (float*)k, (float*)v);
+  }
   return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
