@@ -465,7 +465,7 @@ int jx_kv4_attend(const jx_kv4_cache* cache, int layer, int S, int Hq, const voi
                   long long q_head, void* out, float scale, int window, void* ws, long long ws_bytes, int dtype,
                   void* stream) {
   KV4_CHECK("jx_kv4_attend");
-  if (!q || !out || !ws || ((uintptr_t)out & 15) || ((uintptr_t)ws & 15))
+  if (!q || !out || ((uintptr_t)out & 15) || ((uintptr_t)ws & 15))
     return fail(JX_ERR_ARG, "jx_kv4_attend: null pointer, or out / ws not 16-byte aligned");
   if (layer < 0 || layer >= cache->num_layers || S <= 0 || window < 0)
     return fail(JX_ERR_SHAPE, "jx_kv4_attend: layer out of range, S < 1 or window < 0");
@@ -475,7 +475,8 @@ int jx_kv4_attend(const jx_kv4_cache* cache, int layer, int S, int Hq, const voi
   if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_attend: float32 or bfloat16");
   if ((uintptr_t)q % (dtype == JX_BF16 ? 2 : 4)) return fail(JX_ERR_ARG, "jx_kv4_attend: misaligned queries");
   if (!(scale > -1e30f && scale < 1e30f)) return fail(JX_ERR_ARG, "jx_kv4_attend: scale must be finite");
-  if (ws_bytes < kv4_attend_workspace(*cache, S, Hq, dtype)) return fail(JX_ERR_ARG, "jx_kv4_attend: workspace too small");
+  if ((ws ? ws_bytes : 0) < kv4_attend_workspace(*cache, S, Hq, dtype))
+    return fail(JX_ERR_ARG, "jx_kv4_attend: workspace too small");
   const long long qs[3] = {q_row, q_tok, q_head};
   return kv4_done(run_kv4_attend(*cache, layer, S, Hq, q, qs, out, scale, window, ws, dtype, (cudaStream_t)stream),
                   "jx_kv4_attend");

@@ -782,7 +782,7 @@ Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int dtype) {
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;
   const long long slots = l.tc ? 2ll * 2 * kMostCtas : 2ll * kMostCtas * kMostWarps;   // two for every run
-  l.bytes = l.group ? 16 : l.part_at + slots * tile * (c.head_dim + 2) * 4;
+  l.bytes = l.group ? 0 : l.part_at + slots * tile * (c.head_dim + 2) * 4;
   return l;
 }
 

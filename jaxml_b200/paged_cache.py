@@ -248,18 +248,19 @@ class PagedKVCache:
         if heads % self.num_kv_heads:
             raise ValueError(f"q heads must be a multiple of the {self.num_kv_heads} KV heads, got {heads}.")
         scale = self.head_dim ** -0.5 if scale is None else normalize_float("scale", scale)
-        window = 0 if sliding_window is None else _positive("sliding_window", sliding_window)
+        window = 0 if sliding_window is None else min(_positive("sliding_window", sliding_window), 2 ** 31 - 1)
+        dtype = _DTYPES[q.dtype]
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        key = (S, heads, q.dtype)
-        size = self._ws_bytes.get(key)
+        size = self._ws_bytes.get((S, heads, dtype))
         if size is None:
             n = N.LL()
-            N.check(N.load().jx_kv4_attend_workspace(self._ref, S, heads, _DTYPES[q.dtype], n), "jx_kv4_attend_workspace")
-            self._ws_bytes[key] = size = n.value
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+            N.check(N.load().jx_kv4_attend_workspace(self._ref, S, heads, dtype, n), "jx_kv4_attend_workspace")
+            self._ws_bytes[(S, heads, dtype)] = size = n.value
+        # a workspace of its own for every call: calls on several streams, and graphs, do not share one
+        ws = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None
         st = q.stride()
-        self._call("jx_kv4_attend", layer, S, heads, q.data_ptr(), st[0], st[1], st[2], out.data_ptr(), scale,
-                   min(window, 2 ** 31 - 1), ws.data_ptr(), size, _DTYPES[q.dtype])
+        self._call("jx_kv4_attend", layer, S, heads, q.data_ptr(), st[0], st[1], st[2], out.data_ptr(), scale, window,
+                   ws.data_ptr() if size else None, size, dtype)
         return out
 
     def position_ids(self, length: int) -> torch.Tensor:

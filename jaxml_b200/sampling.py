@@ -312,7 +312,7 @@ def token_log_probs(logits: torch.Tensor, token_ids, top_n: int = 0) -> TokenLog
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, V)      # before the narrowing: a wrapped id would be another token's
         ids = ids.to(device=dev, dtype=torch.int32).contiguous()
-    lp = torch.empty(lead, dtype=torch.float32, device=dev)
+    lp = torch.empty_like(ids, dtype=torch.float32)
     ent = torch.empty_like(lp)
     top_lp = torch.empty(lead + (top_n,), dtype=torch.float32, device=dev)
     top_ids = torch.empty_like(top_lp, dtype=torch.int32)

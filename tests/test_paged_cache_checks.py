@@ -136,7 +136,11 @@ def test_c_entries_refuse_bad_arguments():
     rd = lambda layer=0, n=1, k=p, dt=N.JX_BF16: lib.jx_kv4_read(c, layer, None, 0, n, k, p, dt, None)  # noqa: E731
     assert [rd(layer=1), rd(n=0)] == [S] * 2 and [rd(k=None), rd(k=p + 8)] == [A] * 2 and rd(dt=3) == D
     size = N.LL()
-    assert lib.jx_kv4_attend_workspace(c, 1, 4, N.JX_BF16, size) == N.JX_OK and size.value > 0
+    assert lib.jx_kv4_attend_workspace(c, 1, 4, N.JX_BF16, size) == N.JX_OK and size.value == 0     # short tables need none
+    long = _native_cache(row_pages=1000)
+    assert lib.jx_kv4_attend_workspace(long, 1, 4, N.JX_BF16, size) == N.JX_OK and size.value > 0
+    assert lib.jx_kv4_attend(long, 0, 1, 4, p, 1, 1, 1, p, 1.0, 0, p, size.value - 1, N.JX_BF16, None) == A
+    assert lib.jx_kv4_attend(long, 0, 1, 4, p, 1, 1, 1, p, 1.0, 0, None, 1 << 40, N.JX_BF16, None) == A
     assert lib.jx_kv4_attend_workspace(c, 0, 4, N.JX_BF16, size) == S
     assert lib.jx_kv4_attend_workspace(c, 1, 3, N.JX_BF16, size) == S
 
@@ -144,7 +148,7 @@ def test_c_entries_refuse_bad_arguments():
         return lib.jx_kv4_attend(c, layer, S_, Hq, q, 1, 1, 1, out, scale, window, ws, n, dt, None)
 
     assert [att(layer=1), att(S_=0), att(Hq=3), att(Hq=0), att(window=-1), att(S_=1 << 30)] == [S] * 6
-    assert [att(q=None), att(q=p + 1), att(out=p + 2), att(ws=None), att(n=0), att(scale=float("nan"))] == [A] * 6
+    assert [att(q=None), att(q=p + 1), att(out=p + 2), att(ws=p + 8), att(scale=float("nan"))] == [A] * 5
     assert att(dt=2) == D
     assert lib.jx_kv4_extend(c, None, -1, p, 1 << 40, None) == S
     assert lib.jx_kv4_extend(c, None, 1, None, 1 << 40, None) == A and lib.jx_kv4_extend(c, None, 1, p, 3, None) == A
