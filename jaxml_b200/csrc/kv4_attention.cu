@@ -19,6 +19,7 @@
 //
 // A page's block is one tensor-map box of 144 rows of hd / 2 bytes, swizzled by the copy so that ldmatrix gives every
 // thread its words of the key it owns without bank conflicts.
+#include <algorithm>
 #include "kv4_attend.cuh"
 
 namespace jxb {
@@ -627,9 +628,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendA
   }
 }
 
-// ---- one CTA for every (row, query tile, KV head) -----------------------------------------------------------------
-// Slices of 16 keys go round the CTA's warps and their results meet in shared memory: one launch, and the shortest way
-// from the page table to the result.
+// ---- one CTA, or a cluster of them, for every (row, query tile, KV head) ----------------------------------------
+// A CTA takes its share of the pages; slices of 16 keys go round its warps and their results meet in shared memory, those
+// of a cluster's CTAs in each other's: one launch, and the shortest way from the page table to the result.
 template <int HD, int NT, typename T>
 struct Group {
   using C = Cfg<HD, NT, T>;
@@ -637,7 +638,7 @@ struct Group {
   static constexpr int kPages = HD == 64 ? 8 : 4;          // pages in shared memory at a time
   static constexpr int kJoin = kWarps * C::kSlot * 4;
   static constexpr int kRing = kPages * C::kBlock > kJoin ? kPages * C::kBlock : kJoin;
-  static constexpr int kSmem = kRing + C::kQBytes + kPages * 16 + 1024;
+  static constexpr int kSmem = kRing + C::kQBytes + kPages * 16 + C::kSlot * 4 + 1024;
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
@@ -653,16 +654,23 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
   int* bad = reinterpret_cast<int*>(bars + R::kPages);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const jx_kv4_cache& c = a.c;
-  const int item = blockIdx.x / c.num_kv_heads, head = blockIdx.x - item * c.num_kv_heads;
-  const Item t = item_at<C::kRows>(a, item);
+  float* mine = reinterpret_cast<float*>(bad + 2 * R::kPages);      // [kSlot] this CTA's (O, m, l)
+  const int cs = (int)cluster_nctarank(), rank = (int)cluster_ctarank(), seg = blockIdx.x / cs;
+  const int item = seg / c.num_kv_heads, head = seg - item * c.num_kv_heads;
+  Item t = item_at<C::kRows>(a, item);
   const int f0 = t.qt * C::kRows, rows = min(C::kRows, a.S * a.G - f0);
   if (tid == 0) {
     prefetch_tmap(&map);
     if (c.counts[t.r] > a.S) set_status(c.status, JX_ERR_RANGE);
   }
   if (t.n == 0) {
-    for (int i = tid; i < rows * HD; i += R::kThreads) out_row<HD, T>(a, t.r, head, f0 + i / HD)[i % HD] = from_f<T>(0.f);
+    for (int i = tid; rank == 0 && i < rows * HD; i += R::kThreads)
+      out_row<HD, T>(a, t.r, head, f0 + i / HD)[i % HD] = from_f<T>(0.f);
     return;
+  }
+  {                                     // this CTA's pages
+    const int p = t.n * rank / cs, q = t.n * (rank + 1) / cs;
+    t.p0 += p, t.n = q - p;
   }
   int id = -1;
   if (tid < R::kPages) {
@@ -738,11 +746,43 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
 #pragma unroll
       for (int k = 0; k < 8; ++k) x[k] = fmaf(slot[j * HD + d + k], f, x[k]);
     }
+    if (cs == 1) {
+      const float inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] *= inv;
+      store_row8<T>(out_row<HD, T>(a, t.r, head, f0 + j) + d, x);
+    } else {
+      store_row8<float>(mine + j * HD + d, x);
+      if (d == 0) mine[C::kRows * HD + 2 * j] = mx, mine[C::kRows * HD + 2 * j + 1] = sum;
+    }
+  }
+  if (cs == 1) return;
+  cluster_sync_all();
+  for (int i = rank * R::kThreads + tid; i < rows * (HD / 8); i += cs * R::kThreads) {
+    const int j = i / (HD / 8), d = i % (HD / 8) * 8;
+    const uint32_t ml = smem_u32(mine + C::kRows * HD + 2 * j), at = smem_u32(mine + j * HD + d);
+    float mx = -INFINITY, sum = 0.f, x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int q = 0; q < cs; ++q) mx = fmaxf(mx, dsmem_ld_f32(dsmem_map(ml, q)));
+    const float use = mx == -INFINITY ? 0.f : mx;
+    for (int q = 0; q < cs; ++q) {
+      const uint32_t mq = dsmem_map(ml, q), oq = dsmem_map(at, q);
+      const float f = exp2_f(dsmem_ld_f32(mq) - use);
+      sum = fmaf(dsmem_ld_f32(mq + 4), f, sum);
+#pragma unroll
+      for (int k = 0; k < 8; k += 4) {
+        float4 o;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w) : "r"(oq + k * 4) : "memory");
+        x[k] = fmaf(o.x, f, x[k]), x[k + 1] = fmaf(o.y, f, x[k + 1]);
+        x[k + 2] = fmaf(o.z, f, x[k + 2]), x[k + 3] = fmaf(o.w, f, x[k + 3]);
+      }
+    }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[k] *= inv;
     store_row8<T>(out_row<HD, T>(a, t.r, head, f0 + j) + d, x);
   }
+  cluster_sync_all();      // the others' shared memory is read until here
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
@@ -763,13 +803,23 @@ int sm_count() {
 
 struct Layout {
   int nt, tiles;
-  bool group;            // one CTA per (row, tile, head)
+  int group;             // CTAs per (row, tile, head), 0: equal runs
   bool tc;               // 128 query rows a tile, on tcgen05
   long long items, first_at, part_at, bytes;
 };
-constexpr int kGroupPages = 16, kTcRows = 33;
+// Groups or equal runs. A group has no split to compute and no second launch; its CTAs have to be resident at once
+// (head_dim 64 and 128: two an SM, 256: one) and have few pages each, or equal runs over all of the GPU win. One row,
+// 32 query heads on 8 of 128 features, bf16, microseconds group : runs at 256, 768, 2000, 8000, 16000 cached tokens:
+// 6.4 : 10.8, 7.2 : 11.4, 8.4 : 12.6, 16 : 18.9, 26 : 28; 4 rows 6.8 : 11.2, 7.9 : 11.6, 10.6 : 13.2, 19.7 : 22.7,
+// 32 : 30; 16 rows 6.8 : 11.7, 11.6 : 13.2, and 25 : 21 at 2000; 64 rows 15 : 19, 27 : 30, and 62 : 51 at 2000. A cluster
+// larger than a wave of CTAs loses at once: 16 rows at 768 tokens take 17 with 512 CTAs, 11.6 with 256; 4 rows of 8 heads
+// of 256 features 25 with 256 CTAs, 10.2 with 128. Heads of 64 in fp32 cross over at the same places.
+constexpr int kGroupPages = 4;    // pages a CTA, as long as the wave has room for more CTAs
+constexpr int kGroupMost = 16;    // pages a CTA above which runs win
+constexpr int kGroupWave = 296;   // CTAs resident at once, head_dim 64 and 128
+constexpr int kTcRows = 33;
 constexpr int kMostCtas = 160, kMostWarps = 12;
-Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int dtype) {
+Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int window, int dtype) {
   Layout l;
   const int G = Hq / c.num_kv_heads;
   const long long rows = (long long)S * G;
@@ -778,7 +828,15 @@ Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int dtype) {
   const int tile = l.tc ? 128 : 8 * l.nt;
   l.tiles = (int)((rows + tile - 1) / tile);
   l.items = (long long)c.num_rows * l.tiles;
-  l.group = !l.tc && l.nt <= 2 && c.row_pages <= kGroupPages;
+  l.group = 0;
+  if (!l.tc && l.nt <= 2) {
+    long long pages = c.row_pages;                     // that a row can see
+    if (window > 0) pages = std::min(pages, ((long long)window + S - 2) / kPage + 2);
+    const long long segs = l.items * c.num_kv_heads, wave = kGroupWave / (c.head_dim == 256 ? 2 : 1);
+    int cs = 1;
+    while (cs < 8 && pages > kGroupPages * cs && segs * cs * 2 <= wave) cs *= 2;
+    if (pages <= kGroupMost * cs) l.group = cs;
+  }
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;
   const long long slots = l.tc ? 2ll * 2 * kMostCtas : 2ll * kMostCtas * kMostWarps;   // two for every run
@@ -851,8 +909,20 @@ int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStr
       using R = Group<HD, NT, T>;
       static bool ready[64];
       if (const int rc = allow(kv4_attend_group_kernel<HD, NT, T>, R::kSmem, ready)) return rc;
-      kv4_attend_group_kernel<HD, NT, T><<<a.items * a.c.num_kv_heads, R::kThreads, R::kSmem, s>>>(a, map);
-      return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+      if (l.group == 1) {
+        kv4_attend_group_kernel<HD, NT, T><<<a.items * a.c.num_kv_heads, R::kThreads, R::kSmem, s>>>(a, map);
+        return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+      }
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3((unsigned)(a.items * a.c.num_kv_heads * l.group));
+      cfg.blockDim = dim3(R::kThreads);
+      cfg.dynamicSmemBytes = R::kSmem;
+      cfg.stream = s;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = l.group, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+      cfg.attrs = at, cfg.numAttrs = 1;
+      return cudaLaunchKernelEx(&cfg, kv4_attend_group_kernel<HD, NT, T>, a, map) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
     }
   }
   using R = Runs<HD, NT, T>;
@@ -890,11 +960,12 @@ int launch_hd(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cuda
 
 }  // namespace
 
-long long kv4_attend_workspace(const jx_kv4_cache& c, int S, int Hq, int dtype) { return layout_of(c, S, Hq, dtype).bytes; }
+// Enough for any window: fewer pages never turn a group into runs.
+long long kv4_attend_workspace(const jx_kv4_cache& c, int S, int Hq, int dtype) { return layout_of(c, S, Hq, 0, dtype).bytes; }
 
 int run_kv4_attend(const jx_kv4_cache& c, int layer, int S, int Hq, const void* q, const long long* qs, void* out,
                    float scale, int window, void* ws, int dtype, cudaStream_t s) {
-  const Layout l = layout_of(c, S, Hq, dtype);
+  const Layout l = layout_of(c, S, Hq, window, dtype);
   AttendArgs a;
   a.c = c, a.layer = layer, a.S = S, a.Hq = Hq, a.G = Hq / c.num_kv_heads, a.window = window;
   a.items = (int)l.items, a.tiles = l.tiles, a.sign = scale < 0.f ? -1.f : 1.f;
