@@ -51,4 +51,22 @@ __device__ __forceinline__ uint32_t kv4_nibble(float x, float s) {
   return (uint32_t)((int)q + 8);
 }
 
+// Pairs of bfloat16 from nibbles.
+namespace kv4 {
+__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
+__device__ __forceinline__ uint32_t as_u(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
+// bfloat16 pair 128 + u of the nibbles k and k + 4 of a word (or k of two merged words).
+__device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(r) : "r"(w >> (4 * k)));
+  return r;
+}
+// Code times scale in one fused multiply-add, exact: (128 + u) s - 136 s = (u - 8) s.  136 s is 17 times a 4-bit number, at
+// most 255, times a power of two: a bfloat16.
+__device__ __forceinline__ uint32_t minus136(uint32_t s2) { return as_u(__hmul2(as_b2(s2), as_b2(0xC308C308u))); }
+__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2, uint32_t c2) {
+  return as_u(__hfma2(as_b2(raw2(w, k)), as_b2(s2), as_b2(c2)));
+}
+}  // namespace kv4
+
 }  // namespace jxb

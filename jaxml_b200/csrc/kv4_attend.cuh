@@ -22,21 +22,7 @@ struct AttendArgs {
 };
 
 // ---- small pieces -------------------------------------------------------------------------------------
-__device__ __forceinline__ __nv_bfloat162 as_b2(uint32_t x) { return *reinterpret_cast<__nv_bfloat162*>(&x); }
-__device__ __forceinline__ uint32_t as_u(__nv_bfloat162 x) { return *reinterpret_cast<uint32_t*>(&x); }
-// bfloat16 pair 128 + u of the nibbles k and k + 4 of a word (or k of two merged words).
-__device__ __forceinline__ uint32_t raw2(uint32_t w, int k) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000F000F, 0x43004300, 0xEA;" : "=r"(r) : "r"(w >> (4 * k)));
-  return r;
-}
 __device__ __forceinline__ uint32_t code2(uint32_t w, int k) { return as_u(__hsub2(as_b2(raw2(w, k)), as_b2(0x43084308u))); }
-// Code times scale in one fused multiply-add, exact: (128 + u) s - 136 s = (u - 8) s.  136 s is 17 times a 4-bit number, at
-// most 255, times a power of two: a bfloat16.
-__device__ __forceinline__ uint32_t minus136(uint32_t s2) { return as_u(__hmul2(as_b2(s2), as_b2(0xC308C308u))); }
-__device__ __forceinline__ uint32_t scaled2(uint32_t w, int k, uint32_t s2, uint32_t c2) {
-  return as_u(__hfma2(as_b2(raw2(w, k)), as_b2(s2), as_b2(c2)));
-}
 // Whether a pair of scales has one that the format does not (NaN; 2^120 or more): bits to be or'ed and tested against
 // 0x80008000.
 __device__ __forceinline__ uint32_t bad_scales(uint32_t s2) { return (s2 & 0x7FFF7FFFu) + (0x8000u - kKv4BadScale) * 0x10001u; }

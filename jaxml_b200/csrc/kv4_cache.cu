@@ -4,35 +4,68 @@
 // rows that hold a page.  Forked rows share pages; a shared page that is not full is copied when a row is about to
 // write on it (copy on write in jx_kv4_extend).  Every choice of a page is the lowest free one, rows in order, so the
 // same calls give the same tables whatever the scheduling; the only atomics are integer counts.
+#include <algorithm>
+
 #include "kv4.cuh"
 
 namespace jxb {
 namespace {
 
 // ------------------------------------------------------------------------------------------------
-// append: one CTA per token; 8 channels a thread, 4 threads a group
+// append and read.  A thread owns 8 channels of one head of keys or values (4 threads a group of 32) and goes through
+// tiles of kTok neighbouring positions: a tile starts at a multiple of kTok, so it lies in one page, and its loads are
+// under way together.  The tile's scales are 32 neighbouring bytes at 128 channels; thread j of a group handles the
+// j-th token's.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float* x);
+struct Eight;   // 8 values as they lie in memory
 template <>
-__device__ __forceinline__ void load8<bf16>(const bf16* p, bool vec, float* x) {
-  if (vec) {
-    unpack8(*reinterpret_cast<const uint4*>(p), x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f(p[i]);
+struct Eight<bf16> {
+  uint4 v;
+  __device__ __forceinline__ void zero() { v = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const bf16* p, bool vec) {
+    if (vec) {
+      v = *reinterpret_cast<const uint4*>(p);
+    } else {
+      const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+      v = make_uint4(q[0] | (uint32_t)q[1] << 16, q[2] | (uint32_t)q[3] << 16, q[4] | (uint32_t)q[5] << 16,
+                     q[6] | (uint32_t)q[7] << 16);
+    }
   }
-}
+  __device__ __forceinline__ uint32_t amax_bits() const {   // two 16-bit maxima at a time, widened at the end
+    uint32_t m = max_u16x2(max_u16x2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), max_u16x2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+    return max(m & 0xFFFF0000u, m << 16);
+  }
+  static __device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ void get(float* x) const { unpack8(v, x); }
+};
 template <>
-__device__ __forceinline__ void load8<float>(const float* p, bool vec, float* x) {
-  if (vec) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p, bool vec) {
+    if (vec) {
+      a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    } else {
+      a = make_float4(p[0], p[1], p[2], p[3]), b = make_float4(p[4], p[5], p[6], p[7]);
+    }
+  }
+  __device__ __forceinline__ void get(float* x) const {
     x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
   }
-}
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    float x[8];
+    get(x);
+    uint32_t m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+    return m;
+  }
+};
 
 struct AppendArgs {
   jx_kv4_cache c;
@@ -41,21 +74,25 @@ struct AppendArgs {
   long long row[2], tok[2], head[2];   // element strides
 };
 
-// The nibbles of 8 values of a group.  bfloat16 values: the quotient by a product with 1 / s and one step of correction,
-// which is the correctly rounded one where that matters: a quotient that is a half step is represented exactly, so the
-// correction lands on it, and any other is off a half step by at least 2^-9 of itself, far beyond what the step leaves.
+// The nibbles of 8 values of a group.  bfloat16 values x = X 2^a (X <= 255) over a scale s = M 2^b (M <= 15): a quotient
+// that is no half step is off each of them by at least 1 / 30 or by a 255th of itself, 2^-10.  So x times an approximate
+// 1 / s (off by 2^-19 at most), added to 6144 and rounded there to a multiple of 2^-11, is a half step exactly where x / s
+// is one, and the second sum rounds it to an integer, ties to even, leaving 8 + q in its low byte.  |q| <= 7.44: no clamp.
 // float32 values, and scales near the ends of the range, take the division.
 template <typename T>
-__device__ __forceinline__ uint32_t nibbles(const float* x, float s) {
+__device__ __forceinline__ uint32_t nibbles(const Eight<T>& v, float s) {
+  float x[8];
+  v.get(x);
   uint32_t w = 0;
   if (sizeof(T) == 2 && s > 1e-30f && s < 1e30f) {
-    const float inv = __frcp_rn(s);
+    float inv;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    uint32_t n[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float q0 = x[j] * inv, q = fmaf(fmaf(-q0, s, x[j]), inv, q0);
-      // 1.5 * 2^23 + q rounds to an integer (ties to even) in the lower bits; + 8 makes the nibble.  |q| <= 7.44: no clamp
-      w |= (__float_as_uint(q + 12582920.f) & 15u) << (4 * j);
-    }
+    for (int j = 0; j < 8; ++j) n[j] = __float_as_uint(fmaf(x[j], inv, 6144.f) + (12582920.f - 6144.f));
+    const uint32_t even = __byte_perm(__byte_perm(n[0], n[2], 0x0040), __byte_perm(n[4], n[6], 0x0040), 0x5410);
+    const uint32_t odd = __byte_perm(__byte_perm(n[1], n[3], 0x0040), __byte_perm(n[5], n[7], 0x0040), 0x5410);
+    w = odd * 16u + even;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) w |= kv4_nibble(x[j], s) << (4 * j);
@@ -63,123 +100,128 @@ __device__ __forceinline__ uint32_t nibbles(const float* x, float s) {
   return w;
 }
 
-// Each CTA takes kTok neighbouring tokens of a row: their loads are under way together.
-template <typename T, int kTok>
+template <typename T, int HD, int kTok>
 __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
+  static_assert(kTok == 1 || kTok == 4, "a group of four threads shares the scales of four tokens");
   const jx_kv4_cache& c = a.c;
-  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per, tiles = (a.S + kTok - 1) / kTok;
-  for (long long t = blockIdx.x; t < (long long)c.num_rows * tiles; t += gridDim.x) {
-    const int r = (int)(t / tiles), i0 = (int)(t - (long long)r * tiles) * kTok;
-    const int cnt = c.counts[r];
-    if (i0 == 0 && cnt > a.S && threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
-    if (i0 >= cnt) continue;
-    const int pos0 = c.lengths[r] - cnt + i0;
-    int page[kTok];
+  constexpr int kPer = HD / 8;
+  const int it = blockIdx.y * blockDim.x + threadIdx.x, half = c.num_kv_heads * kPer;
+  const int tiles = (a.S + kTok - 1) / kTok + (kTok > 1), lane = threadIdx.x & 31;
+  const bool lead = it == 0, live = it < 2 * half;   // the others only take part in the shuffles
+  const int which = live && it >= half, head = live ? (it - which * half) / kPer : 0, ch = it % kPer;
+  const T* src = static_cast<const T*>(a.src[which]) + head * a.head[which] + ch * 8;
+  const long long tok = a.tok[which];
+  const int r = blockIdx.z, cnt = c.counts[r], first = c.lengths[r] - cnt, n = min(cnt, a.S);
+  if (lead && blockIdx.x == 0 && cnt > a.S) set_status(c.status, JX_ERR_RANGE);
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int base = (first & ~(kTok - 1)) + tile * kTok, i0 = base - first;   // tokens i0 .. i0 + kTok - 1 of n
+    if (i0 >= n || i0 + kTok <= 0) continue;
+    int page = -1;
+    if (base >= 0 && base < c.row_pages * kPage) page = c.table[(long long)r * c.row_pages + base / kPage];
+    if (page < 0 || page >= c.num_pages) {
+      if (lead) set_status(c.status, JX_ERR_RANGE);
+      continue;
+    }
+    const T* p = src + r * a.row[which] + i0 * tok;
+    Eight<T> x[kTok];
 #pragma unroll
     for (int j = 0; j < kTok; ++j) {
-      const int pos = pos0 + j;
-      page[j] = -1;
-      if (i0 + j < min(cnt, a.S)) {
-        if (pos >= 0 && pos < c.row_pages * kPage) page[j] = c.table[(long long)r * c.row_pages + pos / kPage];
-        if (page[j] < 0 || page[j] >= c.num_pages) {
-          page[j] = -1;
-          if (threadIdx.x == 0) set_status(c.status, JX_ERR_RANGE);
-        }
-      }
+      if (live && i0 + j >= 0 && i0 + j < n) x[j].load(p + j * tok, a.vec);
+      else x[j].zero();
     }
-    for (int it = threadIdx.x; it < items; it += blockDim.x) {   // items and blockDim are multiples of 4
-      const int which = it >= items / 2, rest = it - which * (items / 2), head = rest / per, ch = rest % per;
-      const T* p = static_cast<const T*>(a.src[which]) + r * a.row[which] + i0 * a.tok[which] +
-                   head * a.head[which] + ch * 8;
-      float x[kTok][8];
+    uint32_t own = 0;
 #pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        if (page[j] >= 0) {
-          load8<T>(p + j * a.tok[which], a.vec, x[j]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[j][e] = 0.f;
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) m = max(m, __float_as_uint(x[j][e]) & 0x7FFFFFFFu);
-        const unsigned group = 0xFu << (threadIdx.x & 28);
-        m = max(m, __shfl_xor_sync(group, m, 1));
-        m = max(m, __shfl_xor_sync(group, m, 2));
-        if (page[j] < 0) continue;
-        const float s = kv4_scale(m);
-        const int slot = (pos0 + j) % kPage;
-        unsigned char* blk = kv4_block(c, a.layer, page[j], head);
-        *reinterpret_cast<uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4) = nibbles<T>(x[j], s);
-        if ((ch & 3) == 0)
-          *reinterpret_cast<bf16*>(blk + kv4_scale_offset(hd, which) + (slot * (hd / 32) + (ch >> 2)) * 2) =
-              __float2bfloat16_rn(s);
-      }
+    for (int j = 0; j < kTok; ++j) {
+      uint32_t m = x[j].amax_bits();
+      m = max(m, __shfl_xor_sync(~0u, m, 1));
+      m = max(m, __shfl_xor_sync(~0u, m, 2));
+      if (kTok == 1 || (lane & 3) == j) own = m;
     }
+    const float scale = kv4_scale(own);
+    const int slot = base % kPage;
+    unsigned char* blk = kv4_block(c, a.layer, page, head);
+    unsigned char* at = blk + (which * kPage + slot) * (HD / 2) + ch * 4;
+#pragma unroll
+    for (int j = 0; j < kTok; ++j) {
+      const float s = kTok == 1 ? scale : __shfl_sync(~0u, scale, j, 4);
+      if (live && i0 + j >= 0 && i0 + j < n) *reinterpret_cast<uint32_t*>(at + j * (HD / 2)) = nibbles<T>(x[j], s);
+    }
+    const int mine = kTok == 1 ? 0 : lane & 3;
+    if (live && (kTok == 1 ? (lane & 3) == 0 : i0 + mine >= 0 && i0 + mine < n))
+      *reinterpret_cast<bf16*>(blk + kv4_scale_offset(HD, which) + ((slot + mine) * (HD / 32) + (ch >> 2)) * 2) =
+          __float2bfloat16_rn(scale);
   }
 }
 
-// ------------------------------------------------------------------------------------------------
-// read back: token start + i of every row, zeros outside it
-// ------------------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x);
-template <>
-__device__ __forceinline__ void store8<bf16>(bf16* p, const float* x) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
-                                            pack_bf16x2(x[6], x[7]));
-}
-template <>
-__device__ __forceinline__ void store8<float>(float* p, const float* x) {
+// Read back: token start + i of every row, zeros outside it.
+__device__ __forceinline__ void store8(bf16* p, uint4 v) { *reinterpret_cast<uint4*>(p) = v; }
+__device__ __forceinline__ void store8(float* p, uint4 v) {
+  float x[8];
+  unpack8(v, x);
   reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
-template <typename T, int kTok>
+template <typename T, int HD, int kTok>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const jx_kv4_cache c, int layer, const int* start, int start_add, int n,
                                                        T* k, T* v) {
-  const int hd = c.head_dim, per = hd >> 3, items = 2 * c.num_kv_heads * per, tiles = (n + kTok - 1) / kTok;
-  for (long long t = blockIdx.x; t < (long long)c.num_rows * tiles; t += gridDim.x) {
-    const int r = (int)(t / tiles), i0 = (int)(t - (long long)r * tiles) * kTok;
-    const long long pos0 = (long long)(start ? start[r] : 0) + start_add + i0;
-    const int len = min(c.lengths[r], c.row_pages * kPage);
-    int page[kTok];
-#pragma unroll
-    for (int j = 0; j < kTok; ++j) {
-      page[j] = -1;
-      if (pos0 + j >= 0 && pos0 + j < len) {
-        page[j] = c.table[(long long)r * c.row_pages + (pos0 + j) / kPage];
-        if (page[j] < 0 || page[j] >= c.num_pages) {
-          page[j] = -1;
-          if (threadIdx.x == 0 && i0 + j < n) set_status(c.status, JX_ERR_RANGE);
-        }
+  constexpr int kPer = HD / 8;
+  const int it = blockIdx.y * blockDim.x + threadIdx.x, half = c.num_kv_heads * kPer;
+  const int tiles = (n + kTok - 1) / kTok + (kTok > 1);
+  const int which = it >= half, head = (it - which * half) / kPer, ch = it % kPer;
+  T* dst = (which ? v : k) + (long long)head * HD + ch * 8;
+  const long long tok = (long long)c.num_kv_heads * HD;
+  if (it >= 2 * half) return;
+  const int r = blockIdx.z, len = min(c.lengths[r], c.row_pages * kPage);
+  const long long first = (long long)(start ? start[r] : 0) + start_add;
+  for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const long long base = (first & ~(long long)(kTok - 1)) + (long long)tile * kTok;
+    const int i0 = (int)(base - first);
+    if (i0 >= n || i0 + kTok <= 0) continue;
+    int page = -1;
+    if (base >= 0 && base < len) {
+      page = c.table[(long long)r * c.row_pages + base / kPage];
+      if (page < 0 || page >= c.num_pages) {
+        page = -1;
+        if (it == 0) set_status(c.status, JX_ERR_RANGE);
       }
     }
-    for (int it = threadIdx.x; it < items; it += blockDim.x) {
-      const int which = it >= items / 2, rest = it - which * (items / 2), head = rest / per, ch = rest % per;
-      uint32_t w[kTok];
-      float s[kTok];
+    uint32_t w[kTok], s[kTok];
 #pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        w[j] = 0x88888888u, s[j] = 0.f;
-        if (page[j] >= 0) {
-          const unsigned char* blk = kv4_block(c, layer, page[j], head);
-          const int slot = (int)((pos0 + j) & (kPage - 1));
-          w[j] = *reinterpret_cast<const uint32_t*>(blk + which * kPage * (hd / 2) + slot * (hd / 2) + ch * 4);
-          s[j] = to_f(*reinterpret_cast<const bf16*>(blk + kv4_scale_offset(hd, which) + (slot * (hd / 32) + (ch >> 2)) * 2));
+    for (int j = 0; j < kTok; ++j) w[j] = 0x88888888u, s[j] = 0;
+    if (page >= 0) {
+      const unsigned char* blk = kv4_block(c, layer, page, head);
+      const int slot = (int)(base & (kPage - 1));
+      const unsigned char* at = blk + (which * kPage + slot) * (HD / 2) + ch * 4;
+      const unsigned char* sc = blk + kv4_scale_offset(HD, which) + (slot * (HD / 32) + (ch >> 2)) * 2;
+#pragma unroll
+      for (int j = 0; j < kTok; ++j)
+        if (base + j < len) {
+          w[j] = *reinterpret_cast<const uint32_t*>(at + j * (HD / 2));
+          s[j] = *reinterpret_cast<const uint16_t*>(sc + j * (HD / 32) * 2);
         }
-      }
+    }
+    T* out = dst + ((long long)r * n + i0) * tok;
 #pragma unroll
-      for (int j = 0; j < kTok; ++j) {
-        if (i0 + j >= n) continue;
+    for (int j = 0; j < kTok; ++j) {
+      if (i0 + j < 0 || i0 + j >= n) continue;
+      uint4 o;
+      if (s[j] < kKv4BadScale) {
+        // (128 + u) s - 136 s (kv4.cuh), for the nibbles e and e + 4 at a time
+        const uint32_t s2 = s[j] * 0x10001u, c2 = kv4::minus136(s2);
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = kv4::scaled2(w[j], e, s2, c2);
+        o = make_uint4(__byte_perm(x[0], x[1], 0x5410), __byte_perm(x[2], x[3], 0x5410), __byte_perm(x[0], x[1], 0x7632),
+                       __byte_perm(x[2], x[3], 0x7632));
+      } else {   // NaN, or no scale of this format
         float x[8];
+        const float f = __uint_as_float(s[j] << 16);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)((int)((w[j] >> (4 * e)) & 15u) - 8) * s[j];
-        store8<T>((which ? v : k) + ((((long long)r * n + i0 + j) * c.num_kv_heads + head) * hd + ch * 8), x);
+        for (int e = 0; e < 8; ++e) x[e] = (float)((int)((w[j] >> (4 * e)) & 15u) - 8) * f;
+        o = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
       }
+      store8(out + j * tok, o);
     }
   }
 }
@@ -457,6 +499,54 @@ __global__ void __launch_bounds__(128) kv4_shorten_kernel(const jx_kv4_cache c, 
   }
 }
 
+// Tiles of four positions from four tokens a row on; a shorter call has more threads at one position each.
+constexpr int kTileFrom = 4;
+
+struct Shape {
+  dim3 grid;
+  int threads;
+};
+Shape shape_of(const jx_kv4_cache& c, int n, int tok) {
+  const int items = 2 * c.num_kv_heads * (c.head_dim / 8), threads = items < 256 ? (items + 31) / 32 * 32 : 256;
+  const int chunks = (items + threads - 1) / threads;
+  const int tiles = (n + tok - 1) / tok + (tok > 1), most = std::max(1, 148 * 64 / (chunks * c.num_rows));
+  return {dim3((unsigned)std::min(tiles, most), (unsigned)chunks, (unsigned)c.num_rows), threads};
+}
+
+template <typename T, int HD>
+void launch_append_hd(const AppendArgs& a, cudaStream_t s) {
+  if (a.S >= kTileFrom) {
+    const Shape g = shape_of(a.c, a.S, 4);
+    kv4_append_kernel<T, HD, 4><<<g.grid, g.threads, 0, s>>>(a);
+  } else {
+    const Shape g = shape_of(a.c, a.S, 1);
+    kv4_append_kernel<T, HD, 1><<<g.grid, g.threads, 0, s>>>(a);
+  }
+}
+template <typename T>
+void launch_append(const AppendArgs& a, cudaStream_t s) {
+  if (a.c.head_dim == 64) launch_append_hd<T, 64>(a, s);
+  else if (a.c.head_dim == 128) launch_append_hd<T, 128>(a, s);
+  else launch_append_hd<T, 256>(a, s);
+}
+
+template <typename T, int HD>
+void launch_read_hd(const jx_kv4_cache& c, int layer, const int* start, int start_add, int n, T* k, T* v, cudaStream_t s) {
+  if (n >= kTileFrom) {
+    const Shape g = shape_of(c, n, 4);
+    kv4_read_kernel<T, HD, 4><<<g.grid, g.threads, 0, s>>>(c, layer, start, start_add, n, k, v);
+  } else {
+    const Shape g = shape_of(c, n, 1);
+    kv4_read_kernel<T, HD, 1><<<g.grid, g.threads, 0, s>>>(c, layer, start, start_add, n, k, v);
+  }
+}
+template <typename T>
+void launch_read(const jx_kv4_cache& c, int layer, const int* start, int start_add, int n, T* k, T* v, cudaStream_t s) {
+  if (c.head_dim == 64) launch_read_hd<T, 64>(c, layer, start, start_add, n, k, v, s);
+  else if (c.head_dim == 128) launch_read_hd<T, 128>(c, layer, start, start_add, n, k, v, s);
+  else launch_read_hd<T, 256>(c, layer, start, start_add, n, k, v, s);
+}
+
 }  // namespace
 
 int run_kv4_append(const jx_kv4_cache& c, int layer, int S, const void* k, const void* v, const long long* ks,
@@ -470,35 +560,15 @@ int run_kv4_append(const jx_kv4_cache& c, int layer, int S, const void* k, const
   a.vec = 1;
   for (int i = 0; i < 2; ++i)
     if (((uintptr_t)a.src[i] & 15) || a.row[i] % unit || a.tok[i] % unit || a.head[i] % unit) a.vec = 0;
-  const int items = 2 * c.num_kv_heads * (c.head_dim / 8);
-  const int threads = items < 256 ? (items + 31) / 32 * 32 : 256;
-  const int tok = S >= 4 ? 4 : 1;
-  const long long tiles = (long long)c.num_rows * ((S + tok - 1) / tok);
-  const int grid = (int)(tiles < 148 * 64 ? tiles : 148 * 64);
-  if (dtype == JX_BF16) {
-    if (tok == 4) kv4_append_kernel<bf16, 4><<<grid, threads, 0, s>>>(a);
-    else kv4_append_kernel<bf16, 1><<<grid, threads, 0, s>>>(a);
-  } else {
-    if (tok == 4) kv4_append_kernel<float, 4><<<grid, threads, 0, s>>>(a);
-    else kv4_append_kernel<float, 1><<<grid, threads, 0, s>>>(a);
-  }
+  if (dtype == JX_BF16) launch_append<bf16>(a, s);
+  else launch_append<float>(a, s);
   return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
 int run_kv4_read(const jx_kv4_cache& c, int layer, const int* start, int start_add, int n, void* k, void* v, int dtype,
                  cudaStream_t s) {
-  const int items = 2 * c.num_kv_heads * (c.head_dim / 8);
-  const int threads = items < 256 ? (items + 31) / 32 * 32 : 256;
-  const int tok = n >= 4 ? 4 : 1;
-  const long long tiles = (long long)c.num_rows * ((n + tok - 1) / tok);
-  const int grid = (int)(tiles < 148 * 64 ? tiles : 148 * 64);
-  if (dtype == JX_BF16) {
-    if (tok == 4) kv4_read_kernel<bf16, 4><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (bf16*)k, (bf16*)v);
-    else kv4_read_kernel<bf16, 1><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (bf16*)k, (bf16*)v);
-  } else {
-    if (tok == 4) kv4_read_kernel<float, 4><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (float*)k, (float*)v);
-    else kv4_read_kernel<float, 1><<<grid, threads, 0, s>>>(c, layer, start, start_add, n, (float*)k, (float*)v);
-  }
+  if (dtype == JX_BF16) launch_read(c, layer, start, start_add, n, (bf16*)k, (bf16*)v, s);
+  else launch_read(c, layer, start, start_add, n, (float*)k, (float*)v, s);
   return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
