@@ -222,26 +222,31 @@ __device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0,
   // 64 groups are as good a bound for few elements and cost a sixteenth of the comparisons
   const uint32_t t = want <= 32 ? nth_largest<4>(s.best, &s.bound, mine, want) : nth_largest<1>(s.best, &s.bound, mine, want);
   const int per = rounds_per_slot;
-  // this thread's elements of a slot that are at least `from`
+  // This thread's elements of a slot that are at least `from`.  The comparisons go without branches and the few hits are
+  // read again: this code runs once a row, and a short one costs its instruction fetches (a branch with its body for every
+  // element of a batch took 9 us of a row's 40).
   auto each = [&](int slot, uint32_t from, auto&& f) {
-    const float least = key_value(from);
+    const float least = from == 0 ? -INFINITY : key_value(from);
+#pragma unroll 1
     for (int r = slot * per; r < slot * per + per; ++r) {
       uint4 u[4];
       const int v = v0 + r * 4 * kThreads + tid;
 #pragma unroll
       for (int j = 0; j < 4; ++j) u[j] = v + j * kThreads < v1 ? row.load(v + j * kThreads) : make_uint4(0, 0, 0, 0);
+      uint32_t hits = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (v + j * kThreads >= v1) continue;
         float x[kE];
         Row<T>::floats(u[j], x);
 #pragma unroll
-        for (int e = 0; e < kE; ++e)
-          if (from == 0 || x[e] >= least) {
-            const int i = (v + j * kThreads) * kE + e;
-            const uint32_t k = order_key(x[e]);
-            if (k >= from && i >= row.first && i < row.last) f(k, i - row.first);
-          }
+        for (int e = 0; e < kE; ++e) hits |= x[e] >= least ? 1u << (j * kE + e) : 0u;
+      }
+#pragma unroll 1
+      for (; hits; hits &= hits - 1) {
+        const int b = __ffs(hits) - 1, w = v + b / kE * kThreads, i = w * kE + b % kE;
+        if (w >= v1 || i < row.first || i >= row.last) continue;
+        const uint32_t k = order_key(to_f(row.base[i]));
+        if (k >= from) f(k, i - row.first);
       }
     }
   };
@@ -258,10 +263,11 @@ __device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0,
     __syncthreads();
     return s.n_cand;
   };
-  int n = collect(t);
-  if (n > kCand) {          // so many equal to t: those above it, then the equal ones by index
+  int n = 0;
+#pragma unroll 1
+  for (uint32_t from = t; from <= t + 1; ++from) {   // so many equal to t: those above it, then the equal ones by index
     __syncthreads();
-    n = collect(t + 1);
+    if ((n = collect(from)) <= kCand) break;
   }
   if (n > kCand) {
     // too many above t in a few batches: one after the other
