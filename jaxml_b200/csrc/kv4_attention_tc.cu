@@ -24,6 +24,41 @@ namespace {
 
 constexpr int kRows = 128, kSoft = 128, kDeq = 128, kThreads = kSoft + kDeq + 64, kRing = 3;
 
+template <int kOff>
+__device__ __forceinline__ uint32_t lds_u32(uint32_t at) {
+  uint32_t r;
+  asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(r) : "r"(at), "n"(kOff));
+  return r;
+}
+template <int kOff>
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) {
+  uint16_t r;
+  asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(r) : "r"(at), "n"(kOff));
+  return r;
+}
+__device__ __forceinline__ void lds_v2(uint32_t at, uint32_t& a, uint32_t& b) {
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "r"(at));
+}
+__device__ __forceinline__ void lds_v4(uint32_t at, uint32_t& a, uint32_t& b, uint32_t& c, uint32_t& d) {
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(a), "=r"(b), "=r"(c), "=r"(d) : "r"(at));
+}
+__device__ __forceinline__ void sts_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// Keys 2 E and 2 E + 1 of a group of 8: a word of codes each, at `vp` and `other` bytes on (offsets of the group's first
+// pair), and their scales as a pair, at `sp` of the group's first key.
+template <int HD, int E>
+__device__ __forceinline__ void load_keys(uint32_t vp, uint32_t other, uint32_t sp, uint32_t* x, uint32_t* sc) {
+  constexpr int kLine = 2 * E * (HD / 2), kXor = (kLine >> 7 & (HD / 32 - 1)) << 4;
+  const uint32_t at = vp ^ kXor;
+  x[2 * E] = lds_u32<kLine>(at);
+  // at head_dim 256 a key is a line of its own, and the other key of the pair has its last bit in the xor
+  x[2 * E + 1] = lds_u32<kLine>((HD == 256 ? at ^ 16u : at) + other);
+  constexpr int kKey = HD / 16, kPair = 2 * E * kKey, kHigh = kPair & ~15, kLow = kPair & 15;
+  if constexpr (kKey == 16) sc[E] = lds_u16<0>(sp ^ kPair) | lds_u16<0>(sp ^ (kPair + 16)) << 16;
+  else sc[E] = lds_u16<kLow>(sp ^ kHigh) | lds_u16<kLow + kKey>(sp ^ kHigh) << 16;
+}
+
 template <int HD>
 struct Tc {
   static constexpr int kBlock = kPage * HD + kPage * (HD / 32) * 4;
@@ -296,69 +331,65 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
       const int dt = tid - kSoft, dw = warp - 4;
       const int g = lane & 7, t4 = lane >> 3;
       const int pages = (int)(u1 - u0);
+      // What a thread reads of a block, as offsets that the pages share.  The swizzle exchanges 16-byte pieces within 128
+      // bytes by the number of the line, and blocks begin on whole lines: pieces are stepped through by xor.
+      // K: lane (key g of a group of 8, word t4 of a 16-byte piece); a core matrix's rows are 8 neighbouring lanes
+      const uint32_t ring = smem_u32(smem);
+      const uint32_t k_codes = swz<HD>((dw * 16 + g) * (HD / 2)) + t4 * 4;
+      const uint32_t k_to = smem_u32(kbuf) + dw * 2 * C::kKSbo + t4 * 128 + g * 16;
+      // V: 8 keys x 8 channels (word ch of each key); half of a warp takes the keys of a pair the other way round, for the
+      // banks
+      constexpr int kVStep = kDeq / (HD / 8);      // groups of 8 keys that the threads cover at once
+      const int ch = dt % (HD / 8), vj = dt / (HD / 8);
+      const uint32_t flip = (lane >> 4) & 1;
+      const uint32_t v_codes = swz<HD>(kPage * (HD / 2) + (vj * 8 + flip) * (HD / 2) + ch * 4);
+      const uint32_t v_other = flip ? 0u - HD / 2 : HD / 2;
       // step i: K of page i, V of page i - 1
       int st = 0, ring_use = 0, last_st = 0;
       for (int i = 0; i <= pages; ++i) {
         if (i < pages) {
-          const unsigned char* blk = smem + st * C::kBlock;
           const bool ok = wait(&page_full[st], ring_use) && (i == 0 || wait(&s_done[(i - 1) & 1], ((i - 1) >> 1) & 1));
           if (!__all_sync(~0u, ok)) break;
-          // lane (key g of a group of 8, word t4 of a 16-byte piece): a core matrix's rows are 8 neighbouring lanes
+          const uint32_t blk = ring + st * C::kBlock;
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
-            const int kg = dw * 2 + h, key = kg * 8 + g;
+            const uint32_t sp = blk + swz<HD>(kPage * HD + ((dw * 2 + h) * 8 + g) * (HD / 16));
             uint32_t ks[HD / 64];        // the key's scales, two groups a register
-            const unsigned char* sp = blk + swz<HD>(kPage * HD + key * (HD / 16));
-            if constexpr (HD == 64) {
-              ks[0] = *reinterpret_cast<const uint32_t*>(sp);
-            } else if constexpr (HD == 128) {
-              const uint2 v2 = *reinterpret_cast<const uint2*>(sp);
-              ks[0] = v2.x, ks[1] = v2.y;
-            } else {
-              const uint4 v4 = *reinterpret_cast<const uint4*>(sp);
-              ks[0] = v4.x, ks[1] = v4.y, ks[2] = v4.z, ks[3] = v4.w;
-            }
-            const int codes = swz<HD>(key * (HD / 2)) + t4 * 4;       // the swizzle exchanges whole pieces: group by xor
-            unsigned char* to = kbuf + kg * C::kKSbo + t4 * 128 + g * 16;
+            if constexpr (HD == 64) ks[0] = lds_u32<0>(sp);
+            else if constexpr (HD == 128) lds_v2(sp, ks[0], ks[1]);
+            else lds_v4(sp, ks[0], ks[1], ks[2], ks[3]);
+            const uint32_t codes = blk + k_codes + h * (8 * (HD / 2)), to = k_to + h * C::kKSbo;
 #pragma unroll
             for (int grp = 0; grp < HD / 32; ++grp) {
-              const uint32_t x = *reinterpret_cast<const uint32_t*>(blk + (codes ^ (grp * 16)));
+              const uint32_t x = lds_u32<0>(codes ^ (grp * 16));
               const uint32_t s2 = __byte_perm(ks[grp >> 1], 0, grp & 1 ? 0x3232 : 0x1010), c2 = minus136(s2);
-              *reinterpret_cast<uint4*>(to + grp * 512) =
-                  make_uint4(scaled2(x, 0, s2, c2), scaled2(x, 1, s2, c2), scaled2(x, 2, s2, c2), scaled2(x, 3, s2, c2));
+              sts_v4(to + grp * 512, scaled2(x, 0, s2, c2), scaled2(x, 1, s2, c2), scaled2(x, 2, s2, c2), scaled2(x, 3, s2, c2));
             }
           }
           fence_proxy_async();
           arrive(k_ready);
         }
         if (i > 0) {
-          // V: 8 keys x 8 channels a thread, transposed in registers
           const int j0 = i - 1, b = j0 & 1;
-          const unsigned char* blk = smem + last_st * C::kBlock;
           const bool ok = j0 < 2 || wait(&pv_done[b], ((j0 - 2) >> 1) & 1);
           if (!__all_sync(~0u, ok)) break;
-          unsigned char* vd = vbuf + b * C::kVBytes;
+          const uint32_t blk = ring + last_st * C::kBlock, vd = smem_u32(vbuf) + b * C::kVBytes;
           constexpr int kBlocks = HD / 8 * (kPage / 8);
 #pragma unroll 1
           for (int n = 0; n < (kBlocks + kDeq - 1) / kDeq; ++n) {
-            const int q = dt + n * kDeq;
-            if (kBlocks >= kDeq || q < kBlocks) {
-              const int ch = q % (HD / 8), j = q / (HD / 8), flip = (lane >> 4) & 1;   // half of the warp reads the odd key first
+            const int j = vj + n * kVStep;
+            if (kBlocks >= kDeq || dt < kBlocks) {
+              // transposed in registers.  Keys 2 e and 2 e + 1 (exchanged where flip is set): their line's number adds an xor
               uint32_t x[8], sc[4], cc[4];
-              // a word of a key, keys of 8 rows: the swizzle is that of the row alone
-              const unsigned char* vp = blk + kPage * (HD / 2) + j * 8 * (HD / 2);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int row = e ^ flip;
-                x[e] = *reinterpret_cast<const uint32_t*>(vp + swz<HD>(row * (HD / 2) + ch * 4));
-              }
+              const uint32_t vp = blk + v_codes + n * (kVStep * 8 * (HD / 2));
+              const uint32_t sp = blk + swz<HD>(kPage * HD + kPage * (HD / 16) + j * 8 * (HD / 16) + (ch >> 2) * 2);
+              load_keys<HD, 0>(vp, v_other, sp, x, sc);
+              load_keys<HD, 1>(vp, v_other, sp, x, sc);
+              load_keys<HD, 2>(vp, v_other, sp, x, sc);
+              load_keys<HD, 3>(vp, v_other, sp, x, sc);
               uint32_t worst = 0;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int o = kPage * HD + kPage * (HD / 16) + (j * 8 + 2 * e) * (HD / 16) + (ch >> 2) * 2;
-                sc[e] = lds16(blk + swz<HD>(o)) | (lds16(blk + swz<HD>(o + HD / 16)) << 16);
-                worst |= bad_scales(sc[e]);
-              }
+              for (int e = 0; e < 4; ++e) worst |= bad_scales(sc[e]);
               uint32_t nans = 0;
               if (worst & 0x80008000u) {
                 // no scale of the format: 0 for the product (0 * NaN would reach rows that do not see the key), noted for
@@ -372,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
               }
               if ((ch & 3) == 0) nan_keys[(b * 8 + (ch >> 2)) * 8 + j] = (unsigned char)nans;
               const uint32_t lo_sel = flip ? 0x1054u : 0x5410u, hi_sel = flip ? 0x3276u : 0x7632u;
-              unsigned char* to = vd + ch * C::kVSbo + j * 128;
+              const uint32_t to = vd + ch * C::kVSbo + j * 128;
               uint32_t lo[4], hi[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
@@ -388,8 +419,8 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
                   r[e] = scaled2(lo[e], 0, sc[e], cc[e]), r[4 + e] = scaled2(hi[e], 0, sc[e], cc[e]);
                   lo[e] >>= 4, hi[e] >>= 4;
                 }
-                *reinterpret_cast<uint4*>(to + k * 16) = make_uint4(r[0], r[1], r[2], r[3]);
-                *reinterpret_cast<uint4*>(to + (k + 4) * 16) = make_uint4(r[4], r[5], r[6], r[7]);
+                sts_v4(to + k * 16, r[0], r[1], r[2], r[3]);
+                sts_v4(to + (k + 4) * 16, r[4], r[5], r[6], r[7]);
               }
             }
           }
