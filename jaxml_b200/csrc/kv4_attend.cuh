@@ -18,7 +18,8 @@ struct AttendArgs {
   void* out;
   long long* item_first;   // [items] first unit of an item (written by the first CTA)
   long long* total;        // [2] units, warps
-  float* part;             // [warps][2] slots of 8 * NT rows: O, then m and l
+  // [runs][2] slots of a tile's rows: O, then (m, l) of each row.  O is [rows][hd], of 128 rows (a thread a row) [hd / 4][128][4]
+  float* part;
 };
 
 // ---- small pieces -------------------------------------------------------------------------------------
@@ -101,30 +102,53 @@ __device__ __forceinline__ long long run_of(long long u, long long units, long l
 }
 
 // ---- loading queries ----------------------------------------------------------------------------------------
-// 8 neighbouring channels as fragment registers (0,4) (1,5) (2,6) (3,7), a float32 split into `parts`.
-__device__ __forceinline__ void q_words(const bf16* p, bool vec, float sign, uint4* out) {
-  uint32_t x[4];
-  if (vec) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
-  } else {
-    const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+// 8 neighbouring channels as they lie in memory.
+template <typename T>
+struct QPiece {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = h[2 * i] | ((uint32_t)h[2 * i + 1] << 16);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
   }
+  __device__ __forceinline__ void load_unaligned(const T* p) {
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(x)[i];
+  }
+};
+// N pieces `step` elements apart, zeros for a row that is not there.  All loads are under way together: one after the other
+// they were 16 trips to memory for a row of 128 channels.
+template <int N, typename T>
+__device__ __forceinline__ void q_load(const T* p, int step, bool live, bool vec, QPiece<T>* q) {
+  if (live && vec) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i].load(p + i * step);
+  } else if (live) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) q[i].load_unaligned(p + i * step);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(T) / 2; ++k) q[i].u[k] = make_uint4(0, 0, 0, 0);
+  }
+}
+// A piece as fragment registers (0,4) (1,5) (2,6) (3,7), a float32 split into 3 parts.
+__device__ __forceinline__ void q_words(const QPiece<bf16>& q, float sign, uint4* out) {
+  uint32_t x[4] = {q.u[0].x, q.u[0].y, q.u[0].z, q.u[0].w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) x[i] ^= sign < 0.f ? 0x80008000u : 0u;
   out[0] = make_uint4(__byte_perm(x[0], x[2], 0x5410), __byte_perm(x[0], x[2], 0x7632), __byte_perm(x[1], x[3], 0x5410),
                       __byte_perm(x[1], x[3], 0x7632));
 }
-__device__ __forceinline__ void q_words(const float* p, bool vec, float sign, uint4* out) {
+__device__ __forceinline__ void q_words(const QPiece<float>& q, float sign, uint4* out) {
   float x[8];
-  if (vec) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
+  for (int i = 0; i < 2; ++i) {
+    x[4 * i] = __uint_as_float(q.u[i].x), x[4 * i + 1] = __uint_as_float(q.u[i].y);
+    x[4 * i + 2] = __uint_as_float(q.u[i].z), x[4 * i + 3] = __uint_as_float(q.u[i].w);
   }
 #pragma unroll
   for (int i = 0; i < 8; ++i) x[i] *= sign;

@@ -79,15 +79,13 @@ struct Tile {
       const int f = f0 + nt * 8 + g, s = f / a.G;
       const bool live = f < F && s < t.cnt;
       const T* src = static_cast<const T*>(a.q) + t.r * a.q_row + s * a.q_tok + (head * a.G + (f - s * a.G)) * a.q_head;
+      constexpr int kTogether = C::kGroups < 4 ? C::kGroups : 4;
+      QPiece<T> piece[kTogether];
 #pragma unroll
       for (int i = 0; i < C::kGroups; ++i) {
         uint4 x[C::kQParts];
-        if (live) {
-          q_words(src + i * 32 + tq * 8, a.q_vec, a.sign, x);
-        } else {
-#pragma unroll
-          for (int p = 0; p < C::kQParts; ++p) x[p] = make_uint4(0, 0, 0, 0);
-        }
+        if (i % kTogether == 0) q_load<kTogether>(src + i * 32 + tq * 8, 32, live, a.q_vec, piece);
+        q_words(piece[i % kTogether], a.sign, x);
 #pragma unroll
         for (int p = 0; p < C::kQParts; ++p) {
           if constexpr (C::kQReg) q[nt][p][i] = x[p];
@@ -553,7 +551,17 @@ __global__ void __launch_bounds__(Runs<HD, NT, T>::kThreads, 1)
 // loads under way together; where one row may be spread over the whole grid all warps of a CTA share one.  Rows without a
 // visible key are zero.
 constexpr int kJoinWarps = 8, kMany = 4;
-template <int HD, typename T, bool kSpread>
+template <int kW>
+__device__ __forceinline__ void load_row(const float* p, float* x) {
+  if constexpr (kW == 2) {
+    const float2 v = *reinterpret_cast<const float2*>(p);
+    x[0] = v.x, x[1] = v.y;
+  } else {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+  }
+}
+template <int HD, typename T, bool kSpread, bool kTc>
 __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendArgs a, int rows) {
   constexpr int kR = kSpread ? 1 : kMany, kV = HD / 32;
   pdl_wait();
@@ -585,8 +593,17 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kv4_join_kernel(const AttendA
     for (int q = 0; q < kR; ++q) {
       const int j = j0 + min(q, live - 1);
       mw[q] = slot[rows * HD + 2 * j], lw[q] = slot[rows * HD + 2 * j + 1];
+      if constexpr (kTc) {
+        constexpr int kW = kV < 4 ? kV : 4;
 #pragma unroll
-      for (int i = 0; i < kV; ++i) ow[q][i] = slot[j * HD + lane * kV + i];
+        for (int i = 0; i < kV; i += kW) {
+          const int at = lane * kV + i;
+          load_row<kW>(slot + (at / 4 * 128 + j) * 4 + at % 4, &ow[q][i]);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) ow[q][i] = slot[j * HD + lane * kV + i];
+      }
     }
 #pragma unroll
     for (int q = 0; q < kR; ++q) {
@@ -884,7 +901,7 @@ int allow(K kernel, int bytes, bool (&ready)[64]) {
 }
 
 // The second kernel, for tiles of `rows` query rows and that many runs.
-template <int HD, typename T>
+template <int HD, typename T, bool kTc>
 int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
   const long long segments = a.items * (long long)a.c.num_kv_heads;
   const int there = a.tiles > 1 || a.S * a.G >= rows ? rows : a.S * a.G;
@@ -898,8 +915,8 @@ int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return (few ? cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, false>, a, rows)
-              : cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, true>, a, rows)) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return (few ? cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, false, kTc>, a, rows)
+              : cudaLaunchKernelEx(&cfg, kv4_join_kernel<HD, T, true, kTc>, a, rows)) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
 }
 
 template <int HD, int NT, typename T>
@@ -934,7 +951,7 @@ int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStr
   if (most < grid) grid = (int)most;
   kv4_attend_runs_kernel<HD, NT, T><<<grid, R::kThreads, R::kSmem, s>>>(a, map);
   if (cudaPeekAtLastError() != cudaSuccess) return JX_ERR_CUDA;
-  return join<HD, T>(a, Cfg<HD, NT, T>::kRows, grid * R::kWarps, s);
+  return join<HD, T, false>(a, Cfg<HD, NT, T>::kRows, grid * R::kWarps, s);
 }
 
 template <int HD, typename T>
@@ -943,7 +960,7 @@ int launch_nt(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cuda
     if (l.tc) {
       const int sms = sm_count() < kMostCtas ? sm_count() : kMostCtas;
       if (const int rc = run_kv4_attend_tc(&a, &map, sms, s)) return rc;
-      return join<HD, T>(a, 128, HD == 256 ? sms : 2 * sms, s);
+      return join<HD, T, true>(a, 128, HD == 256 ? sms : 2 * sms, s);
     }
   if (l.nt == 1) return launch<HD, 1, T>(l, a, map, s);
   if constexpr (HD < 256 && sizeof(T) == 2)

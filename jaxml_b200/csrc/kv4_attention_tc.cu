@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();   // the join's launch is under way; it waits for this kernel's end
   const uint32_t tmem = *tmem_slot;
   long long before = 0, units = 0;
 #pragma unroll
@@ -460,10 +461,12 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
 #pragma unroll 1
           for (int part = 0; part < HD / 64; ++part) {
             uint32_t r[32];
+            QPiece<bf16> piece[8];
+            q_load<8>(src + part * 64, 8, live, a.q_vec, piece);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              uint4 x = make_uint4(0, 0, 0, 0);
-              if (live) q_words(src + part * 64 + k * 8, a.q_vec, a.sign, &x);
+              uint4 x;
+              q_words(piece[k], a.sign, &x);
               r[4 * k] = x.x, r[4 * k + 1] = x.y, r[4 * k + 2] = x.z, r[4 * k + 3] = x.w;
             }
             __syncwarp();
@@ -589,7 +592,11 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
                 for (int e = 0; e < 8; ++e)
                   y[e] = (nan_groups >> part) & 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float(r[k + e]) * inv;
                 if (whole) store_row8<bf16>(o + part * 32 + k, y);
-                else store_row8<float>(slot + tid * HD + part * 32 + k, y);
+                else
+#pragma unroll
+                  for (int e = 0; e < 8; e += 4)
+                    *reinterpret_cast<float4*>(slot + ((part * 32 + k + e) / 4 * kRows + tid) * 4) =
+                        make_float4(y[e], y[e + 1], y[e + 2], y[e + 3]);
               }
             }
             __syncwarp();
