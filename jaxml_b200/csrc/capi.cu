@@ -434,7 +434,8 @@ int jx_kv4_append(const jx_kv4_cache* cache, int layer, int S, const void* k, lo
                   void* stream) {
   KV4_CHECK("jx_kv4_append");
   if (!k || !v) return fail(JX_ERR_ARG, "jx_kv4_append: null keys or values");
-  if (layer < 0 || layer >= cache->num_layers || S <= 0) return fail(JX_ERR_SHAPE, "jx_kv4_append: layer out of range, or S < 1");
+  if (layer < 0 || layer >= cache->num_layers || S <= 0 || S > (1 << 30))
+    return fail(JX_ERR_SHAPE, "jx_kv4_append: layer out of range, or S not within [1, 2^30]");
   if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_append: float32 or bfloat16");
   const uintptr_t size = dtype == JX_BF16 ? 2 : 4;
   if ((uintptr_t)k % size || (uintptr_t)v % size) return fail(JX_ERR_ARG, "jx_kv4_append: misaligned keys or values");
@@ -447,7 +448,8 @@ int jx_kv4_read(const jx_kv4_cache* cache, int layer, const int* start, int star
   KV4_CHECK("jx_kv4_read");
   if (!k || !v || ((uintptr_t)k & 15) || ((uintptr_t)v & 15))
     return fail(JX_ERR_ARG, "jx_kv4_read: outputs must be 16-byte aligned");
-  if (layer < 0 || layer >= cache->num_layers || n <= 0) return fail(JX_ERR_SHAPE, "jx_kv4_read: layer out of range, or n < 1");
+  if (layer < 0 || layer >= cache->num_layers || n <= 0 || n > (1 << 30))
+    return fail(JX_ERR_SHAPE, "jx_kv4_read: layer out of range, or n not within [1, 2^30]");
   if (dtype != JX_F32 && dtype != JX_BF16) return fail(JX_ERR_DTYPE, "jx_kv4_read: float32 or bfloat16");
   return kv4_done(run_kv4_read(*cache, layer, start, start_add, n, k, v, dtype, (cudaStream_t)stream), "jx_kv4_read");
 }

@@ -170,9 +170,9 @@ struct Tile {
 #pragma unroll
             for (int k = 0; k < 4; ++k) r[h][k] = C::kRaw ? raw2(kw[h][w], k) : code2(kw[h][w], k);
 #pragma unroll
-          for (int p = 0; p < C::kQParts; ++p) {
+          for (int p = C::kQParts - 1; p >= 0; --p) {   // the small parts first
             const uint4 b = query(0, p, w, lane);
-            if (p == 0) {
+            if (p == C::kQParts - 1) {
               const float c0 = C::kRaw ? init[w][0] : 0.f, c1 = C::kRaw ? init[w][1] : 0.f;
               mma_c(x, r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y, c0, c1, c0, c1);
             } else {
@@ -198,14 +198,20 @@ struct Tile {
             for (int k = 0; k < 4; ++k) r[h][k] = scaled2(kw[h][w], k, s2, c2);
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            float own[4], (&x)[4] = C::kF32 ? own : sc[i][nt];     // float32: a group's products by themselves (Tile)
 #pragma unroll
-            for (int p = 0; p < C::kQParts; ++p) {
+            for (int p = C::kQParts - 1; p >= 0; --p) {
               const uint4 b = query(nt, p, w, lane);
-              if (w == 0 && p == 0) mma_c(sc[i][nt], r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y, 0.f, 0.f, 0.f, 0.f);
-              else mma_bf16(sc[i][nt], r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y);
-              mma_bf16(sc[i][nt], r[0][2], r[1][2], r[0][3], r[1][3], b.z, b.w);
+              if ((C::kF32 || w == 0) && p == C::kQParts - 1) mma_c(x, r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y, 0.f, 0.f, 0.f, 0.f);
+              else mma_bf16(x, r[0][0], r[1][0], r[0][1], r[1][1], b.x, b.y);
+              mma_bf16(x, r[0][2], r[1][2], r[0][3], r[1][3], b.z, b.w);
             }
+            if constexpr (C::kF32) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sc[i][nt][e] = w == 0 ? own[e] : sc[i][nt][e] + own[e];
+            }
+          }
         }
       }
     }
@@ -234,7 +240,7 @@ struct Tile {
         mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, 16));
         mx = fmaxf(mx, m[nt][e]);
         const float use = mx == -INFINITY ? 0.f : -mx * a.scale_log2;      // nothing visible yet: every term is 2^-inf
-        f[e] = exp2_f(fmaf(m[nt][e], a.scale_log2, use));
+        f[e] = exp2_f(__fmul_rn(m[nt][e], a.scale_log2) + use);    // the reference that the older terms were rounded to
         m[nt][e] = mx;
         float sum = 0.f;
 #pragma unroll
@@ -299,10 +305,18 @@ struct Tile {
           const uint32_t a0 = scaled2(lo0, k, s2[0], c2[0]), a1 = scaled2(hi0, k, s2[0], c2[0]);
           const uint32_t a2 = scaled2(lo1, k, s2[1], c2[1]), a3 = scaled2(hi1, k, s2[1], c2[1]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            if constexpr (C::kF32) {
+              float x[4];
+              mma_c(x, a0, a1, a2, a3, pf[i][nt][C::kPParts - 1][0], pf[i][nt][C::kPParts - 1][1], 0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int p = 0; p < C::kPParts; ++p)
-              mma_bf16(acc[wd * 4 + k][nt], a0, a1, a2, a3, pf[i][nt][p][0], pf[i][nt][p][1]);
+              for (int p = C::kPParts - 2; p >= 0; --p) mma_bf16(x, a0, a1, a2, a3, pf[i][nt][p][0], pf[i][nt][p][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[wd * 4 + k][nt][e] += x[e];
+            } else {
+              mma_bf16(acc[wd * 4 + k][nt], a0, a1, a2, a3, pf[i][nt][0][0], pf[i][nt][0][1]);
+            }
+          }
         }
       }
     }
@@ -803,13 +817,6 @@ __global__ void __launch_bounds__(Group<HD, NT, T>::kThreads)
 }
 
 // ---- host ----------------------------------------------------------------------------------------------------
-// Query rows are taken in tiles of 8, 16 or 32: the smallest that holds all S * G rows of a KV head, or 32 (16 where the
-// accumulators of 32 rows would not fit the registers), which then reads every page once per tile.
-int n_tiles_of(int hd, int dtype, long long rows) {
-  const int most = hd == 256 || dtype == JX_F32 ? 2 : 4;
-  return rows <= 8 ? 1 : rows <= 16 || most == 2 ? 2 : 4;
-}
-
 int sm_count() {
   static int n[64] = {0};
   int dev = 0;
@@ -834,19 +841,22 @@ struct Layout {
 constexpr int kGroupPages = 4;    // pages a CTA, as long as the wave has room for more CTAs
 constexpr int kGroupMost = 16;    // pages a CTA above which runs win
 constexpr int kGroupWave = 296;   // CTAs resident at once, head_dim 64 and 128
-constexpr int kTcRows = 33;
+// bfloat16 rows of a KV head (S * G) from which they are 128 a tile on tcgen05, instead of tiles of 8 or 16 on mma.sync that
+// each read the pages: 12 rows of 2048 tokens, 8 of them in the batch, take 25.2 us against 24.4 (mma.sync), 16 rows 26.3
+// either way, 24 rows 27.4 against 45.8, 64 rows 35 against 64; 20 rows of 256 features 40 against 46.
+constexpr int kTcRows = 17;
 constexpr int kMostCtas = 160, kMostWarps = 12;
 Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int window, int dtype) {
   Layout l;
   const int G = Hq / c.num_kv_heads;
   const long long rows = (long long)S * G;
-  l.nt = n_tiles_of(c.head_dim, dtype, rows);
+  l.nt = rows <= 8 ? 1 : 2;     // float32 tiles of 32 rows would not fit the registers
   l.tc = dtype == JX_BF16 && rows >= kTcRows;
   const int tile = l.tc ? 128 : 8 * l.nt;
   l.tiles = (int)((rows + tile - 1) / tile);
   l.items = (long long)c.num_rows * l.tiles;
   l.group = 0;
-  if (!l.tc && l.nt <= 2) {
+  if (!l.tc) {
     long long pages = c.row_pages;                     // that a row can see
     if (window > 0) pages = std::min(pages, ((long long)window + S - 2) / kPage + 2);
     const long long segs = l.items * c.num_kv_heads, wave = kGroupWave / (c.head_dim == 256 ? 2 : 1);
@@ -905,7 +915,10 @@ template <int HD, typename T, bool kTc>
 int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
   const long long segments = a.items * (long long)a.c.num_kv_heads;
   const int there = a.tiles > 1 || a.S * a.G >= rows ? rows : a.S * a.G;
-  const bool few = runs <= 4 * segments;    // some four parts a segment, if they are alike
+  // Parts a segment, if they are alike.  A CTA a query row is better from 2 on (64 rows of 2000 tokens, 3.5 parts: 48.0
+  // against 50.7 us for the whole call; 128 rows, 1.7 parts: 58.8 against 56.8), in tiles of 128 query rows, where most of
+  // its warps have none, from 6 on (4.6 parts: 64.6 against 58.0; 18 parts: 36 against 68).
+  const bool few = runs <= (there >= 32 ? 6 : 2) * segments;
   cudaLaunchConfig_t cfg = {};
   const int each = few ? kJoinWarps * kMany : 1;
   cfg.gridDim = dim3((unsigned)segments, (unsigned)((there + each - 1) / each));
@@ -921,26 +934,24 @@ int join(const AttendArgs& a, int rows, int runs, cudaStream_t s) {
 
 template <int HD, int NT, typename T>
 int launch(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cudaStream_t s) {
-  if constexpr (NT <= 2) {
-    if (l.group) {
-      using R = Group<HD, NT, T>;
-      static bool ready[64];
-      if (const int rc = allow(kv4_attend_group_kernel<HD, NT, T>, R::kSmem, ready)) return rc;
-      if (l.group == 1) {
-        kv4_attend_group_kernel<HD, NT, T><<<a.items * a.c.num_kv_heads, R::kThreads, R::kSmem, s>>>(a, map);
-        return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
-      }
-      cudaLaunchConfig_t cfg = {};
-      cfg.gridDim = dim3((unsigned)(a.items * a.c.num_kv_heads * l.group));
-      cfg.blockDim = dim3(R::kThreads);
-      cfg.dynamicSmemBytes = R::kSmem;
-      cfg.stream = s;
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeClusterDimension;
-      at[0].val.clusterDim.x = l.group, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
-      cfg.attrs = at, cfg.numAttrs = 1;
-      return cudaLaunchKernelEx(&cfg, kv4_attend_group_kernel<HD, NT, T>, a, map) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  if (l.group) {
+    using R = Group<HD, NT, T>;
+    static bool ready[64];
+    if (const int rc = allow(kv4_attend_group_kernel<HD, NT, T>, R::kSmem, ready)) return rc;
+    if (l.group == 1) {
+      kv4_attend_group_kernel<HD, NT, T><<<a.items * a.c.num_kv_heads, R::kThreads, R::kSmem, s>>>(a, map);
+      return cudaPeekAtLastError() == cudaSuccess ? JX_OK : JX_ERR_CUDA;
     }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(a.items * a.c.num_kv_heads * l.group));
+    cfg.blockDim = dim3(R::kThreads);
+    cfg.dynamicSmemBytes = R::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = l.group, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
+    cfg.attrs = at, cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv4_attend_group_kernel<HD, NT, T>, a, map) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
   }
   using R = Runs<HD, NT, T>;
   static_assert(R::kWarps <= kMostWarps, "workspace");
@@ -963,8 +974,6 @@ int launch_nt(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cuda
       return join<HD, T, true>(a, 128, HD == 256 ? sms : 2 * sms, s);
     }
   if (l.nt == 1) return launch<HD, 1, T>(l, a, map, s);
-  if constexpr (HD < 256 && sizeof(T) == 2)
-    if (l.nt == 4) return launch<HD, 4, T>(l, a, map, s);
   return launch<HD, 2, T>(l, a, map, s);
 }
 

@@ -499,8 +499,12 @@ __global__ void __launch_bounds__(128) kv4_shorten_kernel(const jx_kv4_cache c, 
   }
 }
 
-// Tiles of four positions from four tokens a row on; a shorter call has more threads at one position each.
-constexpr int kTileFrom = 4;
+// Tiles of four positions where single ones would fill the GPU's threads already: 8 channels a thread, 16 rows of 8 heads of
+// 128 take 4.5 us a call with single positions and 5.2 with tiles at 4 tokens, 4.75 and 5.15 at 32, 6.8 and 6.2 at 64, 26.9
+// and 16.9 at 512 (append and read).
+bool tiles_of_four(const jx_kv4_cache& c, int n) {
+  return n >= 4 && (long long)c.num_rows * n * 2 * c.num_kv_heads * (c.head_dim / 8) >= 1 << 18;
+}
 
 struct Shape {
   dim3 grid;
@@ -515,7 +519,7 @@ Shape shape_of(const jx_kv4_cache& c, int n, int tok) {
 
 template <typename T, int HD>
 void launch_append_hd(const AppendArgs& a, cudaStream_t s) {
-  if (a.S >= kTileFrom) {
+  if (tiles_of_four(a.c, a.S)) {
     const Shape g = shape_of(a.c, a.S, 4);
     kv4_append_kernel<T, HD, 4><<<g.grid, g.threads, 0, s>>>(a);
   } else {
@@ -532,7 +536,7 @@ void launch_append(const AppendArgs& a, cudaStream_t s) {
 
 template <typename T, int HD>
 void launch_read_hd(const jx_kv4_cache& c, int layer, const int* start, int start_add, int n, T* k, T* v, cudaStream_t s) {
-  if (n >= kTileFrom) {
+  if (tiles_of_four(c, n)) {
     const Shape g = shape_of(c, n, 4);
     kv4_read_kernel<T, HD, 4><<<g.grid, g.threads, 0, s>>>(c, layer, start, start_add, n, k, v);
   } else {

@@ -551,10 +551,12 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_pro
 
 template <typename T>
 int launch(const jx_log_probs_args& a, cudaStream_t s) {
-  // CTAs per row: enough for three on every multiprocessor, while a slice keeps two rounds of vectors
+  // CTAs per row: as long as each has a multiprocessor to itself, and its slice two rounds of vectors.  128256 bfloat16
+  // logits, top 20, 1 : 2 : 4 : 8 CTAs a row: 7 rows 16.7 : 13.7 : 12.8 : 13.6 us, 37 rows 17.3 : 14.4 : 15.0 : 18.5, 74 rows
+  // 17.7 : 14.7 : 18.7 : 29.6, 148 rows 17.5 : 19.4 : 28.8 : 45.6.
   const int e = 16 / (int)sizeof(T);
   int C = 1;
-  while (C < 8 && (long long)a.rows * C < 3 * 148 && a.V / (2 * C) >= 2 * kThreads * 4 * e / 4) C *= 2;
+  while (C < 4 && (long long)a.rows * C * 2 <= 148 && a.V / (2 * C) >= 2 * kThreads * 4 * e / 4) C *= 2;
   const long long nv = ((long long)a.V + e - 1) / e + 1;      // a row off its boundary has one vector more
   const long long per_cta = (nv + C - 1) / C;
   const long long rounds = (per_cta + 4 * kThreads - 1) / (4 * kThreads);

@@ -5,9 +5,9 @@ Writing and reading are exact: every value equals the restatement's.  Page manag
   bfloat16: half a step of the output (2^-8 |o|) and of every probability before its product with v (2^-8 A);
   both:     float32 sums of hd terms in a score, each product and sum off by at most 2^-23 of what has been summed
             (e = hd 2^-23 scale sum |q k|, twice: numerator and normaliser), and of the row's keys (T 2^-23 A);
-  bfloat16: the kernels sum codes with an offset and take it off again.  A key's group enters as 128 + u with u <= 15 and
+  bfloat16: one kernel sums key codes with an offset and takes it off again.  A key's group enters as 128 + u with u <= 15 and
             -136 sum q: what is summed is at most 143 s |q| a channel, over 33 terms (2 * 33 * 2^-23 scale sum 143 s |q|
-            for A).  A value enters as u s and leaves 8 sum p s: at most 15 s each (2 T 2^-23 15 sum p s).
+            for A).
 """
 import random
 
@@ -169,9 +169,7 @@ def _check_attend(got, q, ks, vs, lens, counts, scale, window=0):
         tol = A[:n] * e + 1e-30
         if q.dtype == torch.bfloat16:
             spread = torch.einsum("shd,thd->sht", q[r, :n].double().abs(), ks.scale[r].repeat_interleave(G, 1)).amax(-1)
-            ps = K.attend(q[r].double(), ks[r], vs.scale[r], lens[r], counts[r], scale, window)[:n]
             tol = tol + 2.0 ** -8 * (want[:n].abs() + A[:n]) + A[:n] * 2 * 33 * 2.0 ** -23 * abs(scale) * 143 * spread[..., None]
-            tol = tol + 2 * lens[r] * 2.0 ** -23 * 15 * ps
         err = (got[r, :n] - want[:n]).abs()
         assert (err <= tol).all(), (r, (err / tol).max())
 
@@ -603,3 +601,94 @@ def test_beam_steps_with_scores():
     c.free([1])
     used = int(c.compact())
     assert used == len({p for t in _tables(c) for p in t})
+
+
+# -- sizes at which another kernel or another split takes over ----------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,heads,lens", [(64, 2, [9 * PAGE, 0, 1, 200]), (128, 1, [17 * PAGE - 1, 30, 65, 700]),
+                                           (256, 1, [33 * PAGE, 1, 500, 64]), (128, 3, [70 * PAGE + 1, 2, 64 * 3])])
+@pytest.mark.parametrize("window", [0, 100])
+def test_clusters_of_a_few_rows(dtype, hd, heads, lens, window):
+    """A row's pages shared among 2, 4 and 8 CTAs: rows with fewer pages than CTAs, empty rows, a window that leaves most
+    of the table unseen."""
+    counts = [min(1, n) for n in lens]
+    c, ks, vs = _filled(len(lens), lens, counts, heads, hd, seed=hd)
+    q = _rand((len(lens), 1, heads * 4, hd), dtype, 5, 1.5)
+    got = c.attend(0, q.cuda(), sliding_window=window or None)
+    _check_attend(got, q, ks, vs, lens, counts, hd ** -0.5, window)
+    assert torch.equal(got, c.attend(0, q.cuda(), sliding_window=window or None))
+    c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("S", [2, 4, 5, 16, 17, 32, 33])
+def test_query_tiles(dtype, hd, S):
+    """8, 16 and 128 query rows a KV head and one more, on rows of several pages, an idle one and one that is all new."""
+    lens, counts = [300, S, 90 + S, 64], [S, S, max(1, S - 3), 0]
+    c, ks, vs = _filled(4, lens, counts, 2, hd, seed=S)
+    q = _rand((4, S, 8, hd), dtype, 5, 1.5)
+    _check_attend(c.attend(0, q.cuda()), q, ks, vs, lens, counts, hd ** -0.5)
+    _check_attend(c.attend(0, q.cuda(), sliding_window=70), q, ks, vs, lens, counts, hd ** -0.5, 70)
+
+
+def test_float32_keeps_its_digits_over_a_long_row():
+    """The maximum of a long row moves many times, and its terms are summed thousands at a time: the results stay as near to
+    64 bits as float32 sums of 8000 terms in blocks of 16 are, whatever the order of the keys."""
+    n, hd, heads = 8000, 128, 8
+    for rows, scale in ((1, hd ** -0.5), (40, hd ** -0.5), (40, 4 * hd ** -0.5)):
+        c, ks, vs = _filled(1, [n], [rows], 2, hd, seed=7)
+        m = n
+        q = _rand((1, rows, heads, hd), torch.float32, 5)
+        got = c.attend(0, q.cuda(), scale=scale)[0].double().cpu()
+        k, v = ks[0][:m], vs[0][:m]
+        want = K.attend(q[0].double(), k, v, m, rows, scale, 0)
+        # float32 roundings (2^-24 each): a score is 4 group sums of 32 products in three parts, rounded to within 2^-22 of
+        # the sum of its magnitudes; its exponent, and the maximum's, to 2^-24 of themselves (2^-23 after both); 2^x to
+        # 2^-22; the rows' sums grow over 500 blocks, each to 2^-24 of what is there
+        big = torch.einsum("shd,thd->sht", q[0].double().abs(), k.abs().repeat_interleave(heads // 2, 1)).amax(-1) * scale
+        A = K.attend(q[0].double(), k, v.abs(), m, rows, scale, 0)
+        tol = A * (2 * (big[..., None] * (2.0 ** -22 + 2.0 ** -23) + 2.0 ** -22) + 500 * 2.0 ** -24)
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+        # the roundings are as often up as down: the root mean square stays near the largest kind, that of an exponent of
+        # magnitude up to 16 (at a scale of hd^-0.5; four times that at four times the scale)
+        rms = float((got - want).pow(2).mean().sqrt() / want.pow(2).mean().sqrt())
+        assert rms <= 16 * 2.0 ** -24 * max(1.0, scale * hd ** 0.5), rms
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("hd,heads,rows,S", [(256, 8, 8, 70), (128, 8, 3, 701), (64, 3, 40, 140)])
+@pytest.mark.parametrize("before", [0, 1, 2, 63])
+def test_large_appends_are_exact(dtype, hd, heads, rows, S, before):
+    """Calls of many tokens go in tiles of four positions: rows that begin and end anywhere in a tile, special groups."""
+    width = -(-(before + S) // PAGE)
+    c = _cache(1, rows * width, rows, width * PAGE, heads, hd, fill=0xA5)
+    if before:
+        c.extend(before)
+        c.append(0, torch.ones(rows, before, heads, hd, dtype=dtype, device="cuda"),
+                 torch.ones(rows, before, heads, hd, dtype=dtype, device="cuda"))
+    counts = [S if r % 3 == 0 else max(0, S - 5 * r - 1) for r in range(rows)]
+    k, v = _rand((rows, S, heads, hd), dtype, 1, 3.0), _rand((rows, S, heads, hd), dtype, 2, 1e-3)
+    k[:, 3::7, 0] *= 1e-33                                 # scales below and above the quick division's range
+    k[:, 4::7, 0] *= 1e33
+    k[:, 5::7, 0] = 0.0
+    v[:, 2::9, -1, 7], v[:, 3::9, -1, 40] = float("nan"), float("-inf")
+    steps = (torch.arange(-15, 17, dtype=torch.float32) * 0.5).clamp(-7, 7)     # every half step, of every scale M / 8
+    for i in range(8):
+        k[:, 8 + i, 0, :32] = (steps * (8 + i) / 8).to(dtype)
+    for r in range(rows):
+        k[r, counts[r]:], v[r, counts[r]:] = float("nan"), float("inf")
+    c.extend(torch.tensor(counts, dtype=torch.int32, device="cuda"))
+    c.append(0, k.cuda(), v.cuda())
+    c.check()
+    for out in (torch.float32, torch.bfloat16):
+        for x, got in zip((k, v), c.read(0, before, S + 3, dtype=out)):
+            got = got.double().cpu()
+            for r in range(rows):
+                want = K.dequantised(x[r, :counts[r]])
+                assert torch.equal(torch.isnan(got[r, :counts[r]]), torch.isnan(want))
+                assert torch.equal(got[r, :counts[r]].nan_to_num(0), want.nan_to_num(0)), (r, out)
+                assert (got[r, counts[r]:] == 0).all()
+    if before:
+        one = K.dequantised(torch.ones(32, dtype=dtype))[0]
+        assert all((x == one.float()).all() for x in c.read(0, 0, before, dtype=torch.float32))

@@ -199,6 +199,14 @@ def test_struct_layouts_match_the_header(tmp_path):
         assert all(got[(name, f)] == getattr(cls, f).offset for f, _ in cls._fields_)
 
 
+def test_more_positions_than_a_table_holds_are_refused():
+    lib, p = N.load(), 1 << 20
+    c = _native_cache()
+    for n in ((1 << 30) + 1, 2 ** 31 - 1):
+        assert lib.jx_kv4_append(c, 0, n, p, 0, 0, 1, p, 0, 0, 1, N.JX_BF16, None) == N.JX_ERR_SHAPE
+        assert lib.jx_kv4_read(c, 0, None, 0, n, p, p, N.JX_BF16, None) == N.JX_ERR_SHAPE
+
+
 # -- the format -------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("scale", [1e-39, 1e-30, 1e-3, 1.0, 1e4, 1e30])
 def test_values_are_exact_in_bfloat16_and_within_half_a_step(scale):
