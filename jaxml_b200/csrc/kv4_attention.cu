@@ -17,6 +17,10 @@
 //   V   one fused multiply-add a pair gives code times scale exactly (scaled2).
 // With more rows K is made exact the same way; float32 results need its codes exact before the product.
 //
+// Measured (B200, replayed from a graph): 32 rows of 8192 to 16384 tokens, 32 query heads on 8 of 128 features, bf16, 445 MB
+// of pages: 125 us, 3.6 TB/s; the copies alone take 87 us, the arithmetic alone some 120: 1430 warp instructions a page, of
+// which 800 turn codes into operands.  16 rows of 430 to 768 tokens 11 us, one row of 129 tokens 6.3 us.
+//
 // A page's block is one tensor-map box of 144 rows of hd / 2 bytes, swizzled by the copy so that ldmatrix gives every
 // thread its words of the key it owns without bank conflicts.
 #include <algorithm>

