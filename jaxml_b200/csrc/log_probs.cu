@@ -24,7 +24,6 @@
 namespace jxb {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kSlots = 32;        // batch maxima a thread keeps; a batch is 4 vectors times a whole number of rounds
 constexpr int kCand = 1024;       // elements above t that fit; more (all in a few batches) take the slow way
 constexpr int kMostTop = 64;
@@ -150,8 +149,9 @@ struct SlotKey<bf16> {
   static __device__ __forceinline__ uint32_t unpack(uint16_t k) { return (uint32_t)k << 16 | (k - 1u < 0x7FFFu ? 0xFFFFu : 0u); }
 };
 
-template <typename T>
+template <typename T, int kThreads>
 struct Shared {
+  static constexpr int kWarps = kThreads / 32;
   typename SlotKey<T>::type slot[kSlots][kThreads];   // order keys of the batches' maxima
   __align__(16) unsigned long long cand[kCand];       // order key << 32 | ~index
   unsigned long long list[kMostTop];                  // this CTA's best, in order
@@ -164,6 +164,7 @@ struct Shared {
 };
 
 // Exclusive sum over the CTA's threads.
+template <int kWarps>
 __device__ __forceinline__ int block_exclusive(int x, int* sh, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
@@ -186,7 +187,7 @@ __device__ __forceinline__ int block_exclusive(int x, int* sh, int* total) {
 }
 
 // The want-th largest of the maxima of kThreads / kEach groups of neighbouring threads (all threads; 1 <= want <= groups).
-template <int kEach>
+template <int kEach, int kThreads>
 __device__ __forceinline__ uint32_t nth_largest(uint32_t* best, uint32_t* bound, uint32_t mine, int want) {
   const int tid = threadIdx.x;
 #pragma unroll
@@ -211,18 +212,19 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t* best, uint32_t* bound,
 }
 
 // The top_n largest elements of the slice into s.list (all threads); n_list of them.
-template <typename T>
-__device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0, int v1, int rounds_per_slot, int slots, int top_n,
-                                        uint32_t mine) {
-  constexpr int kE = Row<T>::kE;
+template <typename T, int kThreads>
+__device__ __noinline__ void select_top(Shared<T, kThreads>& s, const Row<T>& row, int v0, int v1, int rounds_per_slot,
+                                        int slots, int top_n, uint32_t mine) {
+  constexpr int kE = Row<T>::kE, kWarps = kThreads / 32;
   const int tid = threadIdx.x;
   const int size = min(v1 * kE, row.last) - max(v0 * kE, row.first);   // elements of the slice
   const int want = min(top_n, max(size, 0));
   if (want == 0) return;
   // mine: the order key of the thread's maximum; 0, below that of -inf, without an element: with fewer threads at work than
   // elements wanted all elements count
-  // 64 groups are as good a bound for few elements and cost a sixteenth of the comparisons
-  const uint32_t t = want <= 32 ? nth_largest<4>(s.best, &s.bound, mine, want) : nth_largest<1>(s.best, &s.bound, mine, want);
+  // groups of 4 threads are as good a bound for few elements and cost a sixteenth of the comparisons
+  const uint32_t t = want <= kThreads / 8 ? nth_largest<4, kThreads>(s.best, &s.bound, mine, want)
+                                          : nth_largest<1, kThreads>(s.best, &s.bound, mine, want);
   const int per = rounds_per_slot;
   // This thread's elements of a slot that are at least `from`.  The comparisons go without branches and the few hits are
   // read again: this code runs once a row, and a short one costs its instruction fetches (a branch with its body for every
@@ -320,7 +322,7 @@ __device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0,
               if (at >= row.first && at < row.last && order_key(x[e]) == t) hit |= 1u << e;
             }
           }
-          int total, p = found + block_exclusive(__popc(hit), s.scan, &total);
+          int total, p = found + block_exclusive<kWarps>(__popc(hit), s.scan, &total);
           for (; hit && p < want; hit &= hit - 1, ++p)
             s.list[p] = ((unsigned long long)t << 32) | (uint32_t)~(v * kE + __ffs(hit) - 1 - row.first);
           found += total;
@@ -332,7 +334,7 @@ __device__ __noinline__ void select_top(Shared<T>& s, const Row<T>& row, int v0,
 }
 
 // Reads the slice: this thread's part of the sums; the batches' maxima where `slot` is given.
-template <typename T, bool kCareful>
+template <typename T, int kThreads, bool kCareful>
 __device__ __forceinline__ Sums stream(const Row<T>& row, int v0, int v1, int rounds, int per_slot, int slots,
                                        typename SlotKey<T>::type* slot) {
   constexpr int kE = Row<T>::kE;
@@ -435,16 +437,16 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int v0, int v1, int ro
   t.w = kCareful ? a0 + a1 : (a0 + a1) * 0.6931471805599453f;
   return t;
 }
-template <typename T>
+template <typename T, int kThreads>
 __device__ __noinline__ Sums stream_careful(const Row<T>& row, int v0, int v1, int rounds, int per_slot, int slots) {
-  return stream<T, true>(row, v0, v1, rounds, per_slot, slots, nullptr);
+  return stream<T, kThreads, true>(row, v0, v1, rounds, per_slot, slots, nullptr);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_probs_args a, int rounds_per_slot) {
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, 1024 / kThreads) log_probs_kernel(const jx_log_probs_args a, int rounds_per_slot) {
   extern __shared__ __align__(16) unsigned char smem[];
-  Shared<T>& s = *reinterpret_cast<Shared<T>*>(smem);
-  constexpr int kE = Row<T>::kE;
+  Shared<T, kThreads>& s = *reinterpret_cast<Shared<T, kThreads>*>(smem);
+  constexpr int kE = Row<T>::kE, kWarps = kThreads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = (int)cluster_nctarank(), rank = (int)cluster_ctarank();
   const int r = blockIdx.x / C;
@@ -465,9 +467,9 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_pro
     id = a.ids[r];
     if (id >= 0 && id < a.V) given = to_f(x[id]);
   }
-  Sums t = stream<T, false>(row, v0, v1, rounds, rounds_per_slot, slots, a.top_n ? &s.slot[0][0] : nullptr);
+  Sums t = stream<T, kThreads, false>(row, v0, v1, rounds, rounds_per_slot, slots, a.top_n ? &s.slot[0][0] : nullptr);
   if (__syncthreads_or(t.m != -INFINITY && !(fabsf(t.m) <= 8192.f)))
-    t = stream_careful<T>(row, v0, v1, rounds, rounds_per_slot, slots);
+    t = stream_careful<T, kThreads>(row, v0, v1, rounds, rounds_per_slot, slots);
   const uint32_t my_key = v0 + tid < v1 ? order_key(t.m) : 0u;
   const bool no_order = __syncthreads_or(t.m != t.m);    // NaN
 #pragma unroll
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_pro
     }
     if (lane == 0) s.mine = t;
   }
-  if (a.top_n && !no_order) select_top<T>(s, row, v0, v1, rounds_per_slot, slots, a.top_n, my_key);
+  if (a.top_n && !no_order) select_top<T, kThreads>(s, row, v0, v1, rounds_per_slot, slots, a.top_n, my_key);
   if (C > 1) {
     cluster_sync_all();
     if (rank == 0) {
@@ -551,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, 4) log_probs_kernel(const jx_log_pro
   }
 }
 
-template <typename T>
-int launch(const jx_log_probs_args& a, cudaStream_t s) {
+template <typename T, int kThreads>
+int launch_with(const jx_log_probs_args& a, cudaStream_t s) {
   // CTAs per row: as long as each has a multiprocessor to itself, and its slice two rounds of vectors.  128256 bfloat16
   // logits, top 20, 1 : 2 : 4 : 8 CTAs a row: 7 rows 16.7 : 13.7 : 12.8 : 13.6 us, 37 rows 17.3 : 14.4 : 15.0 : 18.5, 74 rows
   // 17.7 : 14.7 : 18.7 : 29.6, 148 rows 17.5 : 19.4 : 28.8 : 45.6.
@@ -563,12 +565,12 @@ int launch(const jx_log_probs_args& a, cudaStream_t s) {
   const long long per_cta = (nv + C - 1) / C;
   const long long rounds = (per_cta + 4 * kThreads - 1) / (4 * kThreads);
   const int per_slot = (int)((rounds + kSlots - 1) / kSlots);
-  const int smem = (int)sizeof(Shared<T>);
+  const int smem = (int)sizeof(Shared<T, kThreads>);
   static bool ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return JX_ERR_CUDA;
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    if (cudaFuncSetAttribute(log_probs_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return JX_ERR_CUDA;
+    if (cudaFuncSetAttribute(log_probs_kernel<T, kThreads>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return JX_ERR_CUDA;
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -580,7 +582,16 @@ int launch(const jx_log_probs_args& a, cudaStream_t s) {
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = C, at[0].val.clusterDim.y = 1, at[0].val.clusterDim.z = 1;
   cfg.attrs = at, cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, log_probs_kernel<T>, a, per_slot) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, log_probs_kernel<T, kThreads>, a, per_slot) == cudaSuccess ? JX_OK : JX_ERR_CUDA;
+}
+
+template <typename T>
+int launch(const jx_log_probs_args& a, cudaStream_t s) {
+  // 256 threads a row while all rows are resident at once (4 CTAs a multiprocessor), 128 above: twice the rows in a wave, so
+  // fewer of the waits at a row's end are waited for one after the other.  128256 bfloat16 logits, top 20, 256 : 128 threads:
+  // 148 rows 17.6 : 22.0 us, 592 rows 40.6 : 44.7, 700 rows 56.7 : 50.4, 1024 rows 71 : 64, 2000 rows 121 : 117; 5000 rows of
+  // 32000 139 : 110.
+  return a.rows > 4 * 148 ? launch_with<T, 128>(a, s) : launch_with<T, 256>(a, s);
 }
 
 }  // namespace

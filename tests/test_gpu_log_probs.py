@@ -151,3 +151,26 @@ def test_streams_graphs_and_repeats():
         zi.copy_(i)
         graph.replay()
         assert all(torch.equal(p, w) for p, w in zip(got, _run(src, i, 10)))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V,top_n", [(63, 63), (130, 64), (1003, 17), (5001, 16), (40000, 20), (20011, 0)])
+def test_more_rows_than_are_resident(dtype, V, top_n):
+    """Above 592 rows a row has fewer threads: random rows, rows full of ties, and rows that are hard, in between."""
+    N = 700
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(N, V, generator=g) * 4
+    x[1::5] = torch.round(x[1::5] * 0.5)                                     # many equal to the last one wanted
+    x[2::50], x[3::50] = 0.0, torch.linspace(-50, 50, V)
+    x[4::50, V // 2:], x[5::50, : V // 2] = x[4::50].amax(-1, keepdim=True), float("-inf")
+    x[6::50, :-1], x[7::50, V // 3], x[8::50, V // 3] = float("-inf"), float("nan"), float("inf")
+    x[9::50], x[10::50] = float("-inf"), torch.randn(V, generator=g) * 1e30
+    x[11::50, ::128] += 50
+    x[12::50, :100] += 50
+    x = x.to(dtype)
+    ids = torch.randint(-1, V + 1, (N,), generator=g, dtype=torch.int32)
+    got = _run(x.cuda(), ids.cuda(), top_n)
+    again = _run(x.cuda(), ids.cuda(), top_n)
+    assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(got, again))
+    some = torch.cat([torch.arange(0, 100), torch.arange(585, 605), torch.arange(690, 700)])
+    _check(x[some], ids[some], top_n, [t.cpu()[some] for t in got])
