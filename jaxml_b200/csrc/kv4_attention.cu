@@ -835,16 +835,18 @@ struct Layout {
   bool tc;               // 128 query rows a tile, on tcgen05
   long long items, first_at, part_at, bytes;
 };
-// Groups or equal runs. A group has no split to compute and no second launch; its CTAs have to be resident at once
-// (head_dim 64 and 128: two an SM, 256: one) and have few pages each, or equal runs over all of the GPU win. One row,
-// 32 query heads on 8 of 128 features, bf16, microseconds group : runs at 256, 768, 2000, 8000, 16000 cached tokens:
-// 6.4 : 10.8, 7.2 : 11.4, 8.4 : 12.6, 16 : 18.9, 26 : 28; 4 rows 6.8 : 11.2, 7.9 : 11.6, 10.6 : 13.2, 19.7 : 22.7,
-// 32 : 30; 16 rows 6.8 : 11.7, 11.6 : 13.2, and 25 : 21 at 2000; 64 rows 15 : 19, 27 : 30, and 62 : 51 at 2000. A cluster
-// larger than a wave of CTAs loses at once: 16 rows at 768 tokens take 17 with 512 CTAs, 11.6 with 256; 4 rows of 8 heads
-// of 256 features 25 with 256 CTAs, 10.2 with 128. Heads of 64 in fp32 cross over at the same places.
-constexpr int kGroupPages = 4;    // pages a CTA, as long as the wave has room for more CTAs
-constexpr int kGroupMost = 16;    // pages a CTA above which runs win
-constexpr int kGroupWave = 296;   // CTAs resident at once, head_dim 64 and 128
+// Groups or equal runs.  A group has no split to compute and no second launch; its clusters have to be resident at once and
+// its CTAs to have few pages each, or equal runs over all of the GPU win.  32 query heads on 8 of 128 features, bf16,
+// microseconds group : runs at 256, 768, 2000, 8000, 16000 cached tokens: one row 6.4 : 10.8, 7.2 : 11.4, 8.4 : 12.6,
+// 16 : 18.9, 26 : 28; 4 rows 6.8 : 11.2, 7.9 : 11.6, 10.6 : 13.2, 19.7 : 22.7, 32 : 30; 16 rows 6.8 : 11.7, 11.6 : 13.2, and
+// 25 : 21 at 2000; 64 rows 15 : 19, 27 : 30, and 62 : 51 at 2000.  With tiles of 16 query rows: one row 7.9 : 11.3, 9.5 : 11.9,
+// 10.9 : 13.2; 64 rows 29 : 34, and 52 : 47 at 768.  Clusters that do not fit at once cost twice: 16 rows at 768 tokens take 17
+// in clusters of 4, 11.6 in clusters of 2; 4 rows of tiles of 16 at 1020 tokens 26 in clusters of 8, 12.7 in runs.
+constexpr int kGroupPages = 4;    // pages a CTA, as long as there is room for larger clusters
+constexpr int kGroupMost = 16;    // pages a CTA above which runs win (half of it with tiles of 16 rows)
+// Clusters of 1, 2, 4 and 8 CTAs that 148 multiprocessors hold at once with one CTA each (head_dim 256, tiles of 16) and with
+// two: a cluster stays within a group of some 16 to 20 multiprocessors.
+constexpr int kGroupClusters[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};
 // bfloat16 rows of a KV head (S * G) from which they are 128 a tile on tcgen05, instead of tiles of 8 or 16 on mma.sync that
 // each read the pages: 12 rows of 2048 tokens, 8 of them in the batch, take 25.2 us against 24.4 (mma.sync), 16 rows 26.3
 // either way, 24 rows 27.4 against 45.8, 64 rows 35 against 64; 20 rows of 256 features 40 against 46.
@@ -863,10 +865,11 @@ Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int window, int dtype) {
   if (!l.tc) {
     long long pages = c.row_pages;                     // that a row can see
     if (window > 0) pages = std::min(pages, ((long long)window + S - 2) / kPage + 2);
-    const long long segs = l.items * c.num_kv_heads, wave = kGroupWave / (c.head_dim == 256 ? 2 : 1);
-    int cs = 1;
-    while (cs < 8 && pages > kGroupPages * cs && segs * cs * 2 <= wave) cs *= 2;
-    if (pages <= kGroupMost * cs) l.group = cs;
+    const long long segs = l.items * c.num_kv_heads;
+    const int two = l.nt == 1 && c.head_dim < 256;     // CTAs of a multiprocessor, less one
+    int step = 0;
+    while (step < 3 && pages > kGroupPages << step && segs <= kGroupClusters[two][step + 1]) ++step;
+    if (pages <= (l.nt == 1 ? kGroupMost : kGroupMost / 2) << step) l.group = 1 << step;
   }
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;

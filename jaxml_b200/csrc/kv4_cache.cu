@@ -117,7 +117,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   if (lead && blockIdx.x == 0 && cnt > a.S) set_status(c.status, JX_ERR_RANGE);
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int base = (first & ~(kTok - 1)) + tile * kTok, i0 = base - first;   // tokens i0 .. i0 + kTok - 1 of n
-    if (i0 >= n || i0 + kTok <= 0) continue;
+    if (i0 >= n) break;
+    if (i0 + kTok <= 0) continue;
     int page = -1;
     if (base >= 0 && base < c.row_pages * kPage) page = c.table[(long long)r * c.row_pages + base / kPage];
     if (page < 0 || page >= c.num_pages) {
@@ -179,7 +180,8 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const jx_kv4_cache c, int
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const long long base = (first & ~(long long)(kTok - 1)) + (long long)tile * kTok;
     const int i0 = (int)(base - first);
-    if (i0 >= n || i0 + kTok <= 0) continue;
+    if (i0 >= n) break;
+    if (i0 + kTok <= 0) continue;
     int page = -1;
     if (base >= 0 && base < len) {
       page = c.table[(long long)r * c.row_pages + base / kPage];
