@@ -850,27 +850,30 @@ constexpr int kGroupClusters[2][4] = {{148, 74, 33, 15}, {296, 148, 71, 33}};
 // bfloat16 rows of a KV head (S * G) from which they are 128 a tile on tcgen05, instead of tiles of 8 or 16 on mma.sync that
 // each read the pages: 12 rows of 2048 tokens, 8 of them in the batch, take 25.2 us against 24.4 (mma.sync), 16 rows 26.3
 // either way, 24 rows 27.4 against 45.8, 64 rows 35 against 64; 20 rows of 256 features 40 against 46.
-constexpr int kTcRows = 17;
+// Short rows stay in groups, tiles of 16, while there are few of them: 16 rows of 20 queries at 256 tokens, 256 CTAs, 15 us
+// against 24; one row of 64 queries at 512, 8 clusters, 9.5 against 13.4; 16 rows of 64, 512 CTAs, 20 : 20 at 128 tokens and
+// 23 : 28 at 256; 16 rows of 128, 1024 CTAs, 36 : 26.
+constexpr int kTcRows = 17, kGroupTiles = 512;
 constexpr int kMostCtas = 160, kMostWarps = 12;
 Layout layout_of(const jx_kv4_cache& c, int S, int Hq, int window, int dtype) {
   Layout l;
   const int G = Hq / c.num_kv_heads;
   const long long rows = (long long)S * G;
   l.nt = rows <= 8 ? 1 : 2;     // float32 tiles of 32 rows would not fit the registers
-  l.tc = dtype == JX_BF16 && rows >= kTcRows;
+  auto tiles = [&](int tile) { l.tiles = (int)((rows + tile - 1) / tile), l.items = (long long)c.num_rows * l.tiles; };
+  tiles(8 * l.nt);
+  long long pages = c.row_pages;                       // that a row can see
+  if (window > 0) pages = std::min(pages, ((long long)window + S - 2) / kPage + 2);
+  const long long segs = l.items * c.num_kv_heads;
+  const int two = l.nt == 1 && c.head_dim < 256;       // CTAs of a multiprocessor, less one
+  int step = 0;
+  while (step < 3 && pages > kGroupPages << step && segs <= kGroupClusters[two][step + 1]) ++step;
+  l.group = pages <= (l.nt == 1 ? kGroupMost : kGroupMost / 2) << step ? 1 << step : 0;
+  const bool many = dtype == JX_BF16 && rows >= kTcRows;
+  if (many && segs > kGroupTiles) l.group = 0;
+  l.tc = many && !l.group;
+  if (l.tc) tiles(128);
   const int tile = l.tc ? 128 : 8 * l.nt;
-  l.tiles = (int)((rows + tile - 1) / tile);
-  l.items = (long long)c.num_rows * l.tiles;
-  l.group = 0;
-  if (!l.tc) {
-    long long pages = c.row_pages;                     // that a row can see
-    if (window > 0) pages = std::min(pages, ((long long)window + S - 2) / kPage + 2);
-    const long long segs = l.items * c.num_kv_heads;
-    const int two = l.nt == 1 && c.head_dim < 256;     // CTAs of a multiprocessor, less one
-    int step = 0;
-    while (step < 3 && pages > kGroupPages << step && segs <= kGroupClusters[two][step + 1]) ++step;
-    if (pages <= (l.nt == 1 ? kGroupMost : kGroupMost / 2) << step) l.group = 1 << step;
-  }
   l.first_at = 16;
   l.part_at = (l.first_at + l.items * 8 + 15) / 16 * 16;
   const long long slots = l.tc ? 2ll * 2 * kMostCtas : 2ll * kMostCtas * kMostWarps;   // two for every run
