@@ -996,7 +996,7 @@ int launch_hd(const Layout& l, const AttendArgs& a, const CUtensorMap& map, cuda
 
 }  // namespace
 
-// Enough for any window: fewer pages never turn a group into runs.
+// Enough for any window: fewer pages turn runs and tiles of 128 into groups, which need none, and nothing else.
 long long kv4_attend_workspace(const jx_kv4_cache& c, int S, int Hq, int dtype) { return layout_of(c, S, Hq, 0, dtype).bytes; }
 
 int run_kv4_attend(const jx_kv4_cache& c, int layer, int S, int Hq, const void* q, const long long* qs, void* out,

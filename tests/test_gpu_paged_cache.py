@@ -692,3 +692,21 @@ def test_large_appends_are_exact(dtype, hd, heads, rows, S, before):
     if before:
         one = K.dequantised(torch.ones(32, dtype=dtype))[0]
         assert all((x == one.float()).all() for x in c.read(0, 0, before, dtype=torch.float32))
+
+
+@pytest.mark.parametrize("rows,hd", [(60, 64), (70, 128), (66, 256)])
+def test_many_short_chunks(rows, hd):
+    """Enough rows of a few queries that they share the tiles of 128, several (row, KV head) to a CTA: ragged counts, idle
+    and empty rows, one page and two."""
+    rng = random.Random(rows)
+    S, kv, heads = 9, 4, 8
+    counts = [rng.choice([0, 1, 5, 9, 9]) for _ in range(rows)]
+    lens = [n + rng.choice([0, 0, 3, 55, 60, 64]) for n in counts]
+    c, ks, vs = _filled(rows, lens, counts, kv, hd, seed=rows)
+    q = _rand((rows, S, heads, hd), torch.bfloat16, 5, 1.5)
+    for r, n in enumerate(counts):
+        q[r, n:] = float("nan")
+    for window in (0, 7):
+        got = c.attend(0, q.cuda(), sliding_window=window or None)
+        _check_attend(got, q, ks, vs, lens, counts, hd ** -0.5, window)
+    c.check()
