@@ -111,7 +111,7 @@ struct QPiece {
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
   }
   __device__ __forceinline__ void load_unaligned(const T* p) {
-    T x[8];
+    __align__(16) T x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = p[i];
 #pragma unroll
