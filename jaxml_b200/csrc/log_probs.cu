@@ -430,7 +430,9 @@ __device__ __forceinline__ Sums stream(const Row<T>& row, int v0, int v1, int ro
   Sums t;
   float a0, a1;
   t.m = m;
-  t.ref = kCareful ? (double)ref : (double)ref * 0.6931471805599453;
+  // K is m times the float32 constant, not times log2(e): its inverse takes it back.  ln 2 would leave 1.3e-8 of the row's level
+  // in every log probability (1.1e-4 at 8000).
+  t.ref = kCareful ? (double)ref : (double)ref * (1.0 / (double)kLog2e);
   unpack2(z2, a0, a1);
   t.z = a0 + a1;
   unpack2(w2, a0, a1);

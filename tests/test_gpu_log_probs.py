@@ -174,3 +174,21 @@ def test_more_rows_than_are_resident(dtype, V, top_n):
     assert all(torch.equal(a.nan_to_num(7), b.nan_to_num(7)) for a, b in zip(got, again))
     some = torch.cat([torch.arange(0, 100), torch.arange(585, 605), torch.arange(690, 700)])
     _check(x[some], ids[some], top_n, [t.cpu()[some] for t in got])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N", [1, 700])
+@pytest.mark.parametrize("level", [30.0, -100.0, 1000.0, -1000.0, 8000.0, -8000.0])
+def test_the_level_of_a_row_does_not_matter(dtype, N, level):
+    """A softmax does not change with a constant added to its row: the same tolerance at every level, on random rows and
+    on rows with one entry far above the others (log p = 0 there, never above it by more than the tolerance)."""
+    V, g = 5003, torch.Generator().manual_seed(int(abs(level)))
+    x = torch.randn(N, V, generator=g) * 3 + level
+    x[::2, 77] = level + 150
+    x = x.to(dtype)
+    ids = torch.randint(0, V, (N,), generator=g, dtype=torch.int32)
+    ids[::2] = 77
+    got = _run(x.cuda(), ids.cuda(), 5)
+    some = torch.arange(min(N, 40))
+    _check(x[some], ids[some], 5, [t.cpu()[some] for t in got])
+    assert (got.log_probs[::2].cpu() <= 2.0 ** -22 + (V / 128 + 64) * 2.0 ** -24).all()
