@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
           const bool live = f < F && s < at.t.cnt;
           hi = live ? at.t.base + s : -1;
           lo = live && a.window > 0 ? max(0, hi - a.window + 1) : 0;
-          // what rows that are not there make of a page does not matter: their results are zeros
+          // what rows that are not there make of a page does not matter: zeros are written for them
           all_hi = at.t.base + f0 / a.G;
           all_lo = a.window > 0 ? at.t.base + (f0 + kRows - 1) / a.G - a.window : -1;
           m = -INFINITY, l = 0.f, nan_groups = 0;
@@ -593,7 +593,8 @@ __global__ void __launch_bounds__(kThreads, Tc<HD>::kCtas)
                 float y[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  y[e] = (nan_groups >> part) & 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float(r[k + e]) * inv;
+                  y[e] = hi < 0 ? 0.f        // padding: a visible key of NaN makes its O NaN, which times 0 stays
+                         : (nan_groups >> part) & 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float(r[k + e]) * inv;
                 if (whole) store_row8<bf16>(o + part * 32 + k, y);
                 else
 #pragma unroll

@@ -710,3 +710,34 @@ def test_many_short_chunks(rows, hd):
         got = c.attend(0, q.cuda(), sliding_window=window or None)
         _check_attend(got, q, ks, vs, lens, counts, hd ** -0.5, window)
     c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,kv,hd,S,room", [(2, 2, 64, 70, 500), (2, 2, 128, 70, 500), (3, 1, 256, 40, 500), (2, 2, 128, 70, 0),
+                                               (90, 4, 64, 9, 0), (90, 4, 128, 9, 500), (4, 2, 64, 3, 0), (4, 2, 64, 3, 500)])
+def test_padding_is_zero_beside_a_nan(dtype, rows, kv, hd, S, room):
+    """Queries behind a row's counts are zeros also where a key or value that lies whole pages before the chunk decodes to
+    NaN and the tile's other queries see it."""
+    heads, before = 2 * kv, 200
+    counts = [max(0, S - 1 - r % S) for r in range(rows)]
+    width = -(-(before + S) // PAGE)
+    c = _cache(1, rows * width, rows, (width + room) * PAGE, kv, hd)
+    k, v = _rand((rows, before, kv, hd), torch.float32, 1), _rand((rows, before, kv, hd), torch.float32, 2)
+    k[:, 5, 0, 3] = float("nan")
+    v[:, 150, kv - 1, 40] = float("inf")
+    c.extend(before)
+    c.append(0, k.cuda(), v.cuda())
+    c.extend(torch.tensor(counts, dtype=torch.int32, device="cuda"))
+    x = _rand((rows, S, kv, hd), torch.float32, 3).cuda()
+    c.append(0, x, x)
+    q = _rand((rows, S, heads, hd), dtype, 4).cuda()
+    for window in (None, 190):
+        got = c.attend(0, q, sliding_window=window).cpu()
+        sees = window is None
+        for r, n in enumerate(counts):
+            assert (got[r, n:] == 0).all(), (r, n)
+            first, last = got[r, :n, :2], got[r, :n, -2:]
+            if sees:
+                assert torch.isnan(first).all()
+            assert torch.isnan(last[..., 32:64]).all() and (kv == 1 or torch.isfinite(last[..., :32]).all())
+    c.check()
