@@ -192,7 +192,8 @@ class _DecoderWithHead:
     def _paged_stack(self, params, input_ids, attention_mask, position_ids, cache, use_cache, output_attentions,
                      output_hidden_states):
         """The stack over a ``PagedKVCache``: the mask's tokens of every row (a prompt, a chunk of one, or single
-        tokens, also on rows that hold tokens already) are added to the cache, which changes in place."""
+        tokens, also on rows that hold tokens already) are added to the cache, which changes in place.  A call that
+        raises leaves the rows' lengths and contents as they were."""
         from .decoders import layered_forward
 
         cfg = self.config
@@ -211,12 +212,17 @@ class _DecoderWithHead:
         counts = mask.to(device=dev, dtype=torch.int32).sum(dim=1, dtype=torch.int32)
         if bool((cache.lengths + counts > cfg.max_position_embeddings).any()):
             raise ValueError(f"rows of the paged cache must stay within max_position_embeddings={cfg.max_position_embeddings}.")
+        cache.check()           # what an earlier call left is raised before the rows change
         cache.extend(counts)
         cache.check()
-        h, _, states, _ = layered_forward(
-            self.family, cfg, self.dtype, body, ids.to(dev), mask.to(dev),
-            cache.position_ids(ids.shape[1]) if cfg.use_rope else None,
-            tuple(cache.layer(i) for i in range(cfg.num_layers)), None, self.__dict__["_layered_cache"]["rope"])
+        try:
+            h, _, states, _ = layered_forward(
+                self.family, cfg, self.dtype, body, ids.to(dev), mask.to(dev),
+                cache.position_ids(ids.shape[1]) if cfg.use_rope else None,
+                tuple(cache.layer(i) for i in range(cfg.num_layers)), None, self.__dict__["_layered_cache"]["rope"])
+        except BaseException:
+            cache.rollback(counts)      # some layers have not written their pages: the rows end where they did
+            raise
         return h, cache if use_cache else None, states if output_hidden_states else None, None, False
 
     _has_head = True

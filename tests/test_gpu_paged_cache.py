@@ -741,3 +741,40 @@ def test_padding_is_zero_beside_a_nan(dtype, rows, kv, hd, S, room):
                 assert torch.isnan(first).all()
             assert torch.isnan(last[..., 32:64]).all() and (kv == 1 or torch.isfinite(last[..., :32]).all())
     c.check()
+
+
+@pytest.mark.parametrize("how", ["an earlier error", "no room", "a layer raises"])
+def test_a_model_call_that_fails_leaves_the_rows(how, monkeypatch):
+    """What apply raises over a paged cache, it raises with the rows as they were: an error that an earlier call left on the
+    device, a pool that is full, a layer that fails half way."""
+    from jaxml_b200 import PagedKVCache, decoders
+
+    model, params = _tiny("llama")
+    cfg = model.config
+    ids = torch.randint(0, cfg.vocab_size, (2, 70), generator=torch.Generator().manual_seed(0), dtype=torch.int32)
+    new = lambda: PagedKVCache.init(cfg.num_layers, 6, 2, 256, cfg.num_key_value_heads, 64)  # noqa: E731
+    c, want = new(), new()
+    for x in (c, want):
+        model.apply(params, ids, kv_caches=x)
+    state = [t.clone() for t in (c.table, c.lengths, c.refs)]
+    if how == "an earlier error":
+        c.rollback(10 ** 6)
+        with pytest.raises(RuntimeError, match="device status"):
+            model.apply(params, ids[:, :60], kv_caches=c)
+    elif how == "no room":
+        with pytest.raises(RuntimeError, match="no room"):
+            model.apply(params, torch.cat([ids, ids], 1), kv_caches=c)
+    else:
+        real = decoders.layered_forward
+
+        def half(family, cfg, *args, **kw):
+            real(family, cfg, *args, **kw)
+            raise OSError("a layer")
+
+        monkeypatch.setattr(decoders, "layered_forward", half)
+        with pytest.raises(OSError, match="a layer"):
+            model.apply(params, ids[:, :60], kv_caches=c)
+        monkeypatch.setattr(decoders, "layered_forward", real)
+    assert all(torch.equal(a, b) for a, b in zip(state, (c.table, c.lengths, c.refs)))
+    a, b = (model.apply(params, ids[:, :60], kv_caches=x).logits for x in (c, want))
+    assert torch.equal(a, b) and c.lengths.tolist() == [130, 130]
