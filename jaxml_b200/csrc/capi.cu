@@ -420,6 +420,16 @@ static int kv4_fail(int code, const char* where, const char* msg) {
   return code;
 }
 
+// Whether a call's row vector lies in memory that the call changes while it is read.  `whole`: the cache's own lengths or counts,
+// from their first entry, are fine (a row's entries are read before they are written).
+static bool kv4_in_state(const jx_kv4_cache& c, const void* p, long long bytes, bool whole) {
+  if (!p || (whole && (p == c.lengths || p == c.counts))) return false;
+  const uintptr_t from = (uintptr_t)p, to = from + bytes;
+  auto meets = [&](const void* q, long long n) { return from < (uintptr_t)q + n && (uintptr_t)q < to; };
+  return meets(c.table, 4ll * c.num_rows * c.row_pages) || meets(c.lengths, 4ll * c.num_rows) || meets(c.counts, 4ll * c.num_rows) ||
+         meets(c.refs, 4ll * c.num_pages) || meets(c.status, 4);
+}
+
 static int kv4_done(int rc, const char* where) { return rc == JX_ERR_CUDA ? note_cuda(where) : rc; }
 }  // namespace jxb
 
@@ -496,24 +506,32 @@ int jx_kv4_extend(const jx_kv4_cache* cache, const int* counts, int count, int* 
   if (!counts && count < 0) return fail(JX_ERR_SHAPE, "jx_kv4_extend: count must not be negative");
   if (!ws || ws_ints < kv4_workspace_ints(cache->num_rows, cache->num_pages))
     return fail(JX_ERR_ARG, "jx_kv4_extend: workspace too small");
+  if (kv4_in_state(*cache, counts, 4ll * cache->num_rows, true))
+    return fail(JX_ERR_ARG, "jx_kv4_extend: counts must not lie in the cache's own state, but be its lengths or counts");
   return kv4_done(run_kv4_extend(*cache, counts, count, ws, (cudaStream_t)stream), "jx_kv4_extend");
 }
 
 int jx_kv4_fork(const jx_kv4_cache* cache, const int* parents, void* stream) {
   KV4_CHECK("jx_kv4_fork");
   if (!parents) return fail(JX_ERR_ARG, "jx_kv4_fork: null parents");
+  if (kv4_in_state(*cache, parents, 4ll * cache->num_rows, false))
+    return fail(JX_ERR_ARG, "jx_kv4_fork: parents must not lie in the cache's own state");
   return kv4_done(run_kv4_fork(*cache, parents, (cudaStream_t)stream), "jx_kv4_fork");
 }
 
 int jx_kv4_rollback(const jx_kv4_cache* cache, const int* n, int n_all, void* stream) {
   KV4_CHECK("jx_kv4_rollback");
   if (!n && n_all < 0) return fail(JX_ERR_SHAPE, "jx_kv4_rollback: n must not be negative");
+  if (kv4_in_state(*cache, n, 4ll * cache->num_rows, true))
+    return fail(JX_ERR_ARG, "jx_kv4_rollback: n must not lie in the cache's own state, but be its lengths or counts");
   return kv4_done(run_kv4_shorten(*cache, nullptr, n, n_all, (cudaStream_t)stream), "jx_kv4_rollback");
 }
 
 int jx_kv4_free(const jx_kv4_cache* cache, const unsigned char* rows, void* stream) {
   KV4_CHECK("jx_kv4_free");
   if (!rows) return fail(JX_ERR_ARG, "jx_kv4_free: null rows");
+  if (kv4_in_state(*cache, rows, cache->num_rows, false))
+    return fail(JX_ERR_ARG, "jx_kv4_free: rows must not lie in the cache's own state");
   return kv4_done(run_kv4_shorten(*cache, rows, nullptr, 0, (cudaStream_t)stream), "jx_kv4_free");
 }
 

@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_extend_plan_kernel(const jx_
     const int at = pages_of(len), fresh = cnt > 0 ? pages_of(len + cnt) - at : 0;
     const int base = p.need[r], end = r + 1 < R ? p.need[r + 1] : total;
     const int copy = end - base - fresh;
+    __syncwarp();     // counts may be the cache's own counts or lengths: all lanes have read them before lane 0 writes
     int* row = c.table + (long long)r * c.row_pages;
     for (int j = lane; j < fresh; j += 32) {
       const int page = p.list[base + copy + j];

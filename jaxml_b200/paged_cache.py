@@ -21,7 +21,8 @@ zero tokens of the current call.
 The format is 4.5 bits a value: 4-bit integers -7..7 with one scale of 4 significant bits for every 32 neighbouring
 channels of a token (``include/jxb200.h``).  A group with a non-finite value, or one of magnitude 2^122 or more, decodes
 to NaN.  Calls on one cache that change it must be ordered on the device like writes to any tensor; ``attend`` and
-``read`` may run at the same time.  ``lengths`` and ``counts`` may be read, not written.
+``read`` may run at the same time.  ``lengths`` and ``counts`` may be read, not written, and be given to ``extend`` and
+``rollback``; other arguments must not lie in the cache's own tensors.
 """
 from __future__ import annotations
 

@@ -778,3 +778,27 @@ def test_a_model_call_that_fails_leaves_the_rows(how, monkeypatch):
     assert all(torch.equal(a, b) for a, b in zip(state, (c.table, c.lengths, c.refs)))
     a, b = (model.apply(params, ids[:, :60], kv_caches=x).logits for x in (c, want))
     assert torch.equal(a, b) and c.lengths.tolist() == [130, 130]
+
+
+def test_the_caches_own_lengths_and_counts_as_arguments():
+    """extend and rollback by the lengths or counts of the cache itself are what they are by a copy of them."""
+    rows = 40
+    lens = [(37 * r) % 150 for r in range(rows)]
+
+    def new():
+        c = _cache(1, 8 * rows, rows, 10 * PAGE, 1, 64)
+        c.extend(lens)
+        c.fork([r - r % 3 for r in range(rows)])          # shared last pages
+        c.extend([r % 4 for r in range(rows)])
+        return c
+
+    for name in ("lengths", "counts"):
+        for call in ("extend", "rollback"):
+            a, b = new(), new()
+            getattr(a, call)(getattr(a, name))
+            getattr(b, call)(getattr(b, name).clone())
+            a.check()
+            b.check()
+            assert all(torch.equal(getattr(a, x), getattr(b, x)) for x in ("table", "lengths", "counts", "refs")), (name, call)
+            with pytest.raises(RuntimeError, match="own state"):
+                a.fork(getattr(a, name))

@@ -264,3 +264,19 @@ def test_page_management_keeps_what_rows_wrote():
             used = c.compact()
             assert all(p < used for t in c.table for p in t)
         assert [c.row(r) for r in range(R)] == rows
+
+
+def test_row_vectors_in_the_caches_own_state_are_refused():
+    """A call changes the table, the lengths, the counts and the holders while it reads its row vector."""
+    lib, A = N.load(), N.JX_ERR_ARG
+    at = dict(table=0x10000, lengths=0x20000, counts=0x30000, refs=0x40000, status=0x50000)
+    c = _native_cache(num_rows=8, num_pages=100, row_pages=3, **at)
+    inside = [at["table"], at["table"] + 4 * 8 * 3 - 4, at["table"] - 4, at["lengths"] + 4, at["lengths"] - 4, at["counts"] + 28,
+              at["refs"], at["refs"] + 396, at["status"], at["status"] - 28]
+    for p in inside:
+        assert lib.jx_kv4_extend(c, p, 0, 0x60000, 1 << 40, None) == A, hex(p)
+        assert lib.jx_kv4_rollback(c, p, 0, None) == A and lib.jx_kv4_fork(c, p, None) == A, hex(p)
+    for p in (at["lengths"], at["counts"]):
+        assert lib.jx_kv4_fork(c, p, None) == A
+    for p in (at["table"] - 7, at["refs"] + 399, at["status"] + 3, at["counts"]):
+        assert lib.jx_kv4_free(c, p, None) == A, hex(p)
