@@ -493,9 +493,9 @@ int jx_allreduce_f32(void* const* bases, int rank, int world, long long max_floa
  * clamp(round(x / scale), -7, 7); a group of magnitude 2^122 or more, or not finite, decodes to NaN.
  *
  * Device errors (a row past its table, a pool without free pages, a parent or page out of range) set *status to
- * JX_ERR_RANGE; nothing is read or written out of range.  hd is 64, 128 or 256; at most 8192 rows.  The row vectors that
- * extend, fork, rollback and free take must not lie in the cache's own state; lengths or counts themselves may be given to
- * extend and rollback. */
+ * JX_ERR_RANGE; nothing is read or written out of range.  hd is 64, 128 or 256; at most 8192 rows, 2^24 pages a row and
+ * 2^31 - 1 table entries.  The row vectors that extend, fork, rollback and free take must not lie in the cache's own state;
+ * lengths or counts themselves may be given to extend and rollback. */
 #define JX_KV4_PAGE 64
 typedef struct jx_kv4_cache {
   unsigned char* pages;  /* [num_layers][num_pages][num_kv_heads][72 * head_dim], 16-byte aligned */

@@ -409,6 +409,8 @@ static const char* kv4_bad(const jx_kv4_cache* c, int* code) {
     return "cache sizes must be positive";
   if (c->num_rows > 8192) return "at most 8192 rows";
   if (c->row_pages > (1 << 24)) return "at most 2^24 pages per row";
+  // the pages that all rows ask for are counted in 32 bits
+  if ((long long)c->num_rows * c->row_pages > 0x7FFFFFFF) return "the table must have fewer than 2^31 entries";
   if (c->num_pages > (1 << 28) || c->num_kv_heads > 4096) return "at most 2^28 pages and 4096 KV heads";
   if ((long long)c->num_layers * c->num_pages * c->num_kv_heads > 0x7FFFFFFF) return "layers * pages * KV heads must be below 2^31";
   if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return "head_dim must be 64, 128 or 256";

@@ -280,3 +280,14 @@ def test_row_vectors_in_the_caches_own_state_are_refused():
         assert lib.jx_kv4_fork(c, p, None) == A
     for p in (at["table"] - 7, at["refs"] + 399, at["status"] + 3, at["counts"]):
         assert lib.jx_kv4_free(c, p, None) == A, hex(p)
+
+
+def test_a_table_of_more_entries_than_32_bits_count_is_refused():
+    """Rows could ask for more pages than an int holds, and the plan of an extend would place them outside its list."""
+    lib, p, n = N.load(), 1 << 12, N.LL()
+    for rows, row_pages in ((8192, 1 << 24), (128, 1 << 24), (8192, 1 << 18)):
+        c = _native_cache(num_rows=rows, row_pages=row_pages)
+        assert lib.jx_kv4_workspace_ints(c, n) == N.JX_ERR_SHAPE
+        assert b"2^31" in lib.jx_last_error()
+        assert lib.jx_kv4_extend(c, None, 1, p, 1 << 40, None) == N.JX_ERR_SHAPE
+    assert lib.jx_kv4_workspace_ints(_native_cache(num_rows=127, row_pages=1 << 24), n) == N.JX_OK
