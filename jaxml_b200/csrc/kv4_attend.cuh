@@ -60,9 +60,10 @@ template <int kRows>
 __device__ __forceinline__ Item item_at(const AttendArgs& a, long long item) {
   Item t;
   t.r = (int)(item / a.tiles), t.qt = (int)(item - (long long)t.r * a.tiles);
-  t.cnt = min(a.c.counts[t.r], a.S);
-  const int len = min(a.c.lengths[t.r], a.c.row_pages * kPage);
-  t.base = len - a.c.counts[t.r];
+  // both may be anything in a cache made of given tensors: a difference of two that are not negative does not wrap
+  const int cnt = max(a.c.counts[t.r], 0), len = min(max(a.c.lengths[t.r], 0), a.c.row_pages * kPage);
+  t.cnt = min(cnt, a.S);
+  t.base = len - cnt;
   const int s0 = t.qt * kRows / a.G, s1 = min(min(t.qt * kRows + kRows, a.S * a.G) - 1, t.cnt * a.G - 1) / a.G;
   t.n = 0, t.p0 = 0;
   if (s0 < t.cnt && t.base >= 0) {

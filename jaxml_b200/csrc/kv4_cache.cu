@@ -113,7 +113,10 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendArgs a) {
   const int which = live && it >= half, head = live ? (it - which * half) / kPer : 0, ch = it % kPer;
   const T* src = static_cast<const T*>(a.src[which]) + head * a.head[which] + ch * 8;
   const long long tok = a.tok[which];
-  const int r = blockIdx.z, cnt = c.counts[r], first = c.lengths[r] - cnt, n = min(cnt, a.S);
+  // a cache made of given tensors may hold any length: first is kept where sums with positions do not wrap, and so that no
+  // position below the row's end is another's
+  const int r = blockIdx.z, cnt = max(c.counts[r], 0), n = min(cnt, a.S);
+  const int first = min(max(c.lengths[r], 0) - cnt, c.row_pages * kPage);
   if (lead && blockIdx.x == 0 && cnt > a.S) set_status(c.status, JX_ERR_RANGE);
   for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int base = (first & ~(kTok - 1)) + tile * kTok, i0 = base - first;   // tokens i0 .. i0 + kTok - 1 of n
@@ -484,9 +487,11 @@ __global__ void __launch_bounds__(128) kv4_shorten_kernel(const jx_kv4_cache c, 
                                                           int n_all) {
   const int r = blockIdx.x;
   if (rows && !rows[r]) return;
-  const int len = c.lengths[r], cut = rows ? len : (n ? n[r] : n_all), held = min(pages_of(max(len, 0)), c.row_pages);
+  // a length that no row can have (a cache made of given tensors) is only emptied: pages_of wraps near 2^31
+  const int len = c.lengths[r], cut = rows ? len : (n ? n[r] : n_all), most = c.row_pages * kPage;
+  const int held = pages_of(min(max(len, 0), most));
   __syncthreads();
-  if (cut < 0 || cut > len) {
+  if (cut < 0 || cut > len || (len > most && cut < len)) {
     if (threadIdx.x == 0) {
       c.counts[r] = 0;
       set_status(c.status, JX_ERR_RANGE);

@@ -802,3 +802,28 @@ def test_the_caches_own_lengths_and_counts_as_arguments():
             assert all(torch.equal(getattr(a, x), getattr(b, x)) for x in ("table", "lengths", "counts", "refs")), (name, call)
             with pytest.raises(RuntimeError, match="own state"):
                 a.fork(getattr(a, name))
+
+
+@pytest.mark.parametrize("length", [4 * PAGE + 1, 2 ** 31 - 64, 2 ** 31 - 62, 2 ** 31 - 1, -1, -2 ** 31])
+def test_lengths_that_no_row_can_have(length):
+    """A cache made of given tensors may hold anything: such a row is reported, nothing out of range is touched, and free
+    empties it where its length is positive."""
+    c, ks, vs = _filled(3, [100, 200, 256], [1, 1, 1], 2, 64, seed=4)
+    assert c.row_pages == 4
+    c.lengths[1] = length
+    q = _rand((3, 1, 4, 64), torch.bfloat16, 5).cuda()
+    table, refs = c.table.clone(), c.refs.clone()
+    assert torch.isfinite(c.attend(0, q)[[0, 2]]).all()
+    c.append(0, q[:, :, :2], q[:, :, :2])
+    assert (c.read(0, 300, 8)[0] == 0).all()
+    c.status.zero_()
+    for call in (lambda: c.extend(1), lambda: c.rollback([0, 1, 0]), lambda: c.rollback([0, 70, 0]), lambda: c.rollback([0, -1, 0])):
+        call()
+        with pytest.raises(RuntimeError, match="device status 4"):
+            c.check()
+        assert torch.equal(c.table, table) and torch.equal(c.refs, refs)
+        assert c.lengths.tolist() == [100, length, 256] and c.counts[1] == 0
+    c.free([1])
+    if length > 0:
+        c.check()
+        assert c.lengths.tolist() == [100, 0, 256] and (c.table[1] == -1).all() and int(c.refs.sum()) == 6
