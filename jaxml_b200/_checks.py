@@ -66,3 +66,13 @@ def normalize_dtype(name: str, value: Any) -> torch.dtype:
 
 def dtype_name(dtype: torch.dtype) -> str:
     return {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16"}[dtype]
+
+
+def widened(x: torch.Tensor) -> torch.Tensor:
+    """An unsigned 32- or 64-bit tensor as int64, values that do not fit at the largest; others as they are."""
+    if x.dtype == torch.uint32:
+        return x.to(torch.int64)
+    if x.dtype == torch.uint64:
+        x = x.to(torch.int64)
+        return torch.where(x < 0, 2 ** 63 - 1, x)
+    return x

@@ -32,7 +32,7 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from ._checks import normalize_count, normalize_float
+from ._checks import normalize_count, normalize_float, widened
 
 __all__ = ["PagedKVCache", "PagedKVLayer"]
 
@@ -179,6 +179,7 @@ class PagedKVCache:
             raise ValueError(f"{name} must have shape ({self.num_rows},), got {tuple(x.shape)}.")
         if x.dtype == torch.int32 and x.device == self.device and x.is_contiguous():
             return x
+        x = widened(x)
         if x.dtype == torch.int64:
             x = x.clamp(-2 ** 31, 2 ** 31 - 1)
         return x.to(device=self.device, dtype=torch.int32).contiguous()

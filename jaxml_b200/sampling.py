@@ -23,7 +23,7 @@ import numpy as np
 
 import torch
 
-from ._checks import normalize_bool, normalize_count
+from ._checks import normalize_bool, normalize_count, widened
 
 logger = logging.getLogger(__name__)
 
@@ -309,6 +309,7 @@ def token_log_probs(logits: torch.Tensor, token_ids, top_n: int = 0) -> TokenLog
     if ids.shape != lead:
         raise ValueError(f"token_ids must have the logits' leading shape {tuple(lead)}, got {tuple(ids.shape)}.")
     if ids.dtype != torch.int32 or ids.device != dev or not ids.is_contiguous():
+        ids = widened(ids)
         if ids.dtype == torch.int64:
             ids = ids.clamp(-1, V)      # before the narrowing: a wrapped id would be another token's
         ids = ids.to(device=dev, dtype=torch.int32).contiguous()

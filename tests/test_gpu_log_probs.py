@@ -7,6 +7,7 @@ The entropy adds the same relative error of sum p |d|, d the distance to the max
 """
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -192,3 +193,14 @@ def test_the_level_of_a_row_does_not_matter(dtype, N, level):
     some = torch.arange(min(N, 40))
     _check(x[some], ids[some], 5, [t.cpu()[some] for t in got])
     assert (got.log_probs[::2].cpu() <= 2.0 ** -22 + (V / 128 + 64) * 2.0 ** -24).all()
+
+
+def test_unsigned_ids_do_not_wrap():
+    """An id of 2^32 - 1 is beyond the vocabulary (NaN), not the negative id that asks for nothing (0)."""
+    x = torch.randn(2, 10, generator=torch.Generator().manual_seed(0)).cuda()
+    want = _run(x, [3, 4], 0).log_probs
+    for dtype, big in ((np.uint32, 2 ** 32 - 1), (np.uint64, 2 ** 64 - 1), (np.uint64, 2 ** 32 + 3)):
+        for dev in ("cpu", "cuda"):
+            got = _run(x, torch.from_numpy(np.array([big, 4], dtype=dtype)).to(dev), 0).log_probs
+            assert torch.isnan(got[0]) and got[1] == want[1], (dtype, dev)
+            assert torch.equal(_run(x, torch.from_numpy(np.array([3, 4], dtype=dtype)).to(dev), 0).log_probs, want)

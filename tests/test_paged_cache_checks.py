@@ -3,6 +3,7 @@ of the number format and of the page management that the device tests rely on.""
 import ctypes
 import random
 
+import numpy as np
 import pytest
 import torch
 
@@ -291,3 +292,13 @@ def test_a_table_of_more_entries_than_32_bits_count_is_refused():
         assert b"2^31" in lib.jx_last_error()
         assert lib.jx_kv4_extend(c, None, 1, p, 1 << 40, None) == N.JX_ERR_SHAPE
     assert lib.jx_kv4_workspace_ints(_native_cache(num_rows=127, row_pages=1 << 24), n) == N.JX_OK
+
+
+@pytest.mark.parametrize("dtype,big", [(torch.uint32, 2 ** 32 - 1), (torch.uint32, 2 ** 31), (torch.uint64, 2 ** 64 - 1),
+                                       (torch.uint64, 2 ** 63), (torch.uint64, 2 ** 32 + 1), (torch.int64, 2 ** 32 + 1)])
+def test_unsigned_row_vectors_do_not_wrap(dtype, big):
+    """A parent of 2^32 - 1 is out of range; narrowed bit by bit it would be -1, which empties the row."""
+    t = torch.from_numpy(np.array([big, 1], dtype=str(dtype).split(".")[1]))
+    assert t.dtype == dtype and _cpu_cache()._row_ints("parents", t).tolist() == [2 ** 31 - 1, 1]
+    small = torch.tensor([3, 1]).to(dtype)
+    assert _cpu_cache()._row_ints("parents", small).tolist() == [3, 1]
