@@ -29,6 +29,7 @@ from __future__ import annotations
 import ctypes
 from typing import Optional
 
+import numpy as np
 import torch
 
 from . import _native as N
@@ -196,7 +197,7 @@ class PagedKVCache:
         """Begins a call of ``counts`` more tokens of every row (an int, or int32 [rows]; 0 leaves a row out): the rows
         grow, new pages are taken and shared pages that will be written on are copied.  Without room nothing
         changes, ``counts`` becomes zero and ``check`` raises."""
-        if isinstance(counts, torch.Tensor) or not hasattr(counts, "__index__"):
+        if _is_vector(counts):
             c, n = self._row_ints("counts", counts), 0
         else:
             c, n = None, normalize_count("counts", counts)
@@ -225,7 +226,7 @@ class PagedKVCache:
         if dtype not in _DTYPES:
             raise TypeError(f"dtype must be float32 or bfloat16, got {dtype}.")
         length = self.max_seq_len if length is None else _positive("length", length)
-        if isinstance(start, torch.Tensor) or not hasattr(start, "__index__"):
+        if _is_vector(start):
             ptr, add = self._row_ints("start", start), 0
         else:
             ptr, add = None, normalize_count("start", start)
@@ -281,7 +282,7 @@ class PagedKVCache:
     def rollback(self, n) -> None:
         """Every row loses its last ``n`` tokens (an int, or int32 [rows]); pages that held nothing else are given back.  A
         row of fewer tokens stays as it is and ``check`` raises."""
-        if isinstance(n, torch.Tensor) or not hasattr(n, "__index__"):
+        if _is_vector(n):
             t, n = self._row_ints("n", n), 0
         else:
             t, n = None, normalize_count("n", n)
@@ -345,6 +346,11 @@ class PagedKVLayer:
     def update_and_attend(self, q, k, v, scale: float, sliding_window: Optional[int]) -> torch.Tensor:
         self.cache.append(self.index, k, v)
         return self.cache.attend(self.index, q, scale=scale, sliding_window=sliding_window)
+
+
+def _is_vector(x) -> bool:
+    """Whether an argument is one value for every row (arrays too have ``__index__``)."""
+    return not hasattr(x, "__index__") or isinstance(x, (torch.Tensor, np.ndarray))
 
 
 def _what(x) -> str:

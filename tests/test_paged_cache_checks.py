@@ -302,3 +302,18 @@ def test_unsigned_row_vectors_do_not_wrap(dtype, big):
     assert t.dtype == dtype and _cpu_cache()._row_ints("parents", t).tolist() == [2 ** 31 - 1, 1]
     small = torch.tensor([3, 1]).to(dtype)
     assert _cpu_cache()._row_ints("parents", small).tolist() == [3, 1]
+
+
+def test_numpy_row_vectors_are_taken_as_lists_are():
+    c = _cpu_cache()
+    for call in (c.extend, c.rollback, c.fork, lambda x: c.read(0, x, 1)):
+        for x in ([1, 0], np.array([1, 0]), np.array([1, 0], dtype=np.int16)):
+            with pytest.raises(RuntimeError, match="CUDA device"):      # past its checks
+                call(x)
+        with pytest.raises(ValueError, match="must have shape"):
+            call(np.array([1, 0, 2]))
+        with pytest.raises(TypeError, match="must contain integers"):
+            call(np.array([1.0, 0.0]))
+    for x in (np.int64(1), 1):
+        with pytest.raises(RuntimeError, match="CUDA device"):
+            c.extend(x)
