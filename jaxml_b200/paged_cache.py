@@ -65,7 +65,7 @@ class PagedKVCache:
         head_dim = normalize_count("head_dim", head_dim)
         if head_dim not in HEAD_DIMS:
             raise NotImplementedError(f"PagedKVCache takes a head_dim of 64, 128 or 256, got {head_dim}.")
-        if status is None:
+        if status is None and isinstance(pages, torch.Tensor):
             status = torch.zeros(1, dtype=torch.int32, device=pages.device)
         for name, t, dtype, ndim in (("pages", pages, torch.uint8, 4), ("table", table, torch.int32, 2),
                                      ("lengths", lengths, torch.int32, 1), ("counts", counts, torch.int32, 1),

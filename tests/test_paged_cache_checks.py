@@ -317,3 +317,9 @@ def test_numpy_row_vectors_are_taken_as_lists_are():
     for x in (np.int64(1), 1):
         with pytest.raises(RuntimeError, match="CUDA device"):
             c.extend(x)
+
+
+def test_pages_that_are_no_tensor_are_refused():
+    for pages in (None, np.zeros((1, 4, 2, block_bytes(64)), dtype=np.uint8)):
+        with pytest.raises(TypeError, match="pages must be a 4D torch.uint8 tensor"):
+            _cpu_cache(pages=pages)
