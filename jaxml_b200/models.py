@@ -217,7 +217,7 @@ class _DecoderWithHead:
         cache.check()
         try:
             h, _, states, _ = layered_forward(
-                self.family, cfg, self.dtype, body, ids.to(dev), mask.to(dev),
+                self.family, cfg, self.dtype, body, ids.to(dev), None,      # the cache's counts are the mask
                 cache.position_ids(ids.shape[1]) if cfg.use_rope else None,
                 tuple(cache.layer(i) for i in range(cfg.num_layers)), None, self.__dict__["_layered_cache"]["rope"])
         except BaseException:

@@ -1083,10 +1083,15 @@ class Attention(Block):
             raise ValueError(f"sliding_window must be positive when set, got {window}.")
         B, S = hidden.shape[:2]
         if isinstance(kv_cache, PagedKVLayer):
-            # the cache's counts say which tokens of the call are there; a mask would say it again
             if output_attentions:
                 raise NotImplementedError("output_attentions is not implemented over a paged 4-bit cache.")
             _need_cuda("Attention", q, k, v)
+            if attention_mask is not None:
+                # the cache's counts say which tokens of the call are there; a mask can only say it again
+                mask = attention_mask if isinstance(attention_mask, torch.Tensor) else torch.as_tensor(attention_mask)
+                if tuple(mask.shape) != (B, S) or not torch.equal(
+                        _prefix_lengths(mask.to(hidden.device)), kv_cache.cache.counts):
+                    raise ValueError("attention_mask must hold the cache's counts of this call's tokens, over a paged 4-bit cache.")
             out = kv_cache.update_and_attend(q.to(self.dtype), k.to(self.dtype), v.to(self.dtype),
                                              float(self.attn_scale), window or None)
             kv_cache.cache.check()

@@ -827,3 +827,26 @@ def test_lengths_that_no_row_can_have(length):
     if length > 0:
         c.check()
         assert c.lengths.tolist() == [100, 0, 256] and (c.table[1] == -1).all() and int(c.refs.sum()) == 6
+
+
+def test_a_mask_that_disagrees_with_the_counts_is_refused():
+    """A block over a layer of the cache takes the call's tokens from its counts: a mask may say the same, nothing else."""
+    from jaxml_b200 import ModelConfig
+    from jaxml_b200.nn import Attention
+
+    cfg = ModelConfig(head_dim=64, hidden_size=256, num_heads=4, num_kv_heads=2, num_layers=1, max_position_embeddings=256,
+                      vocab_size=512)
+    block = Attention(cfg, dtype=torch.float32)
+    x = _rand((2, 5, 256), torch.float32, 1).cuda()
+    variables = block.init(0, x)
+    c = _cache(1, 4, 2, 128, 2, 64)
+    c.extend([5, 3])
+    pages = c.pages.clone()
+    for bad in (torch.ones(2, 5, dtype=torch.bool), torch.tensor([[1, 1, 1, 1, 1], [1, 1, 0, 0, 0]]).cuda()):
+        with pytest.raises(ValueError, match="attention_mask must hold the cache's counts"):
+            block.apply(variables, x, attention_mask=bad, kv_cache=c.layer(0))
+    assert torch.equal(c.pages, pages)
+    mask = torch.tensor([[1, 1, 1, 1, 1], [1, 1, 1, 0, 0]])
+    a = block.apply(variables, x, attention_mask=mask, kv_cache=c.layer(0)).attention_output
+    b = block.apply(variables, x, kv_cache=c.layer(0)).attention_output
+    assert torch.equal(a, b)
