@@ -850,3 +850,22 @@ def test_a_mask_that_disagrees_with_the_counts_is_refused():
     a = block.apply(variables, x, attention_mask=mask, kv_cache=c.layer(0)).attention_output
     b = block.apply(variables, x, kv_cache=c.layer(0)).attention_output
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,hd", [(80, 64), (130, 64), (100, 256)])
+def test_many_short_chunks_in_tiles_of_128(rows, hd):
+    """More (row, query tile, KV head) segments than groups are taken for (512), so that several of them come to a CTA of the
+    kernel for tiles of 128 rows at every head size."""
+    rng = random.Random(rows)
+    S, kv, heads = 9, 4, 8
+    assert rows * -(-S * heads // kv // 16) * kv > 512
+    counts = [rng.choice([0, 1, 5, 9, 9]) for _ in range(rows)]
+    lens = [n + rng.choice([0, 0, 3, 55, 60, 64, 200]) for n in counts]
+    c, ks, vs = _filled(rows, lens, counts, kv, hd, seed=rows)
+    q = _rand((rows, S, heads, hd), torch.bfloat16, 5, 1.5)
+    for r, n in enumerate(counts):
+        q[r, n:] = float("nan")
+    for window in (0, 7):
+        got = c.attend(0, q.cuda(), sliding_window=window or None)
+        _check_attend(got, q, ks, vs, lens, counts, hd ** -0.5, window)
+    c.check()
