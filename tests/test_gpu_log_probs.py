@@ -204,3 +204,20 @@ def test_unsigned_ids_do_not_wrap():
             got = _run(x, torch.from_numpy(np.array([big, 4], dtype=dtype)).to(dev), 0).log_probs
             assert torch.isnan(got[0]) and got[1] == want[1], (dtype, dev)
             assert torch.equal(_run(x, torch.from_numpy(np.array([3, 4], dtype=dtype)).to(dev), 0).log_probs, want)
+
+
+def test_logits_of_more_than_32_bits():
+    """Rows that begin more than 2^31 elements into the logits."""
+    N, V = 8300, 262144
+    g = torch.Generator().manual_seed(0)
+    x = torch.zeros(N, V, dtype=torch.bfloat16, device="cuda")
+    some = torch.tensor([0, 1, 4200, 8192, 8298, 8299])
+    rows = (torch.randn(len(some), V, generator=g) * 4).to(torch.bfloat16)
+    x[some.cuda()] = rows.cuda()
+    ids = torch.randint(0, V, (N,), generator=g, dtype=torch.int32)
+    got = _run(x, ids.cuda(), 5)
+    _check(rows, ids[some], 5, [t.cpu()[some] for t in got])
+    flat = torch.ones(N, dtype=torch.bool)
+    flat[some] = False
+    assert (got.top_ids.cpu()[flat] == torch.arange(5)).all()
+    assert (got.log_probs.cpu()[flat] + math.log(V)).abs().max() <= 2.0 ** -22 * (1 + math.log(V)) + (V / 128 + 64) * 2.0 ** -24

@@ -869,3 +869,39 @@ def test_many_short_chunks_in_tiles_of_128(rows, hd):
         got = c.attend(0, q.cuda(), sliding_window=window or None)
         _check_attend(got, q, ks, vs, lens, counts, hd ** -0.5, window)
     c.check()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_pool_of_more_than_32_bits(dtype):
+    """Pages that lie more than 2^32 bytes into the pool: written, read, attended to by each kernel, copied on a write."""
+    heads, hd, layers, pages = 8, 256, 2, 20000
+    c = _cache(layers, pages, 2, 600 * PAGE, heads, hd)
+    assert c.pages.numel() > 2 ** 32 + 2 ** 30
+    c.refs[:pages - 40] = 1                     # held by others: the rows' pages are the last ones
+    n = [150, 130]
+    k, v = _rand((2, max(n), heads, hd), dtype, 1), _rand((2, max(n), heads, hd), dtype, 2)
+    c.extend(n)
+    c.append(layers - 1, k.cuda(), v.cuda())
+    c.check()
+    assert int(c.table[c.table >= 0].min()) >= pages - 40
+    for x, got in zip((k, v), c.read(layers - 1, 0, max(n), dtype=torch.float32)):
+        for r in range(2):
+            assert torch.equal(got[r, :n[r]].double().cpu(), K.dequantised(x[r, :n[r]]))
+    ks, vs = _Rows([k[r, :n[r]] for r in range(2)]), _Rows([v[r, :n[r]] for r in range(2)])
+    last = _rand((2, max(n), heads, hd), dtype, 3)
+    _check_attend(c.attend(layers - 1, last.cuda()), last, ks, vs, n, n, hd ** -0.5)
+    c.rollback(1)
+    c.extend(1)
+    c.append(layers - 1, *(torch.stack([x[r, n[r] - 1:n[r]] for r in range(2)]).cuda() for x in (k, v)))
+    q = _rand((2, 1, 2 * heads, hd), dtype, 4)
+    _check_attend(c.attend(layers - 1, q.cuda()), q, ks, vs, n, [1, 1], hd ** -0.5)
+    _check_attend(c.attend(layers - 1, q.cuda(), sliding_window=100), q, ks, vs, n, [1, 1], hd ** -0.5, 100)
+    before = c.read(layers - 1, 0, n[0])[0][0]
+    c.fork([0, 0])
+    c.extend(1)
+    c.append(layers - 1, torch.zeros(2, 1, heads, hd, dtype=dtype, device="cuda"),
+             torch.zeros(2, 1, heads, hd, dtype=dtype, device="cuda"))
+    c.check()
+    assert c.table[0, 2] != c.table[1, 2]
+    got = c.read(layers - 1, 0, n[0] + 1)[0]
+    assert all(torch.equal(got[r, :n[0]], before) and (got[r, n[0]] == 0).all() for r in range(2))
