@@ -12,8 +12,10 @@ cache holds all layers in one pool of 64-token pages and changes in place, so th
     cache.rollback(n)                       # drafted tokens that were not taken
     cache.free(rows); cache.compact()       # finished rows; used pages to the front of the pool
 
-All state (page table, lengths, reference counts) is on the device and every call is a kernel launch or two on the
-current stream without a host synchronisation, so the loop can be captured in a CUDA graph.  Page choices are
+All state (page table, lengths, reference counts) is on the device and every call of the loop is a kernel launch or two
+on the current stream without a host synchronisation (given ints, or tensors on the cache's device), so the loop can be
+captured in a CUDA graph.  ``check`` and ``resize`` read the device, and so do the blocks and models that take this cache
+(``nn.Attention``, ``apply``): those are not captured.  Page choices are
 deterministic (lowest free page, rows in order).  What only the device can see (a full pool, a row past ``max_seq_len``,
 a parent out of range) sets a status word that ``check`` raises; such an ``extend`` changes nothing and gives every row
 zero tokens of the current call.
