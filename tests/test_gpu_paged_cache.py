@@ -905,3 +905,42 @@ def test_a_pool_of_more_than_32_bits(dtype):
     assert c.table[0, 2] != c.table[1, 2]
     got = c.read(layers - 1, 0, n[0] + 1)[0]
     assert all(torch.equal(got[r, :n[0]], before) and (got[r, n[0]] == 0).all() for r in range(2))
+
+
+def test_a_captured_change_of_rows_gives_the_eager_results():
+    """free, compact, extend, append and attend in one graph: each replay frees and admits the rows that its inputs name."""
+    def state():
+        c = _cache(2, 40, 4, 300, 2, 64, fill=0xFF)
+        c.extend([60, 3, 200, 130])
+        x = _rand((4, 200, 2, 64), torch.bfloat16, 1).cuda()
+        for layer in range(2):
+            c.append(layer, x, x)
+        return c
+
+    def turn(c, gone, admit, kv, q):
+        c.free(gone)
+        used = c.compact()
+        c.extend(admit)
+        c.append(1, kv, kv)
+        return used, c.attend(1, q)
+
+    gone, admit = torch.zeros(4, dtype=torch.bool, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    kv, q = torch.zeros(4, 70, 2, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(4, 70, 4, 64, dtype=torch.bfloat16, device="cuda")
+    a, b = state(), state()
+    turn(b, gone, admit, kv, q)                 # loads what is loaded once
+    b = state()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = turn(b, gone, admit, kv, q)
+    for i in range(8):
+        gone.copy_(torch.tensor([(i + r) % 3 == 0 for r in range(4)]))
+        admit.copy_(torch.tensor([70 if (i + r) % 3 == 0 else 1 for r in range(4)]))
+        kv.copy_(_rand((4, 70, 2, 64), torch.bfloat16, 10 + i))
+        q.copy_(_rand((4, 70, 4, 64), torch.bfloat16, 40 + i))
+        want = turn(a, gone, admit, kv, q)
+        graph.replay()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), i
+        assert all(torch.equal(getattr(a, x), getattr(b, x)) for x in ("table", "lengths", "counts", "refs")), i
+    a.check()
+    b.check()
