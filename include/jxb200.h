@@ -519,7 +519,8 @@ int jx_kv4_read(const jx_kv4_cache* cache, int layer, const int* start, int star
                 void* stream);
 /* Attention of queries [num_rows, S, Hq, hd] (element strides; last axis dense) over a layer's pages.  Query i <
  * counts[r] stands at position p = lengths[r] - counts[r] + i and sees positions <= p, with window > 0 those above p -
- * window; float32 softmax of scale * q.k.  Query head h reads KV head h / (Hq / num_kv_heads).  out: dense
+ * window; float32 softmax of scale * q.k (queries of magnitude below 2^115: partial sums of their products
+ * are not to overflow).  Query head h reads KV head h / (Hq / num_kv_heads).  out: dense
  * [num_rows, S, Hq, hd]; rows of queries behind counts[r] are zero.  ws: jx_kv4_attend_workspace bytes (NULL where that
  * is 0), 16-byte aligned, used by this call alone until it has finished. */
 int jx_kv4_attend_workspace(const jx_kv4_cache* cache, int S, int Hq, int dtype, long long* bytes);

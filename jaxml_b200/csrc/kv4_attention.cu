@@ -13,7 +13,8 @@
 // What bounds a decode step is instructions, not bytes: a page of 64 keys is 9 KB and the multiprocessor has some 400
 // cycles for it at the card's bandwidth.  So with one tile of 8 rows:
 //   K   the k side of an MMA pair is one group of 32 channels, fed with 128 + u; the accumulator starts at
-//       -136 sum q of the group and its result times the key's scale is added up in float32;
+//       -136 sum q of the group and its result times the key's scale is added up in float32 (finite while |q| < 2^115:
+//       136 * 32 < 2^13);
 //   V   one fused multiply-add a pair gives code times scale exactly (scaled2).
 // With more rows K is made exact the same way; float32 results need its codes exact before the product.
 //

@@ -23,8 +23,8 @@ zero tokens of the current call.
 The format is 4.5 bits a value: 4-bit integers -7..7 with one scale of 4 significant bits for every 32 neighbouring
 channels of a token (``include/jxb200.h``).  A group with a non-finite value, or one of magnitude 2^122 or more, decodes
 to NaN.  Calls on one cache that change it must be ordered on the device like writes to any tensor; ``attend`` and
-``read`` may run at the same time.  ``lengths`` and ``counts`` may be read, not written, and be given to ``extend`` and
-``rollback``; other arguments must not lie in the cache's own tensors.
+``read`` may run at the same time.  ``lengths`` and ``counts`` may be read, not written, and be given to ``extend``,
+``rollback`` and ``read``; ``fork`` and ``free`` take no argument that lies in the cache's own tensors.
 """
 from __future__ import annotations
 
@@ -245,8 +245,9 @@ class PagedKVCache:
         """Causal attention of the call's queries [rows, S, heads, hd] over a layer's pages, this call's tokens among
         them: query i of row r stands at position ``lengths[r] - counts[r] + i`` and, with a sliding window, sees that
         many positions back, its own among them.  float32 softmax of ``scale`` (``hd ** -0.5`` by default) times q.k;
-        heads must be a multiple of the KV heads.  Returns [rows, S, heads, hd] in q's dtype, zeros for the padding
-        behind a row's ``counts[r]`` queries."""
+        heads must be a multiple of the KV heads, and queries below 2^115 in magnitude (their products' partial sums are
+        in float32).  Returns [rows, S, heads, hd] in q's dtype, zeros for the padding behind a row's ``counts[r]``
+        queries."""
         layer = self._layer(layer)
         q = self._states("q", q, None)
         S, heads = q.shape[1], q.shape[2]
